@@ -22,6 +22,7 @@ OVERFLOW_MODES = {'NONE': 0, 'WRAP': 1, 'SAT': 2, 'SAT_SYM': 3}
 FLAG_TRAINING = 1
 FLAG_ZERO_NONPOS = 2
 FLAG_ABSMAX_ACCUMULATE = 4
+ADAMW_BLOCK = 256  # HGQ_ADAMW_BLOCK
 
 
 class HGQError(RuntimeError):
@@ -121,6 +122,12 @@ SIGNATURES: dict[str, tuple] = {
         [c_void_p, c_int, c_int, c_int, c_void_p] + [c_int] * 11 + [c_void_p, c_int64, c_double, c_double, c_double, c_void_p]
         + [c_void_p] * 7,
     ),
+    'hgq_adamw_workspace': (c_size_t, [c_int64]),
+    'hgq_adamw_step': (
+        c_int,
+        [c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_double, c_double,
+         c_double, c_double, c_double, c_double, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p],
+    ),
     'hgq_adam_step': (c_int, [c_void_p] * 7 + [c_int64] + [c_float] * 5 + [c_void_p, c_void_p]),
     'hgq_peer_exchange_bytes': (c_size_t, [c_int64]),
     'hgq_peer_buffer_create': (c_int, [c_size_t, c_void_p, c_void_p]),
@@ -163,6 +170,13 @@ class EbopsDenseDesc(ctypes.Structure):
                 ('n_bias', c_int64), ('out_size', ctypes.c_double), ('scale', ctypes.c_double), ('beta', c_void_p),
                 ('ebops', c_void_p), ('ebops_f', c_void_p), ('loss', c_void_p), ('d_bw_in', c_void_p), ('d_bw_w', c_void_p),
                 ('d_bw_bias', c_void_p)]
+
+
+class AdamWTensor(ctypes.Structure):
+    """hgq_adamw_tensor of include/hgq_b200.h."""
+
+    _fields_ = [('w', c_void_p), ('master', c_void_p), ('n', c_int64), ('offset', c_int64), ('decay', ctypes.c_double),
+                ('lo', c_float), ('hi', c_float), ('l1', c_float), ('w_type', ctypes.c_int32)]
 
 
 class ChainLayer(ctypes.Structure):

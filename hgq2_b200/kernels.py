@@ -6,10 +6,14 @@ These functions are the seam between the Python mirror of the reference interfac
 
 from __future__ import annotations
 
+from array import array
+
 import torch
 
 from . import _lib
 from ._lib import FLAG_ABSMAX_ACCUMULATE, FLAG_TRAINING, FLAG_ZERO_NONPOS, OVERFLOW_MODES, ROUND_MODES, check, lib, ptr, require_cuda, stream_handle
+
+ELEMENT_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}  # HGQ_TYPE_*
 
 _workspaces: dict[tuple[int, int, int], torch.Tensor] = {}
 
@@ -646,3 +650,59 @@ def weights_forward(weights_dev, n_weights: int, max_n: int, slots_dev) -> None:
 def weights_backward(weights_dev, n_weights: int, max_n: int, slots_dev) -> None:
     with torch.cuda.device(slots_dev.device):
         check(lib().hgq_weights_backward(ptr(weights_dev), n_weights, max_n, ptr(slots_dev), stream_handle()), 'hgq_weights_backward')
+
+
+# ---- operators that take fp32, bf16 and fp16 -----------------------------------------------------------------------------
+def element_type(*tensors) -> int:
+    """HGQ_TYPE_* of tensors that have to agree in type and device."""
+    first = tensors[0]
+    for t in tensors:
+        if t is not None and (t.dtype != first.dtype or t.device != first.device):
+            raise ValueError(f'expected {first.dtype} on {first.device}, got {t.dtype} on {t.device}')
+    kind = ELEMENT_TYPES.get(first.dtype)
+    if kind is None:
+        raise ValueError(f'{first.dtype} is not supported: fp32, bf16 and fp16 are')
+    return kind
+
+
+def adamw_step(opt, grads, grad_scale: float = 1.0) -> None:
+    """One AdamW step of ``opt`` (a ``train.FusedAdamW``) from one gradient tensor or None per parameter."""
+    dev = opt.m.device
+    grads = list(grads)
+    n = len(opt.tensors)
+    if len(grads) != n:
+        raise ValueError(f'{len(grads)} gradients for {n} tensors')
+    present = [g for g in grads if g is not None]
+    if not present:
+        raise ValueError('no gradients: every entry is None')
+    # checks over whole lists: a model has hundreds of tensors and this loop is on the path of every step
+    T = torch.Tensor
+    if set(map(T.get_device, present)) != {dev.index}:
+        raise ValueError(f'gradients must be on {dev}')
+    shapes = opt._shapes
+    if len(present) < n:
+        shapes = [s for s, g in zip(shapes, grads) if g is not None]
+    if [g.shape for g in present] != shapes:
+        raise ValueError('a gradient does not have the shape of its tensor')
+    dtypes = [g.dtype for g in present]
+    unknown = set(dtypes) - ELEMENT_TYPES.keys()
+    if unknown:
+        raise ValueError(f'gradients of {unknown} are not supported: fp32, bf16 and fp16 are')
+    if not all(map(T.is_contiguous, present)):
+        present = [g.contiguous() for g in present]  # kept alive until the launch below
+    ptrs = list(map(T.data_ptr, present))
+    kinds = [ELEMENT_TYPES[d] for d in dtypes]
+    if len(present) < n:
+        each = iter(zip(ptrs, kinds))
+        ptrs, kinds = zip(*[(0, 0) if g is None else next(each) for g in grads])
+    addresses, types = array('Q', ptrs), bytes(kinds)
+    clip = opt.global_clipnorm or 0.0
+    eight = opt.state_bits == 8
+    with torch.cuda.device(dev):
+        ws = workspace(lib().hgq_adamw_workspace(n), dev, slot=7) if clip else None
+        st = lib().hgq_adamw_step(
+            ptr(opt._table), n, ptr(opt._blocks), opt._first_block.ctypes.data, addresses.buffer_info()[0], types, opt.state_bits,
+            ptr(opt.m), ptr(opt.r if eight else opt.v), ptr(opt.m_scale) if eight else None, ptr(opt.r_scale) if eight else None,
+            opt.lr, opt.b1, opt.b2, opt.eps, grad_scale, clip, ptr(opt.step_count), ptr(opt._ticket), ptr(ws),
+            ws.numel() if ws is not None else 0, stream_handle())
+    check(st, 'hgq_adamw_step')

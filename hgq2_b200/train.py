@@ -17,15 +17,42 @@ from __future__ import annotations
 import math
 import os
 
+import numpy as np
 import torch
 import torch.distributed as dist
 
-from . import _lib
+from . import _lib, kernels
 from .backend import Layer, Variable, join_bookkeeping
 from .constraints import Constant as ConstantConstraint
 from .constraints import Max, Min, MinMax
 from .quantizer.internal import fixed_point_quantizer as _fpq
 from .regularizers import MonoL1
+
+
+def _bounds(v: Variable) -> tuple[float, float]:
+    """The clamp a variable's constraint is, as (lowest, highest) value."""
+    c = v.constraint
+    if c is None:
+        return -math.inf, math.inf
+    if isinstance(c, MinMax):
+        return c.min_value, c.max_value
+    if isinstance(c, Min):
+        return c.min_value, math.inf
+    if isinstance(c, Max):
+        return -math.inf, c.max_value
+    if isinstance(c, ConstantConstraint):
+        return c.value, c.value
+    raise NotImplementedError(f'constraint {type(c).__name__} on {v.path} cannot be fused')
+
+
+def _l1(v: Variable) -> float:
+    """The constant gradient a variable's regularizer adds."""
+    r = v.regularizer
+    if r is None:
+        return 0.0
+    if isinstance(r, MonoL1):
+        return r.l1
+    raise NotImplementedError(f'regularizer {type(r).__name__} on {v.path} cannot be fused')
 
 
 class FlatState:
@@ -60,26 +87,8 @@ class FlatState:
         for v, o, n in zip(self.variables, self.offsets, sizes):
             v.value.data = self.params[o:o + n].view(v.value.shape)
             v.value.grad = self.grads[o:o + n].view(v.value.shape)
-            c = v.constraint
-            if c is None:
-                pass
-            elif isinstance(c, MinMax):
-                lo[o:o + n], hi[o:o + n] = c.min_value, c.max_value
-            elif isinstance(c, Min):
-                lo[o:o + n] = c.min_value
-            elif isinstance(c, Max):
-                hi[o:o + n] = c.max_value
-            elif isinstance(c, ConstantConstraint):
-                lo[o:o + n] = hi[o:o + n] = c.value
-            else:
-                raise NotImplementedError(f'constraint {type(c).__name__} on {v.path} cannot be fused')
-            r = v.regularizer
-            if r is None:
-                pass
-            elif isinstance(r, MonoL1):
-                l1[o:o + n] = r.l1
-            else:
-                raise NotImplementedError(f'regularizer {type(r).__name__} on {v.path} cannot be fused')
+            lo[o:o + n], hi[o:o + n] = _bounds(v)
+            l1[o:o + n] = _l1(v)
         self.lo, self.hi, self.l1 = lo.to(dev), hi.to(dev), l1.to(dev)
 
     def zero_grad(self) -> None:
@@ -134,6 +143,131 @@ class FusedAdam:
                 _lib.stream_handle(),
             )
         _lib.check(st, 'hgq_adam_step_peers')
+
+
+class FusedAdamW:
+    """AdamW over a list of tensors in one launch (two with clipping), with its moments in 32 or in 8 bits.
+
+    ``tensors``: a ``FlatState``, or a sequence of ``Variable`` s and / or tensors (contiguous, on one GPU, no two of them over
+    the same memory).  A ``Variable``'s constraint and ``MonoL1`` regularizer are applied in the same pass.  bf16 and fp16
+    tensors are updated through an fp32 copy that the optimizer keeps (``masters``); the tensor gets its rounded value.
+
+    The rule is Keras' AdamW: ``w`` is first scaled by ``1 - learning_rate * weight_decay``, then takes Adam's step;
+    ``global_clipnorm`` scales all gradients so that their common 2-norm is at most that (a norm that is not finite reaches
+    every weight, as in Keras).  ``weight_decay`` is one number, or one per tensor (0 for biases and bitwidths, say).
+
+    ``state_bits=8`` keeps the moments as e4m3 codes with an fp32 scale per 256 elements of a tensor: ``m`` (times ``m_scale``)
+    and ``r`` (times ``r_scale``), the root of the second moment -- 2 bytes per weight instead of 8.  ``state_bits=32`` keeps
+    fp32 ``m`` and ``v``.  The state arrays are flat; tensor ``i`` starts at ``offsets[i]``, a multiple of 256."""
+
+    def __init__(self, tensors, learning_rate=1e-3, beta_1=0.9, beta_2=0.999, epsilon=1e-7, weight_decay=0.004,
+                 global_clipnorm: float | None = None, state_bits: int = 32):
+        items = list(tensors.variables if isinstance(tensors, FlatState) else tensors)
+        if not items:
+            raise ValueError('no tensors to optimize')
+        if state_bits not in (8, 32):
+            raise ValueError(f'state_bits must be 8 or 32, got {state_bits}')
+        if global_clipnorm is not None and not global_clipnorm > 0:
+            raise ValueError(f'global_clipnorm must be positive, got {global_clipnorm}')
+        if not (0 <= beta_1 < 1 and 0 <= beta_2 < 1):
+            raise ValueError(f'beta_1 and beta_2 must lie in [0, 1), got {beta_1} and {beta_2}')
+        decays = [float(d) for d in weight_decay] if hasattr(weight_decay, '__len__') else [float(weight_decay)] * len(items)
+        if len(decays) != len(items):
+            raise ValueError(f'{len(decays)} weight decays for {len(items)} tensors')
+        self.lr, self.b1, self.b2, self.eps = learning_rate, beta_1, beta_2, epsilon
+        self.global_clipnorm, self.state_bits = global_clipnorm, state_bits
+        self._items = items
+        self.tensors = [v.value.data if isinstance(v, Variable) else v.detach() for v in items]
+        dev = self.tensors[0].device
+        _lib.require_cuda(*self.tensors)
+        spans = []
+        for i, w in enumerate(self.tensors):
+            if w.device != dev:
+                raise ValueError(f'tensor {i} is on {w.device}, tensor 0 on {dev}')
+            if w.dtype not in kernels.ELEMENT_TYPES:
+                raise ValueError(f'tensor {i} is {w.dtype}; fp32, bf16 and fp16 are supported')
+            if not w.is_contiguous():
+                raise ValueError(f'tensor {i} is not contiguous')
+            if w.numel():
+                spans.append((w.data_ptr(), w.data_ptr() + w.numel() * w.element_size(), i))
+        spans.sort()
+        for (_, end, i), (start, _, j) in zip(spans, spans[1:]):
+            if start < end:
+                raise ValueError(f'tensors {min(i, j)} and {max(i, j)} share memory')
+        self.masters = [None if w.dtype == torch.float32 else w.float() for w in self.tensors]
+        block = _lib.ADAMW_BLOCK
+        self._numels, self._shapes = [w.numel() for w in self.tensors], [w.shape for w in self.tensors]
+        counts = [-(-n // block) for n in self._numels]
+        first = np.zeros(len(items) + 1, dtype=np.int64)
+        np.cumsum(counts, out=first[1:])
+        self._first_block = first
+        self.offsets = [int(f) * block for f in first[:-1]]
+        total = int(first[-1]) * block
+        table = (_lib.AdamWTensor * len(items))()
+        for i, (t, v) in enumerate(zip(table, items)):
+            w, master = self.tensors[i], self.masters[i]
+            t.w, t.master, t.n, t.offset = w.data_ptr(), None if master is None else master.data_ptr(), w.numel(), self.offsets[i]
+            t.decay, t.w_type = decays[i], kernels.ELEMENT_TYPES[w.dtype]
+            t.lo, t.hi, t.l1 = (*_bounds(v), _l1(v)) if isinstance(v, Variable) else (-math.inf, math.inf, 0.0)
+        raw = np.frombuffer(table, dtype=np.uint8).copy()
+        pairs = np.empty((int(first[-1]), 2), dtype=np.int32)
+        pairs[:, 0] = np.repeat(np.arange(len(items), dtype=np.int32), counts)
+        pairs[:, 1] = np.arange(int(first[-1])) - np.repeat(first[:-1], counts)
+        self._table, self._blocks = torch.from_numpy(raw).to(dev), torch.from_numpy(pairs).to(dev)
+        kind = torch.float32 if state_bits == 32 else torch.float8_e4m3fn
+        self.m = torch.zeros(total, dtype=torch.uint8 if state_bits == 8 else kind, device=dev).view(kind)
+        second = torch.zeros_like(self.m.view(torch.uint8) if state_bits == 8 else self.m).view(kind)
+        if state_bits == 8:
+            self.r = second
+            self.m_scale = torch.zeros(total // block, dtype=torch.float32, device=dev)
+            self.r_scale = torch.zeros_like(self.m_scale)
+        else:
+            self.v = second
+        self.step_count = torch.zeros((), dtype=torch.int64, device=dev)
+        self._ticket = torch.zeros((), dtype=torch.int32, device=dev)
+
+    def step(self, grads=None, grad_scale: float = 1.0) -> None:
+        """One update.  ``grads``: one tensor (fp32, bf16 or fp16, of the parameter's shape) or None per parameter, None leaving
+        that parameter and its moments as they are; by default the ``.grad`` of each."""
+        if grads is None:
+            grads = [v.value.grad if isinstance(v, Variable) else v.grad for v in self._items]
+        kernels.adamw_step(self, grads, grad_scale)
+
+    def moments(self, i: int) -> tuple[torch.Tensor, torch.Tensor]:
+        """The fp32 values of tensor ``i``'s first and second moment (for inspection; 8-bit states are decoded)."""
+        a, b = self.offsets[i], int(self._first_block[i + 1]) * _lib.ADAMW_BLOCK
+        shape = self.tensors[i].shape
+        if self.state_bits == 32:
+            m, v = self.m[a:b], self.v[a:b]
+        else:
+            s = slice(a // _lib.ADAMW_BLOCK, b // _lib.ADAMW_BLOCK)
+            m, r = ((c[a:b].float().view(-1, _lib.ADAMW_BLOCK) * k[s, None]).view(-1)
+                    for c, k in ((self.m, self.m_scale), (self.r, self.r_scale)))
+            v = r * r
+        n = self._numels[i]
+        return m[:n].clone().view(shape), v[:n].clone().view(shape)
+
+    def _state_arrays(self) -> dict:
+        names = ('m', 'v') if self.state_bits == 32 else ('m', 'r', 'm_scale', 'r_scale')
+        arrays = {name: getattr(self, name) for name in names}
+        arrays['step_count'] = self.step_count
+        arrays.update({f'master_{i}': w for i, w in enumerate(self.masters) if w is not None})
+        return arrays
+
+    def state_dict(self) -> dict:
+        """Copies of the state arrays (codes as bytes) for a checkpoint."""
+        return {k: (a.view(torch.uint8) if a.dtype == torch.float8_e4m3fn else a).clone() for k, a in self._state_arrays().items()}
+
+    def load_state_dict(self, state: dict) -> None:
+        """Take over the arrays of ``state_dict`` of an optimizer over tensors of the same sizes and types."""
+        own = self._state_arrays()
+        if set(own) != set(state):
+            raise ValueError(f'the state has {sorted(state)}, this optimizer keeps {sorted(own)}')
+        for k, a in own.items():
+            if tuple(state[k].shape) != tuple(a.shape):
+                raise ValueError(f'{k} has shape {tuple(state[k].shape)}, expected {tuple(a.shape)}')
+        for k, a in own.items():
+            (a.view(torch.uint8) if a.dtype == torch.float8_e4m3fn else a).copy_(state[k])
 
 
 class PeerExchange:
@@ -275,8 +409,12 @@ class Trainer:
     the per-kernel launch and Python cost that dominates the small models.
     """
 
-    def __init__(self, model: Layer, loss_fn, learning_rate=1e-3, dp: DataParallel | None = None, engine: bool | None = None):
-        """``engine``: run forward and backward through the static step plan of ``hgq2_b200.engine`` (batched bitwidth
+    def __init__(self, model: Layer, loss_fn, learning_rate=1e-3, dp: DataParallel | None = None, engine: bool | None = None,
+                 optimizer=None):
+        """``optimizer``: a callable that makes the optimizer from the trainer's ``FlatState`` (``lambda state: FusedAdamW(state,
+        global_clipnorm=1.0)``); None: ``FusedAdam`` at ``learning_rate``.
+
+        ``engine``: run forward and backward through the static step plan of ``hgq2_b200.engine`` (batched bitwidth
         arithmetic, no autograd graph).  None (default): use it when it covers the model, else the autograd path; True:
         require it (raises ``engine.Unsupported`` otherwise); False: always the autograd path.  The environment variable
         ``HGQ_ENGINE=0`` turns the default off."""
@@ -284,7 +422,7 @@ class Trainer:
         self.loss_fn = loss_fn
         self.dp = dp
         self.state = FlatState(model)
-        self.opt = FusedAdam(self.state, learning_rate=learning_rate)
+        self.opt = FusedAdam(self.state, learning_rate=learning_rate) if optimizer is None else optimizer(self.state)
         self.engine = None
         self.engine_refusal = None  # why the static step plan is not in use (None: it is, or it was not asked for)
         if engine is None:
@@ -302,7 +440,7 @@ class Trainer:
         # gradient exchange over peer memory inside the optimizer kernel (one node, NCCL process group on GPUs);
         # HGQ_PEER_EXCHANGE=0 keeps the NCCL all-reduce
         self.peers = None
-        if (dp is not None and dp.world > 1 and self.state.params.is_cuda and dist.get_backend(dp.group) == 'nccl'
+        if (optimizer is None and dp is not None and dp.world > 1 and self.state.params.is_cuda and dist.get_backend(dp.group) == 'nccl'
                 and os.environ.get('HGQ_PEER_EXCHANGE', '1') != '0'):
             self.peers = PeerExchange.create(dp, self.state.n, self.state.params.device)
         self._graphs = []      # captured steps, one per set of static input buffers

@@ -417,6 +417,48 @@ int hgq_adam_step(float *w, const float *g, float *m, float *v, const float *lo,
                   const float *l1, int64_t n, float lr, float beta1, float beta2, float eps,
                   float grad_scale, long long *step, void *stream);
 
+/* ---- element types of the entries that take more than fp32 -------------------------------- */
+#define HGQ_TYPE_F32 0
+#define HGQ_TYPE_BF16 1
+#define HGQ_TYPE_F16 2
+
+/* ---- AdamW over a list of tensors ----------------------------------------------------------- */
+
+#define HGQ_ADAMW_BLOCK 256 /* consecutive elements of one tensor that share a scale of the 8-bit states */
+
+/* One tensor of the list; the array lives in DEVICE memory. */
+typedef struct {
+    void *w;        /* the parameter, n elements of w_type                                                       */
+    float *master;  /* its fp32 copy that the update works on, or NULL (then w is fp32 and updated itself)       */
+    int64_t n;
+    int64_t offset; /* of its first element in the state arrays; a multiple of HGQ_ADAMW_BLOCK                   */
+    double decay;   /* decoupled weight decay: w <- w (1 - lr decay) before the step                             */
+    float lo, hi;   /* the constraint of the variable applied after the update (-INFINITY / INFINITY: none)      */
+    float l1;       /* added to the scaled gradient (the MonoL1 regulariser's gradient)                          */
+    int32_t w_type; /* HGQ_TYPE_*                                                                                */
+} hgq_adamw_tensor;
+
+/*
+ * One step over all tensors of a list.  Stands in for keras.optimizers.AdamW with global_clipnorm (Keras, not HGQ2, owns it)
+ * followed by the variables' constraints, like hgq_adam_step does for Adam on one flat bucket.
+ *   g' = (g grad_scale + l1) c,  c = min(clipnorm / |g grad_scale + l1| over all tensors, 1), or 1 if clipnorm <= 0
+ *   m = b1 m + (1 - b1) g';  v = b2 v + (1 - b2) g'^2;  alpha = lr sqrt(1 - b2^t) / (1 - b1^t)
+ *   w = clamp(w (1 - lr decay) - alpha m / (sqrt(v) + eps), lo, hi)
+ * blocks: DEVICE array of (tensor, block of that tensor) pairs of int32, the tensors in order, ceil(n / 256) each; first_block:
+ * HOST array of n_tensors + 1 positions in it.  grads / grad_types: HOST arrays, one entry per tensor (read before the call
+ * returns; a captured graph keeps the addresses); a NULL gradient leaves its tensor and states untouched.
+ * state_bits 32: m and v are fp32 arrays.  state_bits 8: m and v are byte arrays of e4m3 codes, v holding sqrt(v); m_scale and
+ * v_scale have one entry per 256 state elements, and a code stands for code * scale.  The rounding is dithered by a fixed
+ * function of the element's place and t, so steps repeat bit for bit.  A state that is not finite is kept as NaN.
+ * step: device counter (starts at 0), advanced by the call; ticket: a device word that starts at 0 and returns to 0.  Calls that
+ * share states must not overlap.  workspace: hgq_adamw_workspace(n_tensors) bytes, needed when clipnorm > 0.
+ */
+size_t hgq_adamw_workspace(int64_t n_tensors);
+int hgq_adamw_step(const hgq_adamw_tensor *tensors, int64_t n_tensors, const int32_t *blocks, const int64_t *first_block,
+                   const void *const *grads, const uint8_t *grad_types, int state_bits, void *m, void *v, float *m_scale,
+                   float *v_scale, double lr, double beta1, double beta2, double eps, double grad_scale, double clipnorm,
+                   long long *step, unsigned *ticket, void *workspace, size_t workspace_bytes, void *stream);
+
 /* ---- gradient exchange over peer memory, fused with the optimizer update ------------------------ */
 
 /*
