@@ -122,6 +122,28 @@ SIGNATURES: dict[str, tuple] = {
         [c_void_p, c_int, c_int, c_int, c_void_p] + [c_int] * 11 + [c_void_p, c_int64, c_double, c_double, c_double, c_void_p]
         + [c_void_p] * 7,
     ),
+    'hgq_group_norm_workspace': (c_size_t, [c_int64, c_int64, c_int, c_int, c_int, c_int]),
+    'hgq_group_norm_fwd': (
+        c_int,
+        [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int, c_int, c_float, c_int, c_int, c_void_p,
+         c_size_t, c_void_p],
+    ),
+    'hgq_group_norm_bwd': (
+        c_int,
+        [c_void_p] * 9 + [c_int64, c_int64, c_int, c_int, c_int, c_int, c_void_p, c_size_t, c_void_p],
+    ),
+    'hgq_gated_scan_workspace': (c_size_t, [c_int64, c_int64, c_int64]),
+    'hgq_gated_scan_states': (c_int64, [c_int64, c_int64, c_int64]),
+    'hgq_gated_scan_fwd': (
+        c_int,
+        [c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64,
+         c_int64, c_int, c_void_p, c_size_t, c_void_p],
+    ),
+    'hgq_gated_scan_bwd': (
+        c_int,
+        [c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64] + [c_void_p] * 7 +
+        [c_int64, c_int64, c_int64, c_int, c_void_p, c_size_t, c_void_p],
+    ),
     'hgq_adamw_workspace': (c_size_t, [c_int64]),
     'hgq_adamw_step': (
         c_int,

@@ -706,3 +706,151 @@ def adamw_step(opt, grads, grad_scale: float = 1.0) -> None:
             opt.lr, opt.b1, opt.b2, opt.eps, grad_scale, clip, ptr(opt.step_count), ptr(opt._ticket), ptr(ws),
             ws.numel() if ws is not None else 0, stream_handle())
     check(st, 'hgq_adamw_step')
+
+
+ACTIVATIONS = {None: 0, 'relu': 1, 'silu': 2, 'gelu': 3}  # HGQ_ACT_*
+
+
+def _group_norm_args(x, gamma, beta, groups: int, activation):
+    require_cuda(x, gamma, beta)
+    if x.dim() < 2:
+        raise ValueError(f'group normalisation takes [batch, ..., channels], got {tuple(x.shape)}')
+    C = x.shape[-1]
+    if groups <= 0 or C == 0 or C % groups:
+        raise ValueError(f'{groups} groups do not divide {C} channels')
+    for p in (gamma, beta):
+        if p is not None and (p.dtype != torch.float32 or p.shape != (C,) or p.device != x.device):
+            raise ValueError(f'scale and offset must be fp32 of shape ({C},) on {x.device}')
+    if activation not in ACTIVATIONS:
+        raise ValueError(f'activation {activation!r} is not one of {list(ACTIVATIONS)}')
+    B = x.shape[0]
+    return B, (x.numel() // (B * C) if B else 0), C, ACTIVATIONS[activation], element_type(x)
+
+
+def group_norm_fwd(x, gamma, beta, groups: int, eps: float = 1e-3, activation: str | None = None):
+    """act(group norm(x) * gamma + beta) of a channels-last x [batch, ..., channels] (fp32, bf16, fp16; statistics in fp32).
+    ``gamma`` / ``beta``: fp32 [channels] or None; ``activation``: None, 'relu', 'silu' or 'gelu'.  Returns (y, mean, rstd), the
+    latter two fp32 [batch, groups] for ``group_norm_bwd``."""
+    B, S, C, act, kind = _group_norm_args(x, gamma, beta, groups, activation)
+    x = x.contiguous()
+    gamma, beta = (p if p is None else p.contiguous() for p in (gamma, beta))
+    y = torch.empty_like(x)
+    stats = torch.empty((2, B, groups), dtype=torch.float32, device=x.device)
+    mean, rstd = stats[0], stats[1]
+    with torch.cuda.device(x.device):
+        ws = workspace(lib().hgq_group_norm_workspace(B, S, C, groups, kind, 0), x.device, slot=8)
+        st = lib().hgq_group_norm_fwd(ptr(x), ptr(gamma), ptr(beta), ptr(y), ptr(mean), ptr(rstd), B, S, C, groups, eps, act, kind,
+                                      ptr(ws), ws.numel() if ws is not None else 0, stream_handle())
+    check(st, 'hgq_group_norm_fwd')
+    return y, mean, rstd
+
+
+def group_norm_bwd(gy, x, gamma, beta, mean, rstd, groups: int, activation: str | None = None, want_dx: bool = True,
+                   want_params: bool = True, out_dgamma=None, out_dbeta=None):
+    """Gradients of ``group_norm_fwd`` from its inputs and saved statistics: (dx like x, dgamma, dbeta fp32 [channels], written to
+    ``out_dgamma`` / ``out_dbeta`` when given); None for what is not wanted."""
+    B, S, C, act, kind = _group_norm_args(x, gamma, beta, groups, activation)
+    require_cuda(gy, mean, rstd)
+    if gy.shape != x.shape:
+        raise ValueError(f'gradient of shape {tuple(gy.shape)} for an output of shape {tuple(x.shape)}')
+    element_type(x, gy)
+    for s in (mean, rstd):
+        if s.dtype != torch.float32 or s.shape != (B, groups) or not s.is_contiguous() or s.device != x.device:
+            raise ValueError(f'mean and rstd must be contiguous fp32 of shape ({B}, {groups})')
+    for o in (out_dgamma, out_dbeta):
+        if o is not None and (o.dtype != torch.float32 or o.numel() != C or not o.is_contiguous() or o.device != x.device):
+            raise ValueError(f'the gradients of scale and offset go to contiguous fp32 tensors of {C} elements on {x.device}')
+    if not (want_dx or want_params):
+        return None, None, None
+    x, gy = x.contiguous(), gy.contiguous()
+    gamma, beta = (p if p is None else p.contiguous() for p in (gamma, beta))
+    dx = torch.empty_like(x) if want_dx else None
+    dgamma = dbeta = None
+    if want_params:
+        dgamma = out_dgamma if out_dgamma is not None else torch.empty(C, dtype=torch.float32, device=x.device)
+        dbeta = out_dbeta if out_dbeta is not None else torch.empty(C, dtype=torch.float32, device=x.device)
+    with torch.cuda.device(x.device):
+        ws = workspace(lib().hgq_group_norm_workspace(B, S, C, groups, kind, 1), x.device, slot=8)
+        st = lib().hgq_group_norm_bwd(ptr(gy), ptr(x), ptr(gamma), ptr(beta), ptr(mean), ptr(rstd), ptr(dx), ptr(dgamma), ptr(dbeta), B,
+                                      S, C, groups, act, kind, ptr(ws), ws.numel() if ws is not None else 0, stream_handle())
+    check(st, 'hgq_group_norm_bwd')
+    return dx, dgamma, dbeta
+
+
+def _sequences(t, what: str):
+    """A [batch, time, features] tensor whose features are contiguous (any batch and time strides; copied otherwise)."""
+    if t.dim() != 3:
+        raise ValueError(f'{what} must be [batch, time, features], got {tuple(t.shape)}')
+    if t.stride(2) != 1 and t.shape[2] > 1:
+        t = t.contiguous()
+    return t
+
+
+def _scan_args(x, z, h0, lengths):
+    require_cuda(x, z, h0, lengths)
+    x, z = _sequences(x, 'x'), _sequences(z, 'z')
+    if x.shape != z.shape:
+        raise ValueError(f'x is {tuple(x.shape)}, z is {tuple(z.shape)}')
+    kind = element_type(x, z)
+    B, T, D = x.shape
+    if h0 is not None:
+        h0 = _scan_state(h0, B, D, x.device, 'h0')
+    if lengths is not None:
+        if lengths.shape != (B,) or lengths.is_floating_point() or lengths.dtype == torch.bool or lengths.device != x.device:
+            raise ValueError(f'lengths must be {B} whole numbers on {x.device}')
+        if lengths.dtype != torch.int32:
+            lengths = lengths.clamp(0, T).to(torch.int32)
+        lengths = lengths.contiguous()
+    return x, z, h0, lengths, kind, B, T, D
+
+
+def _scan_state(h, B: int, D: int, device, what: str):
+    if h.shape != (B, D) or h.dtype != torch.float32 or h.device != device:
+        raise ValueError(f'{what} must be fp32 of shape ({B}, {D}) on {device}, got {h.dtype} {tuple(h.shape)} on {h.device}')
+    return h.contiguous()
+
+
+def gated_scan_fwd(x, z, h0=None, lengths=None, want_states: bool = False):
+    """h_t = a_t h_{t-1} + (1 - a_t) x_t, a_t = sigmoid(z_t), along axis 1 of x, z [batch, time, features] (fp32, bf16 or fp16; the
+    state is fp32).  ``h0`` [batch, features] fp32; ``lengths`` [batch]: steps of each row of a padded batch (h is 0 behind them).
+    Returns (h, h_last, states): the sequence, the fp32 state behind each row's last step, and what ``gated_scan_bwd`` needs when
+    ``want_states`` (None otherwise)."""
+    x, z, h0, lengths, kind, B, T, D = _scan_args(x, z, h0, lengths)
+    dev = x.device
+    h = torch.empty((B, T, D), dtype=x.dtype, device=dev)
+    h_last = torch.empty((B, D), dtype=torch.float32, device=dev)
+    L = lib()
+    with torch.cuda.device(dev):
+        states = torch.empty(L.hgq_gated_scan_states(B, T, D), dtype=torch.float32, device=dev) if want_states else None
+        ws = workspace(L.hgq_gated_scan_workspace(B, T, D), dev, slot=9)
+        st = L.hgq_gated_scan_fwd(ptr(x), x.stride(0), x.stride(1), ptr(z), z.stride(0), z.stride(1), ptr(h0), ptr(lengths), ptr(h),
+                                  ptr(h_last), ptr(states), B, T, D, kind, ptr(ws), ws.numel() if ws is not None else 0, stream_handle())
+    check(st, 'hgq_gated_scan_fwd')
+    return h, h_last, states
+
+
+def gated_scan_bwd(gh, x, z, h0=None, lengths=None, states=None, g_last=None, want_dh0: bool = False):
+    """Gradients of ``gated_scan_fwd`` from the gradient ``gh`` of h (and ``g_last`` of h_last): (dx, dz, dh0 or None)."""
+    x, z, h0, lengths, kind, B, T, D = _scan_args(x, z, h0, lengths)
+    require_cuda(gh, states, g_last)
+    gh = _sequences(gh, 'the gradient of h')
+    if gh.shape != x.shape:
+        raise ValueError(f'gradient of shape {tuple(gh.shape)} for an output of shape {tuple(x.shape)}')
+    element_type(x, gh)
+    dev = x.device
+    if g_last is not None:
+        g_last = _scan_state(g_last, B, D, dev, 'the gradient of h_last')
+    L = lib()
+    with torch.cuda.device(dev):
+        n = L.hgq_gated_scan_states(B, T, D)
+        if n and (states is None or states.numel() != n or states.dtype != torch.float32 or states.device != dev):
+            raise ValueError('states must be what gated_scan_fwd(..., want_states=True) returned for these inputs')
+        dx = torch.empty((B, T, D), dtype=x.dtype, device=dev)
+        dz = torch.empty_like(dx)
+        dh0 = torch.empty((B, D), dtype=torch.float32, device=dev) if want_dh0 else None
+        ws = workspace(L.hgq_gated_scan_workspace(B, T, D), dev, slot=9)
+        st = L.hgq_gated_scan_bwd(ptr(gh), gh.stride(0), gh.stride(1), ptr(x), x.stride(0), x.stride(1), ptr(z), z.stride(0), z.stride(1),
+                                  ptr(h0), ptr(lengths), ptr(states) if n else None, ptr(g_last), ptr(dx), ptr(dz), ptr(dh0), B, T, D, kind,
+                                  ptr(ws), ws.numel() if ws is not None else 0, stream_handle())
+    check(st, 'hgq_gated_scan_bwd')
+    return dx, dz, dh0

@@ -459,6 +459,63 @@ int hgq_adamw_step(const hgq_adamw_tensor *tensors, int64_t n_tensors, const int
                    float *v_scale, double lr, double beta1, double beta2, double eps, double grad_scale, double clipnorm,
                    long long *step, unsigned *ticket, void *workspace, size_t workspace_bytes, void *stream);
 
+/* ---- group normalisation with an activation, channels last ----------------------------------- */
+
+#define HGQ_ACT_NONE 0
+#define HGQ_ACT_RELU 1
+#define HGQ_ACT_SILU 2 /* u sigmoid(u) */
+#define HGQ_ACT_GELU 3 /* u Phi(u), with the error function */
+
+/*
+ * y = act(xhat gamma + beta), xhat = (x - mean) / sqrt(var + eps), mean and (biased) variance over the S positions and the C / G
+ * neighbouring channels of each (sample, group).  Stands in for keras.layers.GroupNormalization followed by an activation
+ * (Keras, not HGQ2, owns both).
+ *   x, y [B, S, C] of `type` (HGQ_TYPE_*), S the product of the spatial extents, G divides C; gamma, beta [C] fp32 or NULL (1, 0);
+ *   mean, rstd [B, G] fp32 are written for the backward pass.
+ * B == 0 or S == 0: nothing is written.  workspace: hgq_group_norm_workspace(..., backward = 0) bytes.
+ */
+size_t hgq_group_norm_workspace(int64_t B, int64_t S, int C, int G, int type, int backward);
+int hgq_group_norm_fwd(const void *x, const float *gamma, const float *beta, void *y, float *mean, float *rstd, int64_t B, int64_t S,
+                       int C, int G, float eps, int activation, int type, void *workspace, size_t workspace_bytes, void *stream);
+
+/*
+ * Its backward from gy, x and the saved statistics: dx [B, S, C] of `type` (may be NULL), dgamma and dbeta [C] fp32
+ * (both or neither; overwritten, zeros when B == 0 or S == 0).  The ReLU's slope at 0 is 0.  Sums are taken in a fixed order.
+ * workspace: hgq_group_norm_workspace(..., backward = 1) bytes.
+ */
+int hgq_group_norm_bwd(const void *gy, const void *x, const float *gamma, const float *beta, const float *mean, const float *rstd,
+                       void *dx, float *dgamma, float *dbeta, int64_t B, int64_t S, int C, int G, int activation, int type,
+                       void *workspace, size_t workspace_bytes, void *stream);
+
+/* ---- gated linear recurrence ----------------------------------------------------------------- */
+
+/*
+ * h_t = a_t h_{t-1} + (1 - a_t) x_t with a_t = sigmoid(z_t), along the time axis of [B, T, D].  No reference counterpart in the
+ * scope of this library: the sequence layer beside attention for axes that are too long for it.
+ *   x, z: element (b, t, d) at b * batch stride + t * time stride + d, strides in elements (slices of a wider projection are read in
+ *   place); h [B, T, D] contiguous, all of `type` (HGQ_TYPE_*).  h0 [B, D] fp32 or NULL (zeros); h_last [B, D] fp32 receives the
+ *   state behind each row's last step.  Outputs must not overlap inputs.
+ *   lengths: [B] int32 on the device, or NULL: row b has lengths[b] steps (clamped to [0, T]); h is 0 behind them, and what x and z
+ *   hold there is not looked at.
+ *   states: NULL, or hgq_gated_scan_states(B, T, D) floats that the backward pass needs (the state at each tile's start).
+ * workspace: hgq_gated_scan_workspace(B, T, D) bytes (0 for most shapes).  Results do not depend on scheduling.
+ */
+size_t hgq_gated_scan_workspace(int64_t B, int64_t T, int64_t D);
+int64_t hgq_gated_scan_states(int64_t B, int64_t T, int64_t D);
+int hgq_gated_scan_fwd(const void *x, int64_t x_batch, int64_t x_time, const void *z, int64_t z_batch, int64_t z_time, const float *h0,
+                       const int32_t *lengths, void *h, float *h_last, float *states, int64_t B, int64_t T, int64_t D, int type,
+                       void *workspace, size_t workspace_bytes, void *stream);
+
+/*
+ * Its backward: gh (strided like x) is the gradient of h, g_last [B, D] fp32 that of h_last or NULL (zeros).  dx, dz [B, T, D]
+ * contiguous of `type`, zero behind a row's length; dh0 [B, D] fp32 or NULL.  x, z, h0, lengths as in the forward call, states as
+ * it left them.  h itself is not needed: it is recomputed in fp32.
+ */
+int hgq_gated_scan_bwd(const void *gh, int64_t g_batch, int64_t g_time, const void *x, int64_t x_batch, int64_t x_time, const void *z,
+                       int64_t z_batch, int64_t z_time, const float *h0, const int32_t *lengths, const float *states, const float *g_last,
+                       void *dx, void *dz, float *dh0, int64_t B, int64_t T, int64_t D, int type, void *workspace, size_t workspace_bytes,
+                       void *stream);
+
 /* ---- gradient exchange over peer memory, fused with the optimizer update ------------------------ */
 
 /*

@@ -1,0 +1,277 @@
+"""The gated linear recurrence (``kernels.gated_scan_fwd`` / ``_bwd``) against its definition in 64 bits."""
+
+import pytest
+import torch
+
+gpu = pytest.mark.gpu
+U = 2.0 ** -24
+HALF_STEP = {torch.float32: 0.0, torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}
+TINY = {torch.float32: 0.0, torch.bfloat16: 0.0, torch.float16: 2.0 ** -25}
+
+SHAPES = [  # (batch, time, features)
+    (1, 1, 1), (64, 1, 256), (3, 2, 33), (2, 15, 7), (2, 16, 32), (2, 17, 64), (5, 31, 100), (700, 64, 64), (3, 255, 40), (2, 256, 32),
+    (2, 257, 31), (1, 1000, 5), (1, 4097, 70), (2, 3001, 300), (40, 300, 129), (1, 20000, 3), (0, 5, 8), (3, 0, 8), (4, 9, 0),
+]
+
+
+def reference(x, z, h0, lengths, gh, g_last):
+    """The definition step by step in fp64 (on the CPU: long axes are many small steps)."""
+    dev = x.device
+    x, z = x.double().cpu(), z.double().cpu()
+    B, T, D = x.shape
+    ends = torch.full((B,), T) if lengths is None else lengths.cpu().clamp(0, T)
+    h = torch.zeros(B, D, dtype=torch.float64) if h0 is None else h0.double().cpu()
+    a, c = torch.sigmoid(z), torch.sigmoid(-z)
+    out, before = torch.zeros_like(x), torch.zeros_like(x)
+    size = h.abs()  # the same recurrence on magnitudes: what rounding errors scale with
+    sizes = torch.zeros_like(x)
+    for t in range(T):
+        live = (t < ends)[:, None]
+        before[:, t] = h
+        h = torch.where(live, a[:, t] * h + c[:, t] * x[:, t], h)
+        size = torch.where(live, a[:, t] * size + c[:, t] * x[:, t].abs(), size)
+        out[:, t] = torch.where(live, h, 0.0)
+        sizes[:, t] = size
+    res = {'h': out, 'h_last': h, 'size': sizes, 'size_last': size}
+    if gh is not None:
+        g = gh.double().cpu()
+        mu = torch.zeros(B, D, dtype=torch.float64) if g_last is None else g_last.double().cpu()
+        size_mu = mu.abs()
+        dx, dz, sdx, sdz = (torch.zeros_like(x) for _ in range(4))
+        for t in range(T - 1, -1, -1):
+            live = (t < ends)[:, None]
+            lam, slam = mu + g[:, t], size_mu + g[:, t].abs()
+            dx[:, t] = torch.where(live, c[:, t] * lam, 0.0)
+            dz[:, t] = torch.where(live, a[:, t] * c[:, t] * lam * (before[:, t] - x[:, t]), 0.0)
+            sdx[:, t] = c[:, t] * slam
+            prev = sizes[:, t - 1] if t else (torch.zeros_like(h) if h0 is None else h0.double().cpu().abs())
+            sdz[:, t] = a[:, t] * c[:, t] * slam * (prev + x[:, t].abs())
+            mu = torch.where(live, a[:, t] * lam, mu)
+            size_mu = torch.where(live, a[:, t] * slam, size_mu)
+        res.update(dx=dx, dz=dz, dh0=mu, size_dx=sdx, size_dz=sdz, size_dh0=size_mu)
+    return {k: v.to(dev) for k, v in res.items()}
+
+
+def close(got, value, size, dtype, memory, what):
+    """A gate and its complement are good to 4 ulps, a step rounds twice more, and errors decay with the state: a step's relative
+    error of 6 U is carried for 1 / (1 - a) steps on average (``memory`` bounds that for these gates), folding the runs and
+    tiles doubles it."""
+    allowed = 2 * 6 * U * memory * size + HALF_STEP[dtype] * (value.abs() + 12 * U * memory * size) + TINY[dtype] + 1e-37
+    d = (got.double() - value).abs()
+    assert bool((d <= allowed).all()), f'{what}: {float((d / allowed).max()):.2f} of the bound'
+
+
+def inputs(shape, dtype, seed, spread=1.5, centre=1.0):
+    B, T, D = shape
+    gen = torch.Generator(device='cuda').manual_seed(seed)
+    n = lambda *s: torch.randn(s, device='cuda', generator=gen)  # noqa: E731
+    x, z, gh = n(B, T, D).to(dtype), (centre + spread * n(B, T, D)).to(dtype), n(B, T, D).to(dtype)
+    return x, z, gh, n(B, D), n(B, D)
+
+
+@gpu
+@pytest.mark.parametrize('dtype', list(HALF_STEP), ids=str)
+@pytest.mark.parametrize('index', range(len(SHAPES)), ids=lambda i: 'x'.join(map(str, SHAPES[i])))
+@pytest.mark.parametrize('padded', [False, True])
+def test_forward_and_backward(index, dtype, padded):
+    from hgq2_b200 import kernels as K
+
+    shape = SHAPES[index]
+    B, T, D = shape
+    x, z, gh, h0, g_last = inputs(shape, dtype, index)
+    if index % 3 == 1:
+        h0 = None
+    if index % 3 == 2:
+        g_last = None
+    lengths = None
+    if padded:
+        lengths = torch.randint(0, T + 1, (B,), device='cuda', generator=torch.Generator(device='cuda').manual_seed(index))
+        if B > 1:
+            lengths[0], lengths[1] = 0, T
+        dead = torch.arange(T, device='cuda')[None, :] >= lengths[:, None]
+        x[dead], z[dead], gh[dead] = float('nan'), float('inf'), float('nan')  # what stands behind a row's end is not looked at
+    want = reference(torch.nan_to_num(x), torch.nan_to_num(z), h0, lengths, torch.nan_to_num(gh), g_last)
+    h, h_last, states = K.gated_scan_fwd(x, z, h0, lengths, want_states=True)
+    assert h.dtype == dtype and h.shape == shape and h_last.shape == (B, D)
+    close(h, want['h'], want['size'], dtype, 40, 'h')
+    close(h_last, want['h_last'], want['size_last'], torch.float32, 40, 'h_last')
+    dx, dz, dh0 = K.gated_scan_bwd(gh, x, z, h0, lengths, states, g_last, want_dh0=True)
+    close(dx, want['dx'], want['size_dx'], dtype, 80, 'dx')
+    close(dz, want['dz'], want['size_dz'], dtype, 160, 'dz')
+    close(dh0, want['dh0'], want['size_dh0'], torch.float32, 80, 'dh0')
+    # without states the forward is the same, and everything repeats bit for bit
+    again, last, none = K.gated_scan_fwd(x, z, h0, lengths)
+    assert none is None and torch.equal(h, again) and torch.equal(h_last, last)
+    assert all(torch.equal(a, b) for a, b in zip((dx, dz), K.gated_scan_bwd(gh, x, z, h0, lengths, states, g_last)))
+
+
+@gpu
+@pytest.mark.parametrize('dtype', list(HALF_STEP), ids=str)
+def test_tokens_one_by_one_equal_the_sequence(dtype):
+    """Serving: the state carried from token to token gives the sequence's outputs."""
+    from hgq2_b200 import kernels as K
+
+    x, z, _, h0, _ = inputs((6, 40, 50), dtype, 1)
+    h, h_last, _ = K.gated_scan_fwd(x, z, h0)
+    state, out = h0, []
+    for t in range(40):
+        y, state, _ = K.gated_scan_fwd(x[:, t:t + 1], z[:, t:t + 1], state)
+        out.append(y)
+    want = reference(x, z, h0, None, None, None)
+    close(torch.cat(out, 1), want['h'], want['size'], dtype, 40, 'token by token')
+    close(state, want['h_last'], want['size_last'], torch.float32, 40, 'state')
+    # pieces of a sequence: a prompt of 23, then the rest
+    a, s, _ = K.gated_scan_fwd(x[:, :23], z[:, :23], h0)
+    b, s, _ = K.gated_scan_fwd(x[:, 23:], z[:, 23:], s)
+    close(torch.cat([a, b], 1), want['h'], want['size'], dtype, 40, 'in two pieces')
+
+
+@gpu
+@pytest.mark.parametrize('T', [1, 40, 700, 9000])
+def test_slices_of_a_wider_projection_are_read_in_place(T):
+    from hgq2_b200 import kernels as K
+
+    gen = torch.Generator(device='cuda').manual_seed(2)
+    p = torch.randn(3, T, 100, device='cuda', generator=gen)
+    x, z = p[..., :45], p[..., 50:95]
+    g = torch.randn(T, 3, 45, device='cuda', generator=gen).transpose(0, 1)  # time-major
+    h, last, states = K.gated_scan_fwd(x, z, want_states=True)
+    hc, lc, sc = K.gated_scan_fwd(x.contiguous(), z.contiguous(), want_states=True)
+    assert torch.equal(h, hc) and torch.equal(last, lc) and torch.equal(states, sc)
+    got = K.gated_scan_bwd(g, x, z, None, None, states)
+    want = K.gated_scan_bwd(g.contiguous(), x.contiguous(), z.contiguous(), None, None, sc)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    # a broadcast gradient (time stride 0) and features with a stride (copied)
+    e = g[:, :1].expand(3, T, 45)
+    assert torch.equal(K.gated_scan_bwd(e, x, z, None, None, states)[0], K.gated_scan_bwd(e.contiguous(), x, z, None, None, states)[0])
+    q = torch.randn(3, 45, T, device='cuda', generator=gen).transpose(1, 2)
+    assert torch.equal(K.gated_scan_fwd(q, z)[0], K.gated_scan_fwd(q.contiguous(), z)[0])
+
+
+@gpu
+def test_gates_at_their_ends():
+    """A gate of exactly 0 forgets, of exactly 1 keeps; very long memory stays accurate."""
+    from hgq2_b200 import kernels as K
+
+    x = torch.randn(2, 600, 40, device='cuda')
+    z = torch.full_like(x, float('inf'))
+    h0 = torch.randn(2, 40, device='cuda')
+    assert torch.equal(K.gated_scan_fwd(x, z, h0)[0], h0[:, None].expand_as(x))
+    z[:, 300:] = float('-inf')
+    h, _, st = K.gated_scan_fwd(x, z, h0, want_states=True)
+    assert torch.equal(h[:, 300:], x[:, 300:])
+    dx, dz, dh0 = K.gated_scan_bwd(torch.ones_like(x), x, z, h0, None, st, want_dh0=True)
+    assert torch.equal(dx[:, 300:], torch.ones_like(dx[:, 300:])) and not bool(dx[:, :300].any()) and not bool(dz.any())
+    assert torch.equal(dh0, torch.full_like(dh0, 300.0))
+    z = torch.full_like(x, 12.0)  # 1 - a = 6e-6: memory of 160000 steps, longer than the sequence
+    want = reference(x, z, h0, None, torch.ones_like(x), None)
+    h, _, st = K.gated_scan_fwd(x, z, h0, want_states=True)
+    close(h, want['h'], want['size'], torch.float32, 600, 'long memory')
+    dx, dz, dh0 = K.gated_scan_bwd(torch.ones_like(x), x, z, h0, None, st, want_dh0=True)
+    close(dx, want['dx'], want['size_dx'], torch.float32, 600, 'dx of long memory')
+    close(dz, want['dz'], want['size_dz'], torch.float32, 1200, 'dz of long memory')
+
+
+@gpu
+def test_gradients_against_differences():
+    from hgq2_b200 import kernels as K
+
+    x, z, gh, h0, g_last = inputs((2, 37, 9), torch.float32, 3)
+    _, _, st = K.gated_scan_fwd(x, z, h0, want_states=True)
+    grads = K.gated_scan_bwd(gh, x, z, h0, None, st, g_last, want_dh0=True)
+    leaves = [t.double() for t in (x, z, h0)]
+
+    def value(ts):
+        r = reference(ts[0], ts[1], ts[2], None, None, None)
+        return float((r['h'] * gh.double()).sum() + (r['h_last'] * g_last.double()).sum())
+
+    gen = torch.Generator(device='cuda').manual_seed(4)
+    for which in range(3):
+        v = torch.randn(leaves[which].shape, device='cuda', generator=gen, dtype=torch.float64)
+        up, down = ([t + s * 1e-5 * v if i == which else t for i, t in enumerate(leaves)] for s in (1, -1))
+        diff = (value(up) - value(down)) / 2e-5
+        products = grads[which].double() * v
+        assert abs(diff - float(products.sum())) <= 1e-5 * float(products.abs().sum())
+
+
+@gpu
+def test_captured_on_another_stream_and_two_at_once():
+    from hgq2_b200 import kernels as K
+
+    cases = [inputs((2, 5000, 64), torch.bfloat16, 5), inputs((300, 70, 64), torch.float32, 6)]
+
+    def both(x, z, gh, h0, g_last):
+        h, last, st = K.gated_scan_fwd(x, z, h0, want_states=True)
+        return (h, last, *K.gated_scan_bwd(gh, x, z, h0, None, st, g_last, want_dh0=True))
+
+    want = [t.clone() for c in cases for t in both(*c)]
+    torch.cuda.synchronize()
+    got = []
+    for c in cases:
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(5):
+                r = both(*c)
+            got += r
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    graphs, outs = [], []
+    for c in cases:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs += both(*c)
+        graphs.append(g)
+    for t in outs:
+        t.zero_()
+    for g in (*graphs, *graphs[::-1]):
+        g.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(outs, want))
+
+
+@gpu
+def test_refusals_on_the_device():
+    from hgq2_b200 import kernels as K
+
+    x = torch.zeros(2, 300, 8, device='cuda')
+    h0 = torch.zeros(2, 8, device='cuda')
+    for kw in (dict(z=x[:1]), dict(z=x.bfloat16()), dict(x=x[0]), dict(x=x.double(), z=x.double()), dict(h0=h0[:1]),
+               dict(h0=h0.bfloat16()), dict(lengths=torch.zeros(3, device='cuda', dtype=torch.int32)), dict(lengths=h0[:, 0])):
+        args = dict(x=x, z=x)
+        args.update(kw)
+        with pytest.raises(ValueError):
+            K.gated_scan_fwd(**args)
+    with pytest.raises(RuntimeError, match='CUDA tensors only'):
+        K.gated_scan_fwd(x, x, lengths=torch.zeros(2, dtype=torch.int32))
+    _, _, st = K.gated_scan_fwd(x, x, want_states=True)
+    assert st.numel() > 0
+    for kw in (dict(gh=x[:1]), dict(gh=x.bfloat16()), dict(states=None), dict(states=st[1:]), dict(g_last=h0[:1])):
+        args = dict(gh=x, x=x, z=x, states=st)
+        args.update(kw)
+        with pytest.raises(ValueError):
+            K.gated_scan_bwd(**args)
+
+
+def test_refusals_need_no_gpu():
+    from hgq2_b200 import _lib, build
+    from hgq2_b200 import kernels as K
+
+    with pytest.raises(RuntimeError, match='CUDA tensors only'):
+        K.gated_scan_fwd(torch.zeros(2, 3, 8), torch.zeros(2, 3, 8))
+    build.build()
+    L = _lib.lib()
+    p = 4096  # never dereferenced: every call below is refused on the host
+
+    def fwd(x=p, last=p, B=1, T=30000, D=8, kind=0, ws=p, nbytes=1 << 30):
+        return L.hgq_gated_scan_fwd(x, 1, 1, p, 1, 1, None, None, p, last, None, B, T, D, kind, ws, nbytes, None)
+
+    def bwd(gh=p, states=p, B=1, T=30000, D=8, kind=0, ws=p, nbytes=1 << 30):
+        return L.hgq_gated_scan_bwd(gh, 1, 1, p, 1, 1, p, 1, 1, None, None, states, None, p, p, None, B, T, D, kind, ws, nbytes, None)
+
+    assert fwd(x=None) == -1 and fwd(last=None) == -1 and bwd(gh=None) == -1 and bwd(states=None) == -1
+    assert fwd(B=-1) == -2 and fwd(T=-1) == -2 and fwd(D=-1) == -2 and fwd(T=1 << 62) == -2 and fwd(B=1 << 40) == -2
+    assert fwd(kind=3) == -3 and bwd(kind=-1) == -3
+    assert fwd(x=p + 2) == -4 and fwd(kind=1, x=p + 1) == -4 and bwd(states=p + 2) == -4
+    need = L.hgq_gated_scan_workspace(1, 30000, 8)
+    assert need > 0 and fwd(nbytes=need - 1) == -5 and bwd(ws=None) == -5
+    assert fwd(B=0) == 0 and bwd(D=0) == 0
+    assert L.hgq_gated_scan_workspace(4096, 64, 64) == 0 and L.hgq_gated_scan_states(4096, 64, 64) == 0
