@@ -141,8 +141,8 @@ SIGNATURES: dict[str, tuple] = {
     ),
     'hgq_gated_scan_bwd': (
         c_int,
-        [c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64] + [c_void_p] * 7 +
-        [c_int64, c_int64, c_int64, c_int, c_void_p, c_size_t, c_void_p],
+        [c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64] + [c_void_p] * 4 +
+        [c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64, c_int64, c_int, c_void_p, c_size_t, c_void_p],
     ),
     'hgq_adamw_workspace': (c_size_t, [c_int64]),
     'hgq_adamw_step': (

@@ -263,6 +263,11 @@ def join_bookkeeping() -> None:
         return
     side = _side_streams.get(torch.cuda.current_device())
     if side is not None and torch.cuda.current_stream() != side:
+        if torch.cuda.is_current_stream_capturing():
+            with torch.cuda.stream(side):
+                forked = torch.cuda.is_current_stream_capturing()
+            if not forked:  # this capture queued nothing there, and work from before it cannot be waited for inside it
+                return
         torch.cuda.current_stream().wait_stream(side)
 
 

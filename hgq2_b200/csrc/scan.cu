@@ -42,6 +42,7 @@ __device__ __forceinline__ void scan_store(__half *p, float v) { *p = __float2ha
 struct ScanDims {
     int64_t B, T, D, channels;       // channels = B D
     int64_t xsb, xst, zsb, zst, gsb, gst;  // batch and time strides of x, z and the upstream gradient, in elements
+    int64_t dxb, dxt, dzb, dzt;            // and of the gradients of x and z
     int WT, WC;                      // warps of a CTA along time and along channels
     int64_t tiles, tiles_per_segment;
     int segments;
@@ -89,7 +90,7 @@ __device__ __forceinline__ void load_run(const T *__restrict__ x, const T *__res
     for (int i = 0; i < STEPS; ++i) {
         const bool live = t0 + i < l.len;
         a[i] = live ? scan_float(zp[i * s.zst]) : 0.f;
-        v[i] = live ? scan_float(xp[i * s.xst]) : 0.f;
+        v[i] = live && x != nullptr ? scan_float(xp[i * s.xst]) : 0.f;
     }
 #pragma unroll
     for (int i = 0; i < STEPS; ++i) {
@@ -237,7 +238,7 @@ __global__ void __launch_bounds__(512) k_scan_bwd(const T *__restrict__ gh, cons
         load_run<T, STEPS>(x, z, s, l, t0, a, c, v);
         const T *gp = gh + l.b * s.gsb + l.d + t0 * s.gst;
 #pragma unroll
-        for (int i = 0; i < STEPS; ++i) g[i] = t0 + i < l.len ? scan_float(gp[i * s.gst]) : 0.f;
+        for (int i = 0; i < STEPS; ++i) g[i] = gh != nullptr && t0 + i < l.len ? scan_float(gp[i * s.gst]) : 0.f;
         float h = 0.f;
         if (l.in) h = states != nullptr ? states[tile * s.channels + l.c] : (h0 != nullptr ? h0[l.c] : 0.f);
         float m = mu;
@@ -269,7 +270,7 @@ __global__ void __launch_bounds__(512) k_scan_bwd(const T *__restrict__ gh, cons
             h = a[i] * h + c[i] * v[i];
             v[i] = d;
         }
-        const int64_t o = (l.b * s.T + t0) * s.D + l.d;
+        T *dxp = dx + l.b * s.dxb + t0 * s.dxt + l.d, *dzp = dz + l.b * s.dzb + t0 * s.dzt + l.d;
 #pragma unroll
         for (int i = STEPS - 1; i >= 0; --i) {
             const float lam = g[i] + m;
@@ -277,8 +278,8 @@ __global__ void __launch_bounds__(512) k_scan_bwd(const T *__restrict__ gh, cons
             m = a[i] * lam;
             if (l.in && t0 + i < s.T) {
                 const bool live = t0 + i < l.len;
-                scan_store(dx + o + i * s.D, live ? gx : 0.f);
-                scan_store(dz + o + i * s.D, live ? a[i] * gx * v[i] : 0.f);
+                scan_store(dxp + i * s.dxt, live ? gx : 0.f);
+                scan_store(dzp + i * s.dzt, live ? a[i] * gx * v[i] : 0.f);
             }
         }
         if (s.WT == 1) mu = m;
@@ -395,11 +396,12 @@ extern "C" int hgq_gated_scan_fwd(const void *x, int64_t x_batch, int64_t x_time
 
 extern "C" int hgq_gated_scan_bwd(const void *gh, int64_t g_batch, int64_t g_time, const void *x, int64_t x_batch, int64_t x_time,
                                   const void *z, int64_t z_batch, int64_t z_time, const float *h0, const int32_t *lengths,
-                                  const float *states, const float *g_last, void *dx, void *dz, float *dh0, int64_t B, int64_t T, int64_t D,
-                                  int type, void *workspace, size_t workspace_bytes, void *stream) {
+                                  const float *states, const float *g_last, void *dx, int64_t dx_batch, int64_t dx_time, void *dz,
+                                  int64_t dz_batch, int64_t dz_time, float *dh0, int64_t B, int64_t T, int64_t D, int type, void *workspace, size_t workspace_bytes,
+                                  void *stream) {
     if (int e = scan_args(B, T, D, type)) return e;
     if (B * D == 0) return HGQ_OK;
-    if (T > 0 && (!gh || !x || !z || !dx || !dz)) return HGQ_ERR_NULL;
+    if (T > 0 && (!x || !z || !dx || !dz)) return HGQ_ERR_NULL;
     const size_t size = type == HGQ_TYPE_F32 ? 4 : 2;
     if (!aligned(gh, size) || !aligned(x, size) || !aligned(z, size) || !aligned(dx, size) || !aligned(dz, size) || !aligned(h0, 4) ||
         !aligned(lengths, 4) || !aligned(states, 4) || !aligned(g_last, 4) || !aligned(dh0, 4))
@@ -409,6 +411,7 @@ extern "C" int hgq_gated_scan_bwd(const void *gh, int64_t g_batch, int64_t g_tim
     if (need > 0 && !aligned(workspace, 8)) return HGQ_ERR_ALIGN;
     ScanDims s = scan_dims(B, T, D);
     s.xsb = x_batch, s.xst = x_time, s.zsb = z_batch, s.zst = z_time, s.gsb = g_batch, s.gst = g_time;
+    s.dxb = dx_batch, s.dxt = dx_time, s.dzb = dz_batch, s.dzt = dz_time;
     if (s.tiles > 1 && !states) return HGQ_ERR_NULL;
     if (s.tiles <= 1) states = nullptr;
     cudaStream_t st = (cudaStream_t)stream;

@@ -40,6 +40,8 @@ from .layers.attn.mha import QMultiHeadAttention
 from .layers.conv import QConv2D
 from .layers.core.dense import QDense
 from .layers.core.einsum_dense import QEinsumDense
+from .layers.gated_recurrence import QGatedRecurrence
+from .layers.group_normalization import GroupNormalization
 from .quantizer.internal.base import DefaultBitwidthMapper
 from .quantizer.internal.fixed_point_quantizer import FixedPointQuantizerKBI, FixedPointQuantizerKIF
 
@@ -615,6 +617,77 @@ class _Attention(_Node):
         return terms
 
 
+class _GroupNorm(_Node):
+    """GroupNormalization: its two variables are not quantised, their gradients go straight into the flat bucket."""
+
+    def __init__(self, eng, layer):
+        self.layer = layer
+        for v in (layer._gamma, layer._beta):
+            if v is not None and v.trainable:
+                eng.covers(v)
+
+    def forward(self, x):
+        layer = self.layer
+        self.x = x.contiguous()
+        y, *self.stats = kernels.group_norm_fwd(self.x, layer.gamma, layer.beta, layer.groups, layer.epsilon, layer.activation)
+        return y
+
+    def backward(self, g, need_dx=True):
+        layer = self.layer
+        outs = [None if v is None or not v.trainable else v.value.grad.view(-1) for v in (layer._gamma, layer._beta)]
+        dx, _, _ = kernels.group_norm_bwd(g, self.x, layer.gamma, layer.beta, *self.stats, layer.groups, layer.activation, want_dx=need_dx,
+                                          want_params=any(o is not None for o in outs), out_dgamma=outs[0], out_dbeta=outs[1])
+        self.x = self.stats = None
+        return dx
+
+
+class _GatedRecurrence(_Node):
+    """QGatedRecurrence on [batch, time, features]: the projection, then the scan in place on its two halves."""
+
+    def __init__(self, eng, layer, in_shape):
+        self.layer = layer
+        _require(not layer.return_state, f'{layer.name}: returns its state')
+        self.proj = _Dense(eng, layer.projection, in_shape)
+        self.oq = None
+        if layer.enable_oq:
+            self.oq = eng.slot(layer.oq, 'act')
+            _require(not self.oq.kbi and self.oq.wrap, f'{layer.name}: output quantizer must be (k, i, f) in WRAP mode')
+            _require(self.oq.n == int(np.prod(layer.compute_output_shape(in_shape)[1:])),
+                     f'{layer.name}: output bitwidth table is not per activation')
+            self.oq.tracked_act = True
+
+    def check(self, batch):
+        self.proj.check(batch)
+
+    def post_allocate(self, eng):
+        self.proj.post_allocate(eng)
+
+    def forward(self, x):
+        self.p = self.proj.forward(x)
+        h, last, self.states = kernels.gated_scan_fwd(self.p[:, :, 0], self.p[:, :, 1], want_states=True)
+        y = h if self.layer.return_sequences else last
+        if self.oq is not None:
+            self.y_pre = y
+            y = kernels.quantize_fwd(y, None, None, self.oq.F.view(-1), self.oq.q.round_mode, 'NONE', training=True,
+                                     want_absmax=True, absmax_out=self.oq.absmax)[0]
+        return y
+
+    def backward(self, g, need_dx=True):
+        if self.oq is not None:
+            g = g.contiguous()
+            kernels.quantize_bwd(g, self.y_pre, None, None, self.oq.F.view(-1), self.oq.q.round_mode, 'NONE', want_dx=False,
+                                 want_di=False, out_df=self.oq.dF.view(-1))
+            self.y_pre = None
+        p, dp = self.p, torch.empty_like(self.p)
+        gh, g_last = (g, None) if self.layer.return_sequences else (None, g)
+        kernels.gated_scan_bwd(gh, p[:, :, 0], p[:, :, 1], None, None, self.states, g_last, out_dx=dp[:, :, 0], out_dz=dp[:, :, 1])
+        self.p = self.states = None
+        return self.proj.backward(dp, need_dx)
+
+    def ebops(self, eng, dense_items):
+        self.proj.ebops(eng, dense_items)
+
+
 class Engine:
     def __init__(self, model, state):
         _require(isinstance(model, Sequential), 'not a Sequential model')
@@ -627,6 +700,7 @@ class Engine:
         self._weights = []  # (variable, slot, offset into the qweights buffer)
         self._wfloats = 0
         self._n_eb = 0
+        self._float_variables: list = []  # variables that are not quantised: their node writes their gradients
         shape = (None,) + tuple(model.input_shape)
         self.nodes: list[_Node] = []
         for layer in model.layers:
@@ -671,6 +745,11 @@ class Engine:
             return _Dense(self, layer, in_shape), layer.compute_output_shape(in_shape)
         if isinstance(layer, QConv2D):
             return _Conv(self, layer, in_shape), layer.compute_output_shape(in_shape)
+        if isinstance(layer, GroupNormalization):
+            return _GroupNorm(self, layer), in_shape
+        if isinstance(layer, QGatedRecurrence):
+            _require(len(in_shape) == 3, 'recurrence input rank')
+            return _GatedRecurrence(self, layer, in_shape), layer.compute_output_shape(in_shape)
         if isinstance(layer, MaxPooling2D):
             _, h, w, c = in_shape
             oh, ow = (h - layer.pool_size[0]) // layer.strides[0] + 1, (w - layer.pool_size[1]) // layer.strides[1] + 1
@@ -703,6 +782,10 @@ class Engine:
         h_q, h_d = _Lazy(), _Lazy()
         self._weights[-1] += (h_q, h_d)
         return h_q, h_d
+
+    def covers(self, variable) -> None:
+        """A node's word that its backward pass writes the gradient of ``variable`` into the flat bucket."""
+        self._float_variables.append(variable)
 
     def new_ebops_term(self) -> int:
         self._n_eb += 1
@@ -767,6 +850,7 @@ class Engine:
             covered.add(id(variable))
             d.n, d.slot = n, slot.index
             d.mode = 2 if slot.tracked_weight else 0
+        covered.update(id(v) for v in self._float_variables)
         missing = [v.path for v in self.state.variables if id(v) not in covered]
         _require(not missing, f'variables outside the engine: {missing[:4]}')
         self._slot_descs = self._upload(slot_descs)

@@ -829,14 +829,18 @@ def gated_scan_fwd(x, z, h0=None, lengths=None, want_states: bool = False):
     return h, h_last, states
 
 
-def gated_scan_bwd(gh, x, z, h0=None, lengths=None, states=None, g_last=None, want_dh0: bool = False):
-    """Gradients of ``gated_scan_fwd`` from the gradient ``gh`` of h (and ``g_last`` of h_last): (dx, dz, dh0 or None)."""
+def gated_scan_bwd(gh, x, z, h0=None, lengths=None, states=None, g_last=None, want_dh0: bool = False, out_dx=None,
+                   out_dz=None):
+    """Gradients of ``gated_scan_fwd`` from the gradients ``gh`` of h and ``g_last`` of h_last (None: zeros): (dx, dz, dh0 or None);
+    dx and dz go to ``out_dx`` / ``out_dz`` when given (like x, the features contiguous, any other strides)."""
     x, z, h0, lengths, kind, B, T, D = _scan_args(x, z, h0, lengths)
     require_cuda(gh, states, g_last)
-    gh = _sequences(gh, 'the gradient of h')
-    if gh.shape != x.shape:
-        raise ValueError(f'gradient of shape {tuple(gh.shape)} for an output of shape {tuple(x.shape)}')
-    element_type(x, gh)
+    if gh is not None:
+        gh = _sequences(gh, 'the gradient of h')
+        if gh.shape != x.shape:
+            raise ValueError(f'gradient of shape {tuple(gh.shape)} for an output of shape {tuple(x.shape)}')
+        element_type(x, gh)
+    gs = (0, 0) if gh is None else gh.stride()
     dev = x.device
     if g_last is not None:
         g_last = _scan_state(g_last, B, D, dev, 'the gradient of h_last')
@@ -845,12 +849,16 @@ def gated_scan_bwd(gh, x, z, h0=None, lengths=None, states=None, g_last=None, wa
         n = L.hgq_gated_scan_states(B, T, D)
         if n and (states is None or states.numel() != n or states.dtype != torch.float32 or states.device != dev):
             raise ValueError('states must be what gated_scan_fwd(..., want_states=True) returned for these inputs')
-        dx = torch.empty((B, T, D), dtype=x.dtype, device=dev)
-        dz = torch.empty_like(dx)
+        for o in (out_dx, out_dz):
+            if o is not None and (o.shape != x.shape or o.dtype != x.dtype or o.device != dev or (o.stride(2) != 1 and D > 1)):
+                raise ValueError(f'gradients go to {x.dtype} tensors of shape {tuple(x.shape)} on {dev} with contiguous features')
+        dx = torch.empty((B, T, D), dtype=x.dtype, device=dev) if out_dx is None else out_dx
+        dz = torch.empty((B, T, D), dtype=x.dtype, device=dev) if out_dz is None else out_dz
         dh0 = torch.empty((B, D), dtype=torch.float32, device=dev) if want_dh0 else None
         ws = workspace(L.hgq_gated_scan_workspace(B, T, D), dev, slot=9)
-        st = L.hgq_gated_scan_bwd(ptr(gh), gh.stride(0), gh.stride(1), ptr(x), x.stride(0), x.stride(1), ptr(z), z.stride(0), z.stride(1),
-                                  ptr(h0), ptr(lengths), ptr(states) if n else None, ptr(g_last), ptr(dx), ptr(dz), ptr(dh0), B, T, D, kind,
-                                  ptr(ws), ws.numel() if ws is not None else 0, stream_handle())
+        st = L.hgq_gated_scan_bwd(ptr(gh), gs[0], gs[1], ptr(x), x.stride(0), x.stride(1), ptr(z), z.stride(0), z.stride(1), ptr(h0),
+                                  ptr(lengths), ptr(states) if n else None, ptr(g_last), ptr(dx), dx.stride(0), dx.stride(1), ptr(dz),
+                                  dz.stride(0), dz.stride(1), ptr(dh0), B, T, D, kind, ptr(ws), ws.numel() if ws is not None else 0,
+                                  stream_handle())
     check(st, 'hgq_gated_scan_bwd')
     return dx, dz, dh0

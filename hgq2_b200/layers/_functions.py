@@ -434,3 +434,45 @@ class QSoftmaxFusedFn(torch.autograd.Function):
                 gf = df5.view(shapes[14])
             grads += [None, gi, gf]
         return (ds, None, None, None, None, None, None, None, *grads)
+
+
+class GroupNormFn(torch.autograd.Function):
+    """act(group norm(x) * gamma + beta) on the channels-last kernels; x and the statistics are kept for the backward pass."""
+
+    @staticmethod
+    def forward(ctx, x, gamma, beta, groups, eps, activation):
+        x = x.contiguous()
+        y, mean, rstd = kernels.group_norm_fwd(x, gamma, beta, groups, eps, activation)
+        ctx.save_for_backward(x, gamma, beta, mean, rstd)
+        ctx.meta = (groups, activation)
+        return y
+
+    @staticmethod
+    def backward(ctx, gy):
+        x, gamma, beta, mean, rstd = ctx.saved_tensors
+        groups, activation = ctx.meta
+        need_x, need_gamma, need_beta = ctx.needs_input_grad[:3]
+        dx, dgamma, dbeta = kernels.group_norm_bwd(gy, x, gamma, beta, mean, rstd, groups, activation, want_dx=need_x,
+                                                   want_params=need_gamma or need_beta)
+        return dx, (dgamma if need_gamma else None), (dbeta if need_beta else None), None, None, None
+
+
+class GatedScanFn(torch.autograd.Function):
+    """The gated linear recurrence on a projection p [batch, time, 2, units] that holds x in p[:, :, 0] and the gate's argument
+    in p[:, :, 1]; both are read, and their gradients written, in place.  Returns (h, h_last)."""
+
+    @staticmethod
+    def forward(ctx, p, h0, lengths):
+        p = p.contiguous()
+        h, h_last, states = kernels.gated_scan_fwd(p[:, :, 0], p[:, :, 1], h0, lengths, want_states=any(ctx.needs_input_grad))
+        ctx.save_for_backward(p, h0, lengths, states)
+        ctx.set_materialize_grads(False)  # an output that is not used has a gradient of None, not a tensor of zeros
+        return h, h_last
+
+    @staticmethod
+    def backward(ctx, gh, g_last):
+        p, h0, lengths, states = ctx.saved_tensors
+        dp = torch.empty_like(p)
+        _, _, dh0 = kernels.gated_scan_bwd(gh, p[:, :, 0], p[:, :, 1], h0, lengths, states, g_last,
+                                           want_dh0=ctx.needs_input_grad[1], out_dx=dp[:, :, 0], out_dz=dp[:, :, 1])
+        return dp, dh0, None

@@ -507,14 +507,14 @@ int hgq_gated_scan_fwd(const void *x, int64_t x_batch, int64_t x_time, const voi
                        void *workspace, size_t workspace_bytes, void *stream);
 
 /*
- * Its backward: gh (strided like x) is the gradient of h, g_last [B, D] fp32 that of h_last or NULL (zeros).  dx, dz [B, T, D]
- * contiguous of `type`, zero behind a row's length; dh0 [B, D] fp32 or NULL.  x, z, h0, lengths as in the forward call, states as
+ * Its backward: gh (strided like x) is the gradient of h, g_last [B, D] fp32 that of h_last; NULL: zeros.  dx, dz
+ * (strided like x, of `type`) are zero behind a row's length; dh0 [B, D] fp32 or NULL.  x, z, h0, lengths as in the forward call, states as
  * it left them.  h itself is not needed: it is recomputed in fp32.
  */
 int hgq_gated_scan_bwd(const void *gh, int64_t g_batch, int64_t g_time, const void *x, int64_t x_batch, int64_t x_time, const void *z,
                        int64_t z_batch, int64_t z_time, const float *h0, const int32_t *lengths, const float *states, const float *g_last,
-                       void *dx, void *dz, float *dh0, int64_t B, int64_t T, int64_t D, int type, void *workspace, size_t workspace_bytes,
-                       void *stream);
+                       void *dx, int64_t dx_batch, int64_t dx_time, void *dz, int64_t dz_batch, int64_t dz_time, float *dh0, int64_t B,
+                       int64_t T, int64_t D, int type, void *workspace, size_t workspace_bytes, void *stream);
 
 /* ---- gradient exchange over peer memory, fused with the optimizer update ------------------------ */
 

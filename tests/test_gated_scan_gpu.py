@@ -141,11 +141,27 @@ def test_slices_of_a_wider_projection_are_read_in_place(T):
     got = K.gated_scan_bwd(g, x, z, None, None, states)
     want = K.gated_scan_bwd(g.contiguous(), x.contiguous(), z.contiguous(), None, None, sc)
     assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    both = torch.full_like(p, 7.0)  # and gradients into the slices of one
+    K.gated_scan_bwd(g, x, z, None, None, states, out_dx=both[..., :45], out_dz=both[..., 50:95])
+    assert torch.equal(both[..., :45], want[0]) and torch.equal(both[..., 50:95], want[1])
+    assert bool((both[..., 45:50] == 7).all() and (both[..., 95:] == 7).all())
     # a broadcast gradient (time stride 0) and features with a stride (copied)
     e = g[:, :1].expand(3, T, 45)
     assert torch.equal(K.gated_scan_bwd(e, x, z, None, None, states)[0], K.gated_scan_bwd(e.contiguous(), x, z, None, None, states)[0])
     q = torch.randn(3, 45, T, device='cuda', generator=gen).transpose(1, 2)
     assert torch.equal(K.gated_scan_fwd(q, z)[0], K.gated_scan_fwd(q.contiguous(), z)[0])
+
+
+@gpu
+@pytest.mark.parametrize('T', [1, 50, 5000])
+def test_only_the_last_state_has_a_gradient(T):
+    from hgq2_b200 import kernels as K
+
+    x, z, _, h0, g_last = inputs((2, T, 33), torch.float32, 7)
+    _, _, st = K.gated_scan_fwd(x, z, h0, want_states=True)
+    got = K.gated_scan_bwd(None, x, z, h0, None, st, g_last, want_dh0=True)
+    want = K.gated_scan_bwd(torch.zeros_like(x), x, z, h0, None, st, g_last, want_dh0=True)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
 
 
 @gpu
@@ -244,7 +260,7 @@ def test_refusals_on_the_device():
         K.gated_scan_fwd(x, x, lengths=torch.zeros(2, dtype=torch.int32))
     _, _, st = K.gated_scan_fwd(x, x, want_states=True)
     assert st.numel() > 0
-    for kw in (dict(gh=x[:1]), dict(gh=x.bfloat16()), dict(states=None), dict(states=st[1:]), dict(g_last=h0[:1])):
+    for kw in (dict(gh=x[:1]), dict(gh=x.bfloat16()), dict(states=None), dict(states=st[1:]), dict(g_last=h0[:1]), dict(out_dx=x[:1]), dict(out_dz=x.bfloat16())):
         args = dict(gh=x, x=x, z=x, states=st)
         args.update(kw)
         with pytest.raises(ValueError):
@@ -264,10 +280,11 @@ def test_refusals_need_no_gpu():
     def fwd(x=p, last=p, B=1, T=30000, D=8, kind=0, ws=p, nbytes=1 << 30):
         return L.hgq_gated_scan_fwd(x, 1, 1, p, 1, 1, None, None, p, last, None, B, T, D, kind, ws, nbytes, None)
 
-    def bwd(gh=p, states=p, B=1, T=30000, D=8, kind=0, ws=p, nbytes=1 << 30):
-        return L.hgq_gated_scan_bwd(gh, 1, 1, p, 1, 1, p, 1, 1, None, None, states, None, p, p, None, B, T, D, kind, ws, nbytes, None)
+    def bwd(states=p, B=1, T=30000, D=8, kind=0, ws=p, nbytes=1 << 30):
+        return L.hgq_gated_scan_bwd(p, 1, 1, p, 1, 1, p, 1, 1, None, None, states, None, p, 1, 1, p, 1, 1, None, B, T, D, kind, ws, nbytes,
+                                    None)
 
-    assert fwd(x=None) == -1 and fwd(last=None) == -1 and bwd(gh=None) == -1 and bwd(states=None) == -1
+    assert fwd(x=None) == -1 and fwd(last=None) == -1 and bwd(states=None) == -1
     assert fwd(B=-1) == -2 and fwd(T=-1) == -2 and fwd(D=-1) == -2 and fwd(T=1 << 62) == -2 and fwd(B=1 << 40) == -2
     assert fwd(kind=3) == -3 and bwd(kind=-1) == -3
     assert fwd(x=p + 2) == -4 and fwd(kind=1, x=p + 1) == -4 and bwd(states=p + 2) == -4
