@@ -3,73 +3,93 @@
 //   h_t = a_t h_{t-1} + c_t x_t,  a_t = sigmoid(z_t),  c_t = 1 - a_t = sigmoid(-z_t)
 //   lambda_t = g_t + a_{t+1} lambda_{t+1};  dx_t = c_t lambda_t;  dz_t = a_t c_t lambda_t (h_{t-1} - x_t);  dh_0 = a_0 lambda_0
 //
-// A step is the affine map h -> a h + b, and maps compose: (A, H) after (A', H') is (A A', A H' + H).  A lane owns one channel
-// (feature of one batch row) for STEPS consecutive time steps held in registers; the warps of a CTA hold consecutive runs of
-// the same 32 channels (a tile of WT x STEPS steps).  Each warp folds its run to one map, the maps meet in shared memory, every
-// warp folds those before its own onto the tile's incoming state and walks its run again from registers.  x and z are read
-// once, all loads of a tile are in flight together, and the state passes from tile to tile in a register: per-channel work in
-// time order, so nothing depends on scheduling.  Products of gates stay in (0, 1): there is no division by them and no
-// logarithm, so a gate that closes (a = 0) is exact.
+// A step is the affine map h -> a h + b, and maps compose: (A, H) after (A', H') is (A A', A H' + H).  A lane owns VEC neighbouring
+// channels (features of one batch row) for kScanSteps consecutive steps held in registers; the WT warps along time of a CTA hold
+// consecutive runs of the same channels (a tile).  Each warp folds its run to one map, the maps meet in shared memory, every warp
+// folds those before its own onto the tile's incoming state and walks its run again from registers.  x and z are read once, all
+// loads of a tile are in flight together, and the state passes from tile to tile in a register: per-channel work in time order,
+// so nothing depends on scheduling.  Products of gates stay in [0, 1]: there is no division by them and no logarithm.
 //
 // Few channels and a long axis leave most SMs without a CTA.  The axis is then cut into segments: a first launch folds each
 // segment to one map, the second starts each segment from the fold of the maps before it (x and z are read twice, the second
-// time mostly from L2).
+// time partly from L2: the second launch takes the segments in the opposite order, the last ones read first).
 //
-// The backward pass needs h_{t-1}.  The forward pass keeps the fp32 state at each tile's start (1 / (16 WT) of the outputs) and the
+// The backward pass needs h_{t-1}.  The forward pass keeps the fp32 state at each tile's start (one number per 64 outputs) and the
 // backward pass recomputes h inside the tile: it never reads h, and gradients of bf16 / fp16 sequences use unrounded states.
 //
 // Steps at or behind a row's length are the identity map: the state passes through, outputs and gradients there are zero.
 // State, maps and gradients are fp32; h, dx, dz are rounded to their type once, on the way out.
+//
+// What bounds it: the arithmetic on the way to the memory rate.  A step costs an exponential, a reciprocal and two walks; written
+// with expf, IEEE divisions and a 64-bit multiply per address it took 93 instructions an element and 149 us for the forward pass of
+// [8192, 64, 64] fp32 (402 MB); with the gates below, running pointers, two channels a lane and no predicates in full runs it is
+// bound by memory.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
+
+#include <initializer_list>
 
 #include "hgq_common.cuh"
 
 namespace hgq {
 
-constexpr int kScanSteps = 16;
-constexpr int kScanMaxWarps = 16;   // along time
-constexpr int kScanMaxSegments = 64;
+constexpr int kScanSteps = 8;
+constexpr int kScanMaxWarps = 8;  // along time
+constexpr int kScanMaxSegments = 128;
 
 __device__ __forceinline__ float scan_float(float v) { return v; }
 __device__ __forceinline__ float scan_float(__nv_bfloat16 v) { return __bfloat162float(v); }
 __device__ __forceinline__ float scan_float(__half v) { return __half2float(v); }
-__device__ __forceinline__ void scan_store(float *p, float v) { *p = v; }
-__device__ __forceinline__ void scan_store(__nv_bfloat16 *p, float v) { *p = __float2bfloat16_rn(v); }
-__device__ __forceinline__ void scan_store(__half *p, float v) { *p = __float2half_rn(v); }
+__device__ __forceinline__ void scan_round(float v, float &o) { o = v; }
+__device__ __forceinline__ void scan_round(float v, __nv_bfloat16 &o) { o = __float2bfloat16_rn(v); }
+__device__ __forceinline__ void scan_round(float v, __half &o) { o = __float2half_rn(v); }
+
+template <typename T, int VEC>
+struct alignas(sizeof(T) * VEC) ScanPack {
+    T v[VEC];
+};
 
 struct ScanDims {
-    int64_t B, T, D, channels;       // channels = B D
+    int64_t B, T, D, channels;             // channels = B D
     int64_t xsb, xst, zsb, zst, gsb, gst;  // batch and time strides of x, z and the upstream gradient, in elements
     int64_t dxb, dxt, dzb, dzt;            // and of the gradients of x and z
-    int WT, WC;                      // warps of a CTA along time and along channels
+    int WT, WC;                            // warps of a CTA along time and along channels
     int64_t tiles, tiles_per_segment;
     int segments;
 };
 
-// sigmoid(z) and sigmoid(-z), both to full relative precision
+// a = sigmoid(z) = 1 / (1 + e) with e = exp(-z), and c = 1 - a = e / (1 + e), each to full relative precision: c is formed as 1 - a
+// only where a < 1/2.  z is held in [-88, 100], where the gates are 0 and 1 in fp32; a NaN stays.  The exponential is
+// 2^(-z log2 e) with the rounding error of the product carried along, the reciprocal's error is one ulp.
 __device__ __forceinline__ void gates(float z, float &a, float &c) {
-    const float e = expf(-fabsf(z)), r = 1.f / (1.f + e), er = e * r;
-    a = z >= 0.f ? r : er;
-    c = z >= 0.f ? er : r;
-    if (z != z) a = c = z;
+    float e, r;
+    asm("max.NaN.f32 %0, %0, 0fC2B00000;" : "+f"(z));
+    asm("min.NaN.f32 %0, %0, 0f42C80000;" : "+f"(z));
+    const float t = z * -1.44269504088896341f;
+    const float lo = fmaf(z, -1.44269504088896341f, -t);
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(t));
+    e = fmaf(e, lo * 0.693147180559945309f, e);
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + e));
+    a = r;
+    c = z < 0.f ? 1.f - r : e * r;
 }
 
 struct Lane {
     int64_t c, b, d;
     int64_t len;  // steps of this row
     bool in;
-    int wt, wc, lane;
+    int wt, row, lane;  // row: of this warp in the CTA's exchange buffer, counted from its channel tile's first warp at row - wt
 };
 
+template <int VEC>
 __device__ __forceinline__ Lane scan_lane(const ScanDims &s, const int32_t *lengths) {
     Lane l;
     const int w = threadIdx.x >> 5;
     l.lane = threadIdx.x & 31;
     l.wt = w % s.WT;
-    l.wc = w / s.WT;
-    l.c = ((int64_t)blockIdx.x * s.WC + l.wc) * 32 + l.lane;
+    l.row = w;
+    l.c = (((int64_t)blockIdx.x * s.WC + w / s.WT) * 32 + l.lane) * VEC;
     l.in = l.c < s.channels;
     l.b = l.in ? l.c / s.D : 0;
     l.d = l.in ? l.c - l.b * s.D : 0;
@@ -81,212 +101,337 @@ __device__ __forceinline__ Lane scan_lane(const ScanDims &s, const int32_t *leng
     return l;
 }
 
-// The gates and inputs of STEPS steps from t0; steps that are not live are the identity.
-template <typename T, int STEPS>
-__device__ __forceinline__ void load_run(const T *__restrict__ x, const T *__restrict__ z, const ScanDims &s, const Lane &l, int64_t t0,
-                                         float (&a)[STEPS], float (&c)[STEPS], float (&v)[STEPS]) {
-    const T *xp = x + l.b * s.xsb + l.d + t0 * s.xst, *zp = z + l.b * s.zsb + l.d + t0 * s.zst;
+// STEPS packs of a strided sequence from step t0; steps that are not live read as zero.  p: the lane's channel at step t0.
+template <typename T, int VEC, int STEPS>
+__device__ __forceinline__ void load_packs(const T *__restrict__ p, int64_t stride, bool full, int64_t left, float (&v)[STEPS][VEC]) {
+    using P = ScanPack<T, VEC>;
+    P q[STEPS];
+    if (full) {
 #pragma unroll
-    for (int i = 0; i < STEPS; ++i) {
-        const bool live = t0 + i < l.len;
-        a[i] = live ? scan_float(zp[i * s.zst]) : 0.f;
-        v[i] = live && x != nullptr ? scan_float(xp[i * s.xst]) : 0.f;
-    }
+        for (int i = 0; i < STEPS; ++i, p += stride) q[i] = *reinterpret_cast<const P *>(p);
 #pragma unroll
-    for (int i = 0; i < STEPS; ++i) {
-        const float zi = a[i];
-        gates(zi, a[i], c[i]);
-        if (t0 + i >= l.len) a[i] = 1.f, c[i] = 0.f;
+        for (int i = 0; i < STEPS; ++i)
+#pragma unroll
+            for (int k = 0; k < VEC; ++k) v[i][k] = scan_float(q[i].v[k]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < STEPS; ++i, p += stride) {
+#pragma unroll
+            for (int k = 0; k < VEC; ++k) v[i][k] = 0.f;
+            if (i < left) {
+                q[i] = *reinterpret_cast<const P *>(p);
+#pragma unroll
+                for (int k = 0; k < VEC; ++k) v[i][k] = scan_float(q[i].v[k]);
+            }
+        }
     }
 }
 
-// Segment fold, one CTA per (channel tile, segment): agg[segment][channel] = (A, H).
-template <typename T, int STEPS>
-__global__ void __launch_bounds__(512) k_scan_fold(const T *__restrict__ x, const T *__restrict__ z, const int32_t *__restrict__ lengths,
-                                                   const ScanDims s, float2 *__restrict__ agg) {
-    __shared__ float2 sh[2][kScanMaxWarps][32];
-    const Lane l = scan_lane(s, lengths);
-    const int seg = blockIdx.y;
-    const int64_t first = seg * s.tiles_per_segment, last = min(s.tiles, first + s.tiles_per_segment);
-    float A = 1.f, H = 0.f;
-    for (int64_t tile = first; tile < last; ++tile) {
-        float a[STEPS], c[STEPS], v[STEPS];
-        load_run<T, STEPS>(x, z, s, l, (tile * s.WT + l.wt) * STEPS, a, c, v);
-        float ra = 1.f, rh = 0.f;
+template <typename T, int VEC, int STEPS>
+__device__ __forceinline__ void store_packs(T *p, int64_t stride, bool full, int64_t left, const float (&v)[STEPS][VEC]) {
+    using P = ScanPack<T, VEC>;
 #pragma unroll
-        for (int i = 0; i < STEPS; ++i) {
-            rh = a[i] * rh + c[i] * v[i];
-            ra *= a[i];
-        }
-        float2(*buf)[32] = sh[tile & 1];
-        buf[l.wc * s.WT + l.wt][l.lane] = make_float2(ra, rh);
-        __syncthreads();
-        if (l.wt == 0)
-            for (int w = 0; w < s.WT; ++w) {
-                const float2 q = buf[l.wc * s.WT + w][l.lane];
-                H = q.x * H + q.y;
-                A *= q.x;
+    for (int i = 0; i < STEPS; ++i, p += stride) {
+        P q;
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) scan_round(v[i][k], q.v[k]);
+        if (full || i < left) *reinterpret_cast<P *>(p) = q;
+    }
+}
+
+template <int VEC, int STEPS>
+__device__ __forceinline__ void make_gates(bool full, int64_t left, float (&a)[STEPS][VEC], float (&c)[STEPS][VEC]) {
+#pragma unroll
+    for (int i = 0; i < STEPS; ++i)
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) gates(a[i][k], a[i][k], c[i][k]);
+    if (!full) {
+#pragma unroll
+        for (int i = 0; i < STEPS; ++i)
+            if (i >= left) {
+#pragma unroll
+                for (int k = 0; k < VEC; ++k) a[i][k] = 1.f, c[i][k] = 0.f;
             }
     }
-    if (l.wt == 0 && l.in) agg[(int64_t)seg * s.channels + l.c] = make_float2(A, H);
 }
 
-template <typename T, int STEPS>
-__global__ void __launch_bounds__(512) k_scan_fwd(const T *__restrict__ x, const T *__restrict__ z, const float *__restrict__ h0,
-                                                  const int32_t *__restrict__ lengths, const ScanDims s, const float2 *__restrict__ agg,
-                                                  T *__restrict__ out, float *__restrict__ h_last, float *__restrict__ states) {
-    __shared__ float2 sh[2][kScanMaxWarps][32];
-    const Lane l = scan_lane(s, lengths);
+template <int VEC>
+struct alignas(8 * VEC) Map {  // h -> A h + H for VEC channels
+    float A[VEC], H[VEC];
+};
+
+// Segment fold of the forward recurrence: agg[segment][channel] = (A, H).
+template <typename T, int VEC, int STEPS>
+__global__ void __launch_bounds__(256) k_scan_fold(const T *__restrict__ x, const T *__restrict__ z, const int32_t *__restrict__ lengths,
+                                                   const ScanDims s, float2 *__restrict__ agg) {
+    __shared__ Map<VEC> sh[2][kScanMaxWarps][32];
+    const Lane l = scan_lane<VEC>(s, lengths);
     const int seg = blockIdx.y;
     const int64_t first = seg * s.tiles_per_segment, last = min(s.tiles, first + s.tiles_per_segment);
-    float carry = (l.in && h0 != nullptr) ? h0[l.c] : 0.f;
-    if (l.in)
-        for (int k = 0; k < seg; ++k) {
-            const float2 q = agg[(int64_t)k * s.channels + l.c];
-            carry = q.x * carry + q.y;
-        }
+    float A[VEC], H[VEC];
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) A[k] = 1.f, H[k] = 0.f;
     for (int64_t tile = first; tile < last; ++tile) {
-        const int64_t t0 = (tile * s.WT + l.wt) * STEPS;
-        float a[STEPS], c[STEPS], v[STEPS];
-        load_run<T, STEPS>(x, z, s, l, t0, a, c, v);
-        if (states != nullptr && l.wt == 0 && l.in) states[tile * s.channels + l.c] = carry;
-        float h = carry;
-        if (s.WT > 1) {
+        const int64_t t0 = (tile * s.WT + l.wt) * STEPS, left = l.len - t0;
+        const bool full = __all_sync(0xffffffffu, left >= STEPS);
+        float a[STEPS][VEC], c[STEPS][VEC], v[STEPS][VEC];
+        load_packs<T, VEC, STEPS>(z + l.b * s.zsb + l.d + t0 * s.zst, s.zst, full, left, a);
+        load_packs<T, VEC, STEPS>(x + l.b * s.xsb + l.d + t0 * s.xst, s.xst, full, left, v);
+        make_gates<VEC, STEPS>(full, left, a, c);
+        Map<VEC> m;
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) {
             float ra = 1.f, rh = 0.f;
 #pragma unroll
             for (int i = 0; i < STEPS; ++i) {
-                v[i] *= c[i];
-                rh = a[i] * rh + v[i];
-                ra *= a[i];
+                rh = a[i][k] * rh + c[i][k] * v[i][k];
+                ra *= a[i][k];
             }
-            float2(*buf)[32] = sh[tile & 1];
-            buf[l.wc * s.WT + l.wt][l.lane] = make_float2(ra, rh);
+            m.A[k] = ra, m.H[k] = rh;
+        }
+        Map<VEC>(*buf)[32] = sh[tile & 1];
+        buf[l.row][l.lane] = m;
+        __syncthreads();
+        if (l.wt == 0)
+            for (int w = 0; w < s.WT; ++w) {
+                const Map<VEC> q = buf[l.row + w][l.lane];
+#pragma unroll
+                for (int k = 0; k < VEC; ++k) {
+                    H[k] = q.A[k] * H[k] + q.H[k];
+                    A[k] *= q.A[k];
+                }
+            }
+    }
+    if (l.wt == 0 && l.in)
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) agg[(int64_t)seg * s.channels + l.c + k] = make_float2(A[k], H[k]);
+}
+
+template <typename T, int VEC, int STEPS>
+__global__ void __launch_bounds__(256) k_scan_fwd(const T *__restrict__ x, const T *__restrict__ z, const float *__restrict__ h0,
+                                                  const int32_t *__restrict__ lengths, const ScanDims s, const float2 *__restrict__ agg,
+                                                  T *__restrict__ out, float *__restrict__ h_last, float *__restrict__ states) {
+    __shared__ Map<VEC> sh[2][kScanMaxWarps][32];
+    const Lane l = scan_lane<VEC>(s, lengths);
+    const int seg = s.segments - 1 - blockIdx.y;
+    const int64_t first = seg * s.tiles_per_segment, last = min(s.tiles, first + s.tiles_per_segment);
+    float carry[VEC];
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) carry[k] = (l.in && h0 != nullptr) ? h0[l.c + k] : 0.f;
+    if (l.in)
+#pragma unroll 4
+        for (int j = 0; j < seg; ++j)
+#pragma unroll
+            for (int k = 0; k < VEC; ++k) {
+                const float2 q = agg[(int64_t)j * s.channels + l.c + k];
+                carry[k] = q.x * carry[k] + q.y;
+            }
+    for (int64_t tile = first; tile < last; ++tile) {
+        const int64_t t0 = (tile * s.WT + l.wt) * STEPS, left = l.len - t0;
+        const bool full = __all_sync(0xffffffffu, left >= STEPS);
+        float a[STEPS][VEC], c[STEPS][VEC], v[STEPS][VEC];
+        load_packs<T, VEC, STEPS>(z + l.b * s.zsb + l.d + t0 * s.zst, s.zst, full, left, a);
+        load_packs<T, VEC, STEPS>(x + l.b * s.xsb + l.d + t0 * s.xst, s.xst, full, left, v);
+        make_gates<VEC, STEPS>(full, left, a, c);
+#pragma unroll
+        for (int i = 0; i < STEPS; ++i)
+#pragma unroll
+            for (int k = 0; k < VEC; ++k) v[i][k] *= c[i][k];
+        if (states != nullptr && l.wt == 0 && l.in)
+#pragma unroll
+            for (int k = 0; k < VEC; ++k) states[tile * s.channels + l.c + k] = carry[k];
+        float h[VEC];
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) h[k] = carry[k];
+        if (s.WT > 1) {
+            Map<VEC> m;
+#pragma unroll
+            for (int k = 0; k < VEC; ++k) {
+                float ra = 1.f, rh = 0.f;
+#pragma unroll
+                for (int i = 0; i < STEPS; ++i) {
+                    rh = a[i][k] * rh + v[i][k];
+                    ra *= a[i][k];
+                }
+                m.A[k] = ra, m.H[k] = rh;
+            }
+            Map<VEC>(*buf)[32] = sh[tile & 1];
+            buf[l.row][l.lane] = m;
             __syncthreads();
             for (int w = 0; w < s.WT; ++w) {
-                if (w == l.wt) h = carry;
-                const float2 q = buf[l.wc * s.WT + w][l.lane];
-                carry = q.x * carry + q.y;
+                const Map<VEC> q = buf[l.row - l.wt + w][l.lane];
+#pragma unroll
+                for (int k = 0; k < VEC; ++k) {
+                    if (w == l.wt) h[k] = carry[k];
+                    carry[k] = q.A[k] * carry[k] + q.H[k];
+                }
             }
-        } else {
-#pragma unroll
-            for (int i = 0; i < STEPS; ++i) v[i] *= c[i];
         }
-        T *op = out + (l.b * s.T + t0) * s.D + l.d;
 #pragma unroll
-        for (int i = 0; i < STEPS; ++i) {
-            h = a[i] * h + v[i];
-            if (l.in && t0 + i < s.T) scan_store(op + i * s.D, t0 + i < l.len ? h : 0.f);
-        }
-        if (s.WT == 1) carry = h;
+        for (int i = 0; i < STEPS; ++i)
+#pragma unroll
+            for (int k = 0; k < VEC; ++k) {
+                h[k] = a[i][k] * h[k] + v[i][k];
+                v[i][k] = full || i < left ? h[k] : 0.f;
+            }
+        if (s.WT == 1)
+#pragma unroll
+            for (int k = 0; k < VEC; ++k) carry[k] = h[k];
+        store_packs<T, VEC, STEPS>(out + (l.b * s.T + t0) * s.D + l.d, s.D, full, l.in ? s.T - t0 : 0, v);
     }
-    if (seg == s.segments - 1 && l.wt == 0 && l.in) h_last[l.c] = carry;
+    if (seg == s.segments - 1 && l.wt == 0 && l.in)
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) h_last[l.c + k] = carry[k];
 }
 
 // Segment fold of the backward recurrence: agg[segment][channel] = (A, L), the map of the gradient that arrives from the right.
-template <typename T, int STEPS>
-__global__ void __launch_bounds__(512) k_scan_bwd_fold(const T *__restrict__ gh, const T *__restrict__ z, const int32_t *__restrict__ lengths,
+template <typename T, int VEC, int STEPS>
+__global__ void __launch_bounds__(256) k_scan_bwd_fold(const T *__restrict__ gh, const T *__restrict__ z, const int32_t *__restrict__ lengths,
                                                        const ScanDims s, float2 *__restrict__ agg) {
-    __shared__ float2 sh[2][kScanMaxWarps][32];
-    const Lane l = scan_lane(s, lengths);
+    __shared__ Map<VEC> sh[2][kScanMaxWarps][32];
+    const Lane l = scan_lane<VEC>(s, lengths);
     const int seg = blockIdx.y;
     const int64_t first = seg * s.tiles_per_segment, last = min(s.tiles, first + s.tiles_per_segment);
-    ScanDims sg = s;
-    sg.xsb = s.gsb, sg.xst = s.gst;
-    float A = 1.f, L = 0.f;
-    for (int64_t tile = last - 1; tile >= first; --tile) {
-        float a[STEPS], c[STEPS], g[STEPS];
-        load_run<T, STEPS>(gh, z, sg, l, (tile * s.WT + l.wt) * STEPS, a, c, g);
-        float ra = 1.f, rl = 0.f;
+    float A[VEC], L[VEC];
 #pragma unroll
-        for (int i = STEPS - 1; i >= 0; --i) {
-            rl = a[i] * (g[i] + rl);
-            ra *= a[i];
+    for (int k = 0; k < VEC; ++k) A[k] = 1.f, L[k] = 0.f;
+    for (int64_t tile = last - 1; tile >= first; --tile) {
+        const int64_t t0 = (tile * s.WT + l.wt) * STEPS, left = l.len - t0;
+        const bool full = __all_sync(0xffffffffu, left >= STEPS);
+        float a[STEPS][VEC], c[STEPS][VEC], g[STEPS][VEC];
+        load_packs<T, VEC, STEPS>(z + l.b * s.zsb + l.d + t0 * s.zst, s.zst, full, left, a);
+        load_packs<T, VEC, STEPS>(gh + l.b * s.gsb + l.d + t0 * s.gst, s.gst, full && gh != nullptr, gh != nullptr ? left : 0, g);
+        make_gates<VEC, STEPS>(full, left, a, c);
+        Map<VEC> m;
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) {
+            float ra = 1.f, rl = 0.f;
+#pragma unroll
+            for (int i = STEPS - 1; i >= 0; --i) {
+                rl = a[i][k] * (g[i][k] + rl);
+                ra *= a[i][k];
+            }
+            m.A[k] = ra, m.H[k] = rl;
         }
-        float2(*buf)[32] = sh[tile & 1];
-        buf[l.wc * s.WT + l.wt][l.lane] = make_float2(ra, rl);
+        Map<VEC>(*buf)[32] = sh[tile & 1];
+        buf[l.row][l.lane] = m;
         __syncthreads();
         if (l.wt == 0)
             for (int w = s.WT - 1; w >= 0; --w) {
-                const float2 q = buf[l.wc * s.WT + w][l.lane];
-                L = q.x * L + q.y;
-                A *= q.x;
+                const Map<VEC> q = buf[l.row + w][l.lane];
+#pragma unroll
+                for (int k = 0; k < VEC; ++k) {
+                    L[k] = q.A[k] * L[k] + q.H[k];
+                    A[k] *= q.A[k];
+                }
             }
     }
-    if (l.wt == 0 && l.in) agg[(int64_t)seg * s.channels + l.c] = make_float2(A, L);
+    if (l.wt == 0 && l.in)
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) agg[(int64_t)seg * s.channels + l.c + k] = make_float2(A[k], L[k]);
 }
 
-template <typename T, int STEPS>
-__global__ void __launch_bounds__(512) k_scan_bwd(const T *__restrict__ gh, const T *__restrict__ x, const T *__restrict__ z,
+template <typename T, int VEC, int STEPS>
+__global__ void __launch_bounds__(256, VEC == 2 ? 2 : 3) k_scan_bwd(const T *__restrict__ gh, const T *__restrict__ x, const T *__restrict__ z,
                                                   const float *__restrict__ h0, const int32_t *__restrict__ lengths,
                                                   const float *__restrict__ states, const float *__restrict__ g_last, const ScanDims s,
                                                   const float2 *__restrict__ agg, T *__restrict__ dx, T *__restrict__ dz,
                                                   float *__restrict__ dh0) {
-    __shared__ float2 sh[2][kScanMaxWarps][32];
-    __shared__ float shl[2][kScanMaxWarps][32];
-    const Lane l = scan_lane(s, lengths);
-    const int seg = blockIdx.y;
+    __shared__ Map<VEC> sh[2][kScanMaxWarps][32];
+    __shared__ float shl[2][kScanMaxWarps][VEC][32];
+    const Lane l = scan_lane<VEC>(s, lengths);
+    const int seg = blockIdx.y;  // the fold went through the segments in this order too, each from its end
     const int64_t first = seg * s.tiles_per_segment, last = min(s.tiles, first + s.tiles_per_segment);
-    float mu = (l.in && g_last != nullptr) ? g_last[l.c] : 0.f;  // gradient of the state behind the tile
+    float mu[VEC];  // gradient of the state behind the tile
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) mu[k] = (l.in && g_last != nullptr) ? g_last[l.c + k] : 0.f;
     if (l.in)
-        for (int k = s.segments - 1; k > seg; --k) {
-            const float2 q = agg[(int64_t)k * s.channels + l.c];
-            mu = q.x * mu + q.y;
-        }
-    for (int64_t tile = last - 1; tile >= first; --tile) {
-        const int64_t t0 = (tile * s.WT + l.wt) * STEPS;
-        float a[STEPS], c[STEPS], v[STEPS], g[STEPS];
-        load_run<T, STEPS>(x, z, s, l, t0, a, c, v);
-        const T *gp = gh + l.b * s.gsb + l.d + t0 * s.gst;
+#pragma unroll 4
+        for (int j = s.segments - 1; j > seg; --j)
 #pragma unroll
-        for (int i = 0; i < STEPS; ++i) g[i] = gh != nullptr && t0 + i < l.len ? scan_float(gp[i * s.gst]) : 0.f;
-        float h = 0.f;
-        if (l.in) h = states != nullptr ? states[tile * s.channels + l.c] : (h0 != nullptr ? h0[l.c] : 0.f);
-        float m = mu;
-        if (s.WT > 1) {
-            float ra = 1.f, rh = 0.f, rl = 0.f;
-#pragma unroll
-            for (int i = 0; i < STEPS; ++i) {
-                rh = a[i] * rh + c[i] * v[i];
-                ra *= a[i];
+            for (int k = 0; k < VEC; ++k) {
+                const float2 q = agg[(int64_t)j * s.channels + l.c + k];
+                mu[k] = q.x * mu[k] + q.y;
             }
+    for (int64_t tile = last - 1; tile >= first; --tile) {
+        const int64_t t0 = (tile * s.WT + l.wt) * STEPS, left = l.len - t0;
+        const bool full = __all_sync(0xffffffffu, left >= STEPS);
+        float a[STEPS][VEC], c[STEPS][VEC], v[STEPS][VEC], g[STEPS][VEC], h[VEC];
+        load_packs<T, VEC, STEPS>(z + l.b * s.zsb + l.d + t0 * s.zst, s.zst, full, left, a);
+        load_packs<T, VEC, STEPS>(x + l.b * s.xsb + l.d + t0 * s.xst, s.xst, full, left, v);
+        load_packs<T, VEC, STEPS>(gh + l.b * s.gsb + l.d + t0 * s.gst, s.gst, full && gh != nullptr, gh != nullptr ? left : 0, g);
 #pragma unroll
-            for (int i = STEPS - 1; i >= 0; --i) rl = a[i] * (g[i] + rl);
-            const int row = l.wc * s.WT + l.wt, buf = (int)(tile & 1);
-            sh[buf][row][l.lane] = make_float2(ra, rh);
-            shl[buf][row][l.lane] = rl;
+        for (int k = 0; k < VEC; ++k) {
+            h[k] = 0.f;
+            if (l.in) h[k] = states != nullptr ? states[tile * s.channels + l.c + k] : (h0 != nullptr ? h0[l.c + k] : 0.f);
+        }
+        make_gates<VEC, STEPS>(full, left, a, c);
+        float m[VEC];
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) m[k] = mu[k];
+        if (s.WT > 1) {
+            Map<VEC> run;
+            const int buf = (int)(tile & 1), base = l.row - l.wt;
+#pragma unroll
+            for (int k = 0; k < VEC; ++k) {
+                float ra = 1.f, rh = 0.f, rl = 0.f;
+#pragma unroll
+                for (int i = 0; i < STEPS; ++i) {
+                    rh = a[i][k] * rh + c[i][k] * v[i][k];
+                    ra *= a[i][k];
+                }
+#pragma unroll
+                for (int i = STEPS - 1; i >= 0; --i) rl = a[i][k] * (g[i][k] + rl);
+                run.A[k] = ra, run.H[k] = rh;
+                shl[buf][l.row][k][l.lane] = rl;
+            }
+            sh[buf][l.row][l.lane] = run;
             __syncthreads();
             for (int w = 0; w < l.wt; ++w) {
-                const float2 q = sh[buf][l.wc * s.WT + w][l.lane];
-                h = q.x * h + q.y;
+                const Map<VEC> q = sh[buf][base + w][l.lane];
+#pragma unroll
+                for (int k = 0; k < VEC; ++k) h[k] = q.A[k] * h[k] + q.H[k];
             }
-            for (int w = s.WT - 1; w >= 0; --w) {
-                if (w == l.wt) m = mu;
-                mu = sh[buf][l.wc * s.WT + w][l.lane].x * mu + shl[buf][l.wc * s.WT + w][l.lane];
-            }
+            for (int w = s.WT - 1; w >= 0; --w)
+#pragma unroll
+                for (int k = 0; k < VEC; ++k) {
+                    if (w == l.wt) m[k] = mu[k];
+                    mu[k] = sh[buf][base + w][l.lane].A[k] * mu[k] + shl[buf][base + w][k][l.lane];
+                }
         }
 #pragma unroll
-        for (int i = 0; i < STEPS; ++i) {
-            const float d = h - v[i];
-            h = a[i] * h + c[i] * v[i];
-            v[i] = d;
-        }
-        T *dxp = dx + l.b * s.dxb + t0 * s.dxt + l.d, *dzp = dz + l.b * s.dzb + t0 * s.dzt + l.d;
+        for (int i = 0; i < STEPS; ++i)
 #pragma unroll
-        for (int i = STEPS - 1; i >= 0; --i) {
-            const float lam = g[i] + m;
-            const float gx = c[i] * lam;
-            m = a[i] * lam;
-            if (l.in && t0 + i < s.T) {
-                const bool live = t0 + i < l.len;
-                scan_store(dxp + i * s.dxt, live ? gx : 0.f);
-                scan_store(dzp + i * s.dzt, live ? a[i] * gx * v[i] : 0.f);
+            for (int k = 0; k < VEC; ++k) {
+                const float d = h[k] - v[i][k];
+                h[k] = a[i][k] * h[k] + c[i][k] * v[i][k];
+                v[i][k] = d;
             }
-        }
-        if (s.WT == 1) mu = m;
+#pragma unroll
+        for (int i = STEPS - 1; i >= 0; --i)
+#pragma unroll
+            for (int k = 0; k < VEC; ++k) {
+                const float lam = g[i][k] + m[k];
+                const float gx = c[i][k] * lam;
+                m[k] = a[i][k] * lam;
+                const bool live = full || i < left;
+                v[i][k] = live ? a[i][k] * gx * v[i][k] : 0.f;
+                g[i][k] = live ? gx : 0.f;
+            }
+        if (s.WT == 1)
+#pragma unroll
+            for (int k = 0; k < VEC; ++k) mu[k] = m[k];
+        const int64_t rest = l.in ? s.T - t0 : 0;
+        store_packs<T, VEC, STEPS>(dx + l.b * s.dxb + l.d + t0 * s.dxt, s.dxt, full, rest, g);
+        store_packs<T, VEC, STEPS>(dz + l.b * s.dzb + l.d + t0 * s.dzt, s.dzt, full, rest, v);
     }
-    if (seg == 0 && l.wt == 0 && l.in && dh0 != nullptr) dh0[l.c] = mu;
+    if (seg == 0 && l.wt == 0 && l.in && dh0 != nullptr)
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) dh0[l.c + k] = mu[k];
 }
 
+// Tile geometry.  It depends on the shape alone (not on alignment), because the backward pass reads the states that the forward
+// pass laid down; VEC only says how many channels a lane takes.
 static int scan_steps(int64_t T) { return T == 1 ? 1 : kScanSteps; }
 
 static ScanDims scan_dims(int64_t B, int64_t T, int64_t D) {
@@ -296,19 +441,30 @@ static ScanDims scan_dims(int64_t B, int64_t T, int64_t D) {
     const int64_t runs = (T + steps - 1) / steps;
     s.WT = 1;
     while (s.WT < runs && s.WT < kScanMaxWarps) s.WT <<= 1;
-    s.WC = s.WT < 8 ? 8 / s.WT : 1;
+    s.WC = 8 / s.WT;
     s.tiles = (runs + s.WT - 1) / s.WT;
-    const int64_t ctas = (s.channels + 32 * s.WC - 1) / (32 * s.WC);
+    // Cut the axis when the channels alone do not give every SM a CTA; 4 CTAs of 256 threads an SM is what their registers allow.
+    const int64_t ctas = (s.channels + 64 * s.WC - 1) / (64 * s.WC);
     const int64_t sms = num_sms();
     int64_t segments = 1;
     if (ctas < sms && s.tiles > 1) {
-        segments = (4 * sms + ctas - 1) / ctas;
+        segments = 4 * sms / ctas;
         if (segments > kScanMaxSegments) segments = kScanMaxSegments;
         if (segments > s.tiles) segments = s.tiles;
     }
     s.tiles_per_segment = s.tiles > 0 ? (s.tiles + segments - 1) / segments : 0;
     s.segments = s.tiles > 0 ? (int)((s.tiles + s.tiles_per_segment - 1) / s.tiles_per_segment) : 1;
     return s;
+}
+
+// Two neighbouring channels as one access: an even number of features, strides and addresses that keep every pair aligned.
+static bool scan_pairs(int64_t D, size_t size, std::initializer_list<const void *> ptrs, std::initializer_list<int64_t> strides) {
+    if (D % 2 != 0) return false;
+    for (const void *p : ptrs)
+        if (!aligned(p, 2 * size)) return false;
+    for (int64_t st : strides)
+        if (st % 2 != 0) return false;
+    return true;
 }
 
 static int scan_args(int64_t B, int64_t T, int64_t D, int type) {
@@ -337,39 +493,44 @@ extern "C" int64_t hgq_gated_scan_states(int64_t B, int64_t T, int64_t D) {
 
 namespace {
 
-template <typename T>
+template <typename T, int VEC>
 int scan_fwd(const ScanDims &s, const void *x, const void *z, const float *h0, const int32_t *lengths, void *h, float *h_last, float *states,
              float2 *agg, cudaStream_t st) {
-    const dim3 grid((unsigned)((s.channels + 32 * s.WC - 1) / (32 * s.WC)), (unsigned)s.segments);
+    const dim3 grid((unsigned)((s.channels + 32 * VEC * s.WC - 1) / (32 * VEC * s.WC)), (unsigned)s.segments);
     const unsigned threads = 32 * s.WT * s.WC;
+    const T *px = (const T *)x, *pz = (const T *)z;
     if (s.segments > 1) {
-        k_scan_fold<T, kScanSteps><<<grid, threads, 0, st>>>((const T *)x, (const T *)z, lengths, s, agg);
+        k_scan_fold<T, VEC, kScanSteps><<<grid, threads, 0, st>>>(px, pz, lengths, s, agg);
         if (int e = check_launch()) return e;
     }
-    if (s.T == 1) k_scan_fwd<T, 1><<<grid, threads, 0, st>>>((const T *)x, (const T *)z, h0, lengths, s, agg, (T *)h, h_last, states);
-    else k_scan_fwd<T, kScanSteps><<<grid, threads, 0, st>>>((const T *)x, (const T *)z, h0, lengths, s, agg, (T *)h, h_last, states);
+    if (s.T == 1) k_scan_fwd<T, VEC, 1><<<grid, threads, 0, st>>>(px, pz, h0, lengths, s, agg, (T *)h, h_last, states);
+    else k_scan_fwd<T, VEC, kScanSteps><<<grid, threads, 0, st>>>(px, pz, h0, lengths, s, agg, (T *)h, h_last, states);
     return check_launch();
 }
 
-template <typename T>
+template <typename T, int VEC>
 int scan_bwd(const ScanDims &s, const void *gh, const void *x, const void *z, const float *h0, const int32_t *lengths, const float *states,
              const float *g_last, void *dx, void *dz, float *dh0, float2 *agg, cudaStream_t st) {
-    const dim3 grid((unsigned)((s.channels + 32 * s.WC - 1) / (32 * s.WC)), (unsigned)s.segments);
+    const dim3 grid((unsigned)((s.channels + 32 * VEC * s.WC - 1) / (32 * VEC * s.WC)), (unsigned)s.segments);
     const unsigned threads = 32 * s.WT * s.WC;
+    const T *pg = (const T *)gh, *px = (const T *)x, *pz = (const T *)z;
     if (s.segments > 1) {
-        k_scan_bwd_fold<T, kScanSteps><<<grid, threads, 0, st>>>((const T *)gh, (const T *)z, lengths, s, agg);
+        k_scan_bwd_fold<T, VEC, kScanSteps><<<grid, threads, 0, st>>>(pg, pz, lengths, s, agg);
         if (int e = check_launch()) return e;
     }
-    if (s.T == 1)
-        k_scan_bwd<T, 1><<<grid, threads, 0, st>>>((const T *)gh, (const T *)x, (const T *)z, h0, lengths, states, g_last, s, agg, (T *)dx,
-                                                  (T *)dz, dh0);
-    else
-        k_scan_bwd<T, kScanSteps><<<grid, threads, 0, st>>>((const T *)gh, (const T *)x, (const T *)z, h0, lengths, states, g_last, s, agg,
-                                                           (T *)dx, (T *)dz, dh0);
+    if (s.T == 1) k_scan_bwd<T, VEC, 1><<<grid, threads, 0, st>>>(pg, px, pz, h0, lengths, states, g_last, s, agg, (T *)dx, (T *)dz, dh0);
+    else k_scan_bwd<T, VEC, kScanSteps><<<grid, threads, 0, st>>>(pg, px, pz, h0, lengths, states, g_last, s, agg, (T *)dx, (T *)dz, dh0);
     return check_launch();
 }
 
 }  // namespace
+
+#define SCAN_DISPATCH(FN, ...)                                                       \
+    do {                                                                             \
+        if (type == HGQ_TYPE_F32) return pairs ? FN<float, 2>(__VA_ARGS__) : FN<float, 1>(__VA_ARGS__); \
+        if (type == HGQ_TYPE_BF16) return pairs ? FN<__nv_bfloat16, 2>(__VA_ARGS__) : FN<__nv_bfloat16, 1>(__VA_ARGS__); \
+        return pairs ? FN<__half, 2>(__VA_ARGS__) : FN<__half, 1>(__VA_ARGS__);      \
+    } while (0)
 
 extern "C" int hgq_gated_scan_fwd(const void *x, int64_t x_batch, int64_t x_time, const void *z, int64_t z_batch, int64_t z_time,
                                   const float *h0, const int32_t *lengths, void *h, float *h_last, float *states, int64_t B, int64_t T,
@@ -389,9 +550,8 @@ extern "C" int hgq_gated_scan_fwd(const void *x, int64_t x_batch, int64_t x_time
     if (s.tiles <= 1) states = nullptr;
     cudaStream_t st = (cudaStream_t)stream;
     float2 *agg = (float2 *)workspace;
-    if (type == HGQ_TYPE_F32) return scan_fwd<float>(s, x, z, h0, lengths, h, h_last, states, agg, st);
-    if (type == HGQ_TYPE_BF16) return scan_fwd<__nv_bfloat16>(s, x, z, h0, lengths, h, h_last, states, agg, st);
-    return scan_fwd<__half>(s, x, z, h0, lengths, h, h_last, states, agg, st);
+    const bool pairs = scan_pairs(D, size, {x, z, h}, {x_batch, x_time, z_batch, z_time});
+    SCAN_DISPATCH(scan_fwd, s, x, z, h0, lengths, h, h_last, states, agg, st);
 }
 
 extern "C" int hgq_gated_scan_bwd(const void *gh, int64_t g_batch, int64_t g_time, const void *x, int64_t x_batch, int64_t x_time,
@@ -416,7 +576,6 @@ extern "C" int hgq_gated_scan_bwd(const void *gh, int64_t g_batch, int64_t g_tim
     if (s.tiles <= 1) states = nullptr;
     cudaStream_t st = (cudaStream_t)stream;
     float2 *agg = (float2 *)workspace;
-    if (type == HGQ_TYPE_F32) return scan_bwd<float>(s, gh, x, z, h0, lengths, states, g_last, dx, dz, dh0, agg, st);
-    if (type == HGQ_TYPE_BF16) return scan_bwd<__nv_bfloat16>(s, gh, x, z, h0, lengths, states, g_last, dx, dz, dh0, agg, st);
-    return scan_bwd<__half>(s, gh, x, z, h0, lengths, states, g_last, dx, dz, dh0, agg, st);
+    const bool pairs = scan_pairs(D, size, {gh, x, z, dx, dz}, {g_batch, g_time, x_batch, x_time, z_batch, z_time, dx_batch, dx_time, dz_batch, dz_time});
+    SCAN_DISPATCH(scan_bwd, s, gh, x, z, h0, lengths, states, g_last, dx, dz, dh0, agg, st);
 }
