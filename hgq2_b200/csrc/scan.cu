@@ -37,6 +37,7 @@ namespace hgq {
 constexpr int kScanSteps = 8;
 constexpr int kScanMaxWarps = 8;  // along time
 constexpr int kScanMaxSegments = 128;
+constexpr int kFwdCtas = 3, kBwdCtas = 2;  // CTAs of 256 threads an SM, by their registers
 
 __device__ __forceinline__ float scan_float(float v) { return v; }
 __device__ __forceinline__ float scan_float(__nv_bfloat16 v) { return __bfloat162float(v); }
@@ -59,20 +60,31 @@ struct ScanDims {
     int segments;
 };
 
-// a = sigmoid(z) = 1 / (1 + e) with e = exp(-z), and c = 1 - a = e / (1 + e), each to full relative precision: c is formed as 1 - a
-// only where a < 1/2.  z is held in [-88, 100], where the gates are 0 and 1 in fp32; a NaN stays.  The exponential is
-// 2^(-z log2 e) with the rounding error of the product carried along, the reciprocal's error is one ulp.
+// a = sigmoid(z) = 1 / (1 + e) with e = exp(-z), and c = 1 - a = e / (1 + e), each to full relative precision (c is not the
+// difference where a is near 1).  fp32: z is held in [-88, 100], where the gates are 0 and 1; the exponential is 2^(-z log2 e) with
+// the rounding error of the product carried along, the reciprocal's error is one ulp.  bf16 and fp16: z has at most 11 bits and
+// the outputs no more, the product's rounding (|z| 2^-24 of e) is far below both; a closed gate is 2^-126.  A NaN stays.
+template <typename T>
 __device__ __forceinline__ void gates(float z, float &a, float &c) {
     float e, r;
-    asm("max.NaN.f32 %0, %0, 0fC2B00000;" : "+f"(z));
-    asm("min.NaN.f32 %0, %0, 0f42C80000;" : "+f"(z));
-    const float t = z * -1.44269504088896341f;
-    const float lo = fmaf(z, -1.44269504088896341f, -t);
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(t));
-    e = fmaf(e, lo * 0.693147180559945309f, e);
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + e));
-    a = r;
-    c = z < 0.f ? 1.f - r : e * r;
+    if (sizeof(T) == 4) {
+        asm("max.NaN.f32 %0, %0, 0fC2B00000;" : "+f"(z));
+        asm("min.NaN.f32 %0, %0, 0f42C80000;" : "+f"(z));
+        const float t = z * -1.44269504088896341f;
+        const float lo = fmaf(z, -1.44269504088896341f, -t);
+        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(t));
+        e = fmaf(e, lo * 0.693147180559945309f, e);
+        asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + e));
+        a = r;
+        c = z < 0.f ? 1.f - r : e * r;
+    } else {
+        float t = z * -1.44269504088896341f;
+        asm("min.NaN.f32 %0, %0, 0f42FC0000;" : "+f"(t));  // 126
+        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(t));
+        asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + e));
+        a = r;
+        c = e * r;
+    }
 }
 
 struct Lane {
@@ -83,13 +95,13 @@ struct Lane {
 };
 
 template <int VEC>
-__device__ __forceinline__ Lane scan_lane(const ScanDims &s, const int32_t *lengths) {
+__device__ __forceinline__ Lane scan_lane(const ScanDims &s, int WT, const int32_t *lengths) {
     Lane l;
     const int w = threadIdx.x >> 5;
     l.lane = threadIdx.x & 31;
-    l.wt = w % s.WT;
+    l.wt = w % WT;
     l.row = w;
-    l.c = (((int64_t)blockIdx.x * s.WC + w / s.WT) * 32 + l.lane) * VEC;
+    l.c = (((int64_t)blockIdx.x * s.WC + w / WT) * 32 + l.lane) * VEC;
     l.in = l.c < s.channels;
     l.b = l.in ? l.c / s.D : 0;
     l.d = l.in ? l.c - l.b * s.D : 0;
@@ -101,7 +113,8 @@ __device__ __forceinline__ Lane scan_lane(const ScanDims &s, const int32_t *leng
     return l;
 }
 
-// STEPS packs of a strided sequence from step t0; steps that are not live read as zero.  p: the lane's channel at step t0.
+// STEPS packs of a strided sequence as fp32; p: the lane's channel at the first of them, `left`: how many of them are live (the
+// others read as zero).
 template <typename T, int VEC, int STEPS>
 __device__ __forceinline__ void load_packs(const T *__restrict__ p, int64_t stride, bool full, int64_t left, float (&v)[STEPS][VEC]) {
     using P = ScanPack<T, VEC>;
@@ -109,23 +122,58 @@ __device__ __forceinline__ void load_packs(const T *__restrict__ p, int64_t stri
     if (full) {
 #pragma unroll
         for (int i = 0; i < STEPS; ++i, p += stride) q[i] = *reinterpret_cast<const P *>(p);
-#pragma unroll
-        for (int i = 0; i < STEPS; ++i)
-#pragma unroll
-            for (int k = 0; k < VEC; ++k) v[i][k] = scan_float(q[i].v[k]);
     } else {
 #pragma unroll
         for (int i = 0; i < STEPS; ++i, p += stride) {
 #pragma unroll
-            for (int k = 0; k < VEC; ++k) v[i][k] = 0.f;
-            if (i < left) {
-                q[i] = *reinterpret_cast<const P *>(p);
-#pragma unroll
-                for (int k = 0; k < VEC; ++k) v[i][k] = scan_float(q[i].v[k]);
-            }
+            for (int k = 0; k < VEC; ++k) scan_round(0.f, q[i].v[k]);
+            if (i < left) q[i] = *reinterpret_cast<const P *>(p);
         }
     }
+#pragma unroll
+    for (int i = 0; i < STEPS; ++i)
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) v[i][k] = scan_float(q[i].v[k]);
 }
+
+// The same through shared memory, fetched a tile ahead: every lane copies and later reads its own packs (no barrier), a copy
+// whose step is not live writes zeros.  Registers would hold the next tile's packs as well, at the price of spills.
+template <typename T, int VEC, int STEPS>
+__device__ __forceinline__ void fetch_packs(ScanPack<T, VEC> *dst, const T *__restrict__ p, int64_t stride, bool full, int64_t left) {
+    constexpr int bytes = sizeof(T) * VEC;
+    static_assert(bytes == 4 || bytes == 8, "copies of 4 or 8 bytes");
+    uint32_t d = (uint32_t)__cvta_generic_to_shared(dst);
+#pragma unroll
+    for (int i = 0; i < STEPS; ++i, d += 32 * bytes, p += stride) {
+        if (full || i < left) asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(d), "l"(p), "n"(bytes) : "memory");
+        else dst[i * 32] = ScanPack<T, VEC>{};
+    }
+}
+
+template <typename T, int VEC, int STEPS>
+__device__ __forceinline__ void staged_packs(const ScanPack<T, VEC> *src, float (&v)[STEPS][VEC]) {
+#pragma unroll
+    for (int i = 0; i < STEPS; ++i) {
+        const ScanPack<T, VEC> q = src[i * 32];
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) v[i][k] = scan_float(q.v[k]);
+    }
+}
+
+// One tile's packs of N sequences, the next tile's on the way while this one's are used.
+template <typename T, int VEC, int STEPS, int N, bool AHEAD>
+struct Stages {
+    using P = ScanPack<T, VEC>;
+    P *base;  // this lane's column of its warp's buffers: [2][N][STEPS][32]
+
+    __device__ __forceinline__ explicit Stages(unsigned char *smem) {
+        base = reinterpret_cast<P *>(smem) + (threadIdx.x >> 5) * (2 * N * STEPS * 32) + (threadIdx.x & 31);
+    }
+    __device__ __forceinline__ P *at(int64_t tile, int n) const { return base + ((tile & 1) * N + n) * STEPS * 32; }
+    static __device__ __forceinline__ void commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+    static __device__ __forceinline__ void wait_but_newest() { asm volatile("cp.async.wait_group 1;" ::: "memory"); }
+    static __device__ __forceinline__ void wait_all() { asm volatile("cp.async.wait_group 0;" ::: "memory"); }
+};
 
 template <typename T, int VEC, int STEPS>
 __device__ __forceinline__ void store_packs(T *p, int64_t stride, bool full, int64_t left, const float (&v)[STEPS][VEC]) {
@@ -139,12 +187,12 @@ __device__ __forceinline__ void store_packs(T *p, int64_t stride, bool full, int
     }
 }
 
-template <int VEC, int STEPS>
+template <typename T, int VEC, int STEPS>
 __device__ __forceinline__ void make_gates(bool full, int64_t left, float (&a)[STEPS][VEC], float (&c)[STEPS][VEC]) {
 #pragma unroll
     for (int i = 0; i < STEPS; ++i)
 #pragma unroll
-        for (int k = 0; k < VEC; ++k) gates(a[i][k], a[i][k], c[i][k]);
+        for (int k = 0; k < VEC; ++k) gates<T>(a[i][k], a[i][k], c[i][k]);
     if (!full) {
 #pragma unroll
         for (int i = 0; i < STEPS; ++i)
@@ -161,23 +209,47 @@ struct alignas(8 * VEC) Map {  // h -> A h + H for VEC channels
 };
 
 // Segment fold of the forward recurrence: agg[segment][channel] = (A, H).
-template <typename T, int VEC, int STEPS>
+template <typename T, int VEC, int STEPS, int WARPS, bool AHEAD>
 __global__ void __launch_bounds__(256) k_scan_fold(const T *__restrict__ x, const T *__restrict__ z, const int32_t *__restrict__ lengths,
                                                    const ScanDims s, float2 *__restrict__ agg) {
     __shared__ Map<VEC> sh[2][kScanMaxWarps][32];
-    const Lane l = scan_lane<VEC>(s, lengths);
+    const int WT = WARPS > 0 ? WARPS : s.WT;
+    const Lane l = scan_lane<VEC>(s, WT, lengths);
     const int seg = blockIdx.y;
     const int64_t first = seg * s.tiles_per_segment, last = min(s.tiles, first + s.tiles_per_segment);
     float A[VEC], H[VEC];
 #pragma unroll
     for (int k = 0; k < VEC; ++k) A[k] = 1.f, H[k] = 0.f;
+    extern __shared__ __align__(16) unsigned char staging[];
+    const Stages<T, VEC, STEPS, 2, AHEAD> stages(staging);
+    [[maybe_unused]] auto fetch = [&](auto tile) {
+        const int64_t t0 = (tile * WT + l.wt) * STEPS, left = l.len - t0;
+        const bool full = __all_sync(0xffffffffu, left >= STEPS);
+        fetch_packs<T, VEC, STEPS>(stages.at(tile, 0), z + l.b * s.zsb + l.d + t0 * s.zst, s.zst, full, left);
+        fetch_packs<T, VEC, STEPS>(stages.at(tile, 1), x + l.b * s.xsb + l.d + t0 * s.xst, s.xst, full, left);
+        stages.commit();
+    };
+    if constexpr (AHEAD) {
+        if (first < last) fetch(first);
+    }
     for (int64_t tile = first; tile < last; ++tile) {
-        const int64_t t0 = (tile * s.WT + l.wt) * STEPS, left = l.len - t0;
+        const int64_t t0 = (tile * WT + l.wt) * STEPS, left = l.len - t0;
         const bool full = __all_sync(0xffffffffu, left >= STEPS);
         float a[STEPS][VEC], c[STEPS][VEC], v[STEPS][VEC];
-        load_packs<T, VEC, STEPS>(z + l.b * s.zsb + l.d + t0 * s.zst, s.zst, full, left, a);
-        load_packs<T, VEC, STEPS>(x + l.b * s.xsb + l.d + t0 * s.xst, s.xst, full, left, v);
-        make_gates<VEC, STEPS>(full, left, a, c);
+        if constexpr (AHEAD) {
+            if (tile + 1 < last) {
+                fetch(tile + 1);
+                stages.wait_but_newest();
+            } else {
+                stages.wait_all();
+            }
+            staged_packs<T, VEC, STEPS>(stages.at(tile, 0), a);
+            staged_packs<T, VEC, STEPS>(stages.at(tile, 1), v);
+        } else {
+            load_packs<T, VEC, STEPS>(z + l.b * s.zsb + l.d + t0 * s.zst, s.zst, full, left, a);
+            load_packs<T, VEC, STEPS>(x + l.b * s.xsb + l.d + t0 * s.xst, s.xst, full, left, v);
+        }
+        make_gates<T, VEC, STEPS>(full, left, a, c);
         Map<VEC> m;
 #pragma unroll
         for (int k = 0; k < VEC; ++k) {
@@ -193,7 +265,8 @@ __global__ void __launch_bounds__(256) k_scan_fold(const T *__restrict__ x, cons
         buf[l.row][l.lane] = m;
         __syncthreads();
         if (l.wt == 0)
-            for (int w = 0; w < s.WT; ++w) {
+#pragma unroll
+            for (int w = 0; w < WT; ++w) {
                 const Map<VEC> q = buf[l.row + w][l.lane];
 #pragma unroll
                 for (int k = 0; k < VEC; ++k) {
@@ -207,12 +280,13 @@ __global__ void __launch_bounds__(256) k_scan_fold(const T *__restrict__ x, cons
         for (int k = 0; k < VEC; ++k) agg[(int64_t)seg * s.channels + l.c + k] = make_float2(A[k], H[k]);
 }
 
-template <typename T, int VEC, int STEPS>
-__global__ void __launch_bounds__(256) k_scan_fwd(const T *__restrict__ x, const T *__restrict__ z, const float *__restrict__ h0,
+template <typename T, int VEC, int STEPS, int WARPS, bool AHEAD>
+__global__ void __launch_bounds__(256, VEC == 2 ? kFwdCtas : 4) k_scan_fwd(const T *__restrict__ x, const T *__restrict__ z, const float *__restrict__ h0,
                                                   const int32_t *__restrict__ lengths, const ScanDims s, const float2 *__restrict__ agg,
                                                   T *__restrict__ out, float *__restrict__ h_last, float *__restrict__ states) {
     __shared__ Map<VEC> sh[2][kScanMaxWarps][32];
-    const Lane l = scan_lane<VEC>(s, lengths);
+    const int WT = WARPS > 0 ? WARPS : s.WT;
+    const Lane l = scan_lane<VEC>(s, WT, lengths);
     const int seg = s.segments - 1 - blockIdx.y;
     const int64_t first = seg * s.tiles_per_segment, last = min(s.tiles, first + s.tiles_per_segment);
     float carry[VEC];
@@ -226,13 +300,36 @@ __global__ void __launch_bounds__(256) k_scan_fwd(const T *__restrict__ x, const
                 const float2 q = agg[(int64_t)j * s.channels + l.c + k];
                 carry[k] = q.x * carry[k] + q.y;
             }
+    extern __shared__ __align__(16) unsigned char staging[];
+    const Stages<T, VEC, STEPS, 2, AHEAD> stages(staging);
+    [[maybe_unused]] auto fetch = [&](auto tile) {
+        const int64_t t0 = (tile * WT + l.wt) * STEPS, left = l.len - t0;
+        const bool full = __all_sync(0xffffffffu, left >= STEPS);
+        fetch_packs<T, VEC, STEPS>(stages.at(tile, 0), z + l.b * s.zsb + l.d + t0 * s.zst, s.zst, full, left);
+        fetch_packs<T, VEC, STEPS>(stages.at(tile, 1), x + l.b * s.xsb + l.d + t0 * s.xst, s.xst, full, left);
+        stages.commit();
+    };
+    if constexpr (AHEAD) {
+        if (first < last) fetch(first);
+    }
     for (int64_t tile = first; tile < last; ++tile) {
-        const int64_t t0 = (tile * s.WT + l.wt) * STEPS, left = l.len - t0;
+        const int64_t t0 = (tile * WT + l.wt) * STEPS, left = l.len - t0;
         const bool full = __all_sync(0xffffffffu, left >= STEPS);
         float a[STEPS][VEC], c[STEPS][VEC], v[STEPS][VEC];
-        load_packs<T, VEC, STEPS>(z + l.b * s.zsb + l.d + t0 * s.zst, s.zst, full, left, a);
-        load_packs<T, VEC, STEPS>(x + l.b * s.xsb + l.d + t0 * s.xst, s.xst, full, left, v);
-        make_gates<VEC, STEPS>(full, left, a, c);
+        if constexpr (AHEAD) {
+            if (tile + 1 < last) {
+                fetch(tile + 1);
+                stages.wait_but_newest();
+            } else {
+                stages.wait_all();
+            }
+            staged_packs<T, VEC, STEPS>(stages.at(tile, 0), a);
+            staged_packs<T, VEC, STEPS>(stages.at(tile, 1), v);
+        } else {
+            load_packs<T, VEC, STEPS>(z + l.b * s.zsb + l.d + t0 * s.zst, s.zst, full, left, a);
+            load_packs<T, VEC, STEPS>(x + l.b * s.xsb + l.d + t0 * s.xst, s.xst, full, left, v);
+        }
+        make_gates<T, VEC, STEPS>(full, left, a, c);
 #pragma unroll
         for (int i = 0; i < STEPS; ++i)
 #pragma unroll
@@ -243,7 +340,7 @@ __global__ void __launch_bounds__(256) k_scan_fwd(const T *__restrict__ x, const
         float h[VEC];
 #pragma unroll
         for (int k = 0; k < VEC; ++k) h[k] = carry[k];
-        if (s.WT > 1) {
+        if (WT > 1) {
             Map<VEC> m;
 #pragma unroll
             for (int k = 0; k < VEC; ++k) {
@@ -258,7 +355,8 @@ __global__ void __launch_bounds__(256) k_scan_fwd(const T *__restrict__ x, const
             Map<VEC>(*buf)[32] = sh[tile & 1];
             buf[l.row][l.lane] = m;
             __syncthreads();
-            for (int w = 0; w < s.WT; ++w) {
+#pragma unroll
+            for (int w = 0; w < WT; ++w) {
                 const Map<VEC> q = buf[l.row - l.wt + w][l.lane];
 #pragma unroll
                 for (int k = 0; k < VEC; ++k) {
@@ -272,9 +370,14 @@ __global__ void __launch_bounds__(256) k_scan_fwd(const T *__restrict__ x, const
 #pragma unroll
             for (int k = 0; k < VEC; ++k) {
                 h[k] = a[i][k] * h[k] + v[i][k];
-                v[i][k] = full || i < left ? h[k] : 0.f;
+                v[i][k] = h[k];
             }
-        if (s.WT == 1)
+        if (!full)
+#pragma unroll
+            for (int i = 0; i < STEPS; ++i)
+#pragma unroll
+                for (int k = 0; k < VEC; ++k) v[i][k] = i < left ? v[i][k] : 0.f;
+        if (WT == 1)
 #pragma unroll
             for (int k = 0; k < VEC; ++k) carry[k] = h[k];
         store_packs<T, VEC, STEPS>(out + (l.b * s.T + t0) * s.D + l.d, s.D, full, l.in ? s.T - t0 : 0, v);
@@ -285,23 +388,47 @@ __global__ void __launch_bounds__(256) k_scan_fwd(const T *__restrict__ x, const
 }
 
 // Segment fold of the backward recurrence: agg[segment][channel] = (A, L), the map of the gradient that arrives from the right.
-template <typename T, int VEC, int STEPS>
+template <typename T, int VEC, int STEPS, int WARPS, bool AHEAD>
 __global__ void __launch_bounds__(256) k_scan_bwd_fold(const T *__restrict__ gh, const T *__restrict__ z, const int32_t *__restrict__ lengths,
                                                        const ScanDims s, float2 *__restrict__ agg) {
     __shared__ Map<VEC> sh[2][kScanMaxWarps][32];
-    const Lane l = scan_lane<VEC>(s, lengths);
+    const int WT = WARPS > 0 ? WARPS : s.WT;
+    const Lane l = scan_lane<VEC>(s, WT, lengths);
     const int seg = blockIdx.y;
     const int64_t first = seg * s.tiles_per_segment, last = min(s.tiles, first + s.tiles_per_segment);
     float A[VEC], L[VEC];
 #pragma unroll
     for (int k = 0; k < VEC; ++k) A[k] = 1.f, L[k] = 0.f;
+    extern __shared__ __align__(16) unsigned char staging[];
+    const Stages<T, VEC, STEPS, 2, AHEAD> stages(staging);
+    [[maybe_unused]] auto fetch = [&](auto tile) {
+        const int64_t t0 = (tile * WT + l.wt) * STEPS, left = l.len - t0;
+        const bool full = __all_sync(0xffffffffu, left >= STEPS);
+        fetch_packs<T, VEC, STEPS>(stages.at(tile, 0), z + l.b * s.zsb + l.d + t0 * s.zst, s.zst, full, left);
+        fetch_packs<T, VEC, STEPS>(stages.at(tile, 1), gh + l.b * s.gsb + l.d + t0 * s.gst, s.gst, full && gh != nullptr, gh != nullptr ? left : 0);
+        stages.commit();
+    };
+    if constexpr (AHEAD) {
+        if (first < last) fetch(last - 1);
+    }
     for (int64_t tile = last - 1; tile >= first; --tile) {
-        const int64_t t0 = (tile * s.WT + l.wt) * STEPS, left = l.len - t0;
+        const int64_t t0 = (tile * WT + l.wt) * STEPS, left = l.len - t0;
         const bool full = __all_sync(0xffffffffu, left >= STEPS);
         float a[STEPS][VEC], c[STEPS][VEC], g[STEPS][VEC];
-        load_packs<T, VEC, STEPS>(z + l.b * s.zsb + l.d + t0 * s.zst, s.zst, full, left, a);
-        load_packs<T, VEC, STEPS>(gh + l.b * s.gsb + l.d + t0 * s.gst, s.gst, full && gh != nullptr, gh != nullptr ? left : 0, g);
-        make_gates<VEC, STEPS>(full, left, a, c);
+        if constexpr (AHEAD) {
+            if (tile > first) {
+                fetch(tile - 1);
+                stages.wait_but_newest();
+            } else {
+                stages.wait_all();
+            }
+            staged_packs<T, VEC, STEPS>(stages.at(tile, 0), a);
+            staged_packs<T, VEC, STEPS>(stages.at(tile, 1), g);
+        } else {
+            load_packs<T, VEC, STEPS>(z + l.b * s.zsb + l.d + t0 * s.zst, s.zst, full, left, a);
+            load_packs<T, VEC, STEPS>(gh + l.b * s.gsb + l.d + t0 * s.gst, s.gst, full && gh != nullptr, gh != nullptr ? left : 0, g);
+        }
+        make_gates<T, VEC, STEPS>(full, left, a, c);
         Map<VEC> m;
 #pragma unroll
         for (int k = 0; k < VEC; ++k) {
@@ -317,7 +444,8 @@ __global__ void __launch_bounds__(256) k_scan_bwd_fold(const T *__restrict__ gh,
         buf[l.row][l.lane] = m;
         __syncthreads();
         if (l.wt == 0)
-            for (int w = s.WT - 1; w >= 0; --w) {
+#pragma unroll
+            for (int w = WT - 1; w >= 0; --w) {
                 const Map<VEC> q = buf[l.row + w][l.lane];
 #pragma unroll
                 for (int k = 0; k < VEC; ++k) {
@@ -331,15 +459,16 @@ __global__ void __launch_bounds__(256) k_scan_bwd_fold(const T *__restrict__ gh,
         for (int k = 0; k < VEC; ++k) agg[(int64_t)seg * s.channels + l.c + k] = make_float2(A[k], L[k]);
 }
 
-template <typename T, int VEC, int STEPS>
-__global__ void __launch_bounds__(256, VEC == 2 ? 2 : 3) k_scan_bwd(const T *__restrict__ gh, const T *__restrict__ x, const T *__restrict__ z,
+template <typename T, int VEC, int STEPS, int WARPS, bool AHEAD>
+__global__ void __launch_bounds__(256, VEC == 2 ? kBwdCtas : 3) k_scan_bwd(const T *__restrict__ gh, const T *__restrict__ x, const T *__restrict__ z,
                                                   const float *__restrict__ h0, const int32_t *__restrict__ lengths,
                                                   const float *__restrict__ states, const float *__restrict__ g_last, const ScanDims s,
                                                   const float2 *__restrict__ agg, T *__restrict__ dx, T *__restrict__ dz,
                                                   float *__restrict__ dh0) {
     __shared__ Map<VEC> sh[2][kScanMaxWarps][32];
     __shared__ float shl[2][kScanMaxWarps][VEC][32];
-    const Lane l = scan_lane<VEC>(s, lengths);
+    const int WT = WARPS > 0 ? WARPS : s.WT;
+    const Lane l = scan_lane<VEC>(s, WT, lengths);
     const int seg = blockIdx.y;  // the fold went through the segments in this order too, each from its end
     const int64_t first = seg * s.tiles_per_segment, last = min(s.tiles, first + s.tiles_per_segment);
     float mu[VEC];  // gradient of the state behind the tile
@@ -353,23 +482,48 @@ __global__ void __launch_bounds__(256, VEC == 2 ? 2 : 3) k_scan_bwd(const T *__r
                 const float2 q = agg[(int64_t)j * s.channels + l.c + k];
                 mu[k] = q.x * mu[k] + q.y;
             }
+    extern __shared__ __align__(16) unsigned char staging[];
+    const Stages<T, VEC, STEPS, 3, AHEAD> stages(staging);
+    [[maybe_unused]] auto fetch = [&](auto tile) {
+        const int64_t t0 = (tile * WT + l.wt) * STEPS, left = l.len - t0;
+        const bool full = __all_sync(0xffffffffu, left >= STEPS);
+        fetch_packs<T, VEC, STEPS>(stages.at(tile, 0), z + l.b * s.zsb + l.d + t0 * s.zst, s.zst, full, left);
+        fetch_packs<T, VEC, STEPS>(stages.at(tile, 1), x + l.b * s.xsb + l.d + t0 * s.xst, s.xst, full, left);
+        fetch_packs<T, VEC, STEPS>(stages.at(tile, 2), gh + l.b * s.gsb + l.d + t0 * s.gst, s.gst, full && gh != nullptr, gh != nullptr ? left : 0);
+        stages.commit();
+    };
+    if constexpr (AHEAD) {
+        if (first < last) fetch(last - 1);
+    }
     for (int64_t tile = last - 1; tile >= first; --tile) {
-        const int64_t t0 = (tile * s.WT + l.wt) * STEPS, left = l.len - t0;
+        const int64_t t0 = (tile * WT + l.wt) * STEPS, left = l.len - t0;
         const bool full = __all_sync(0xffffffffu, left >= STEPS);
         float a[STEPS][VEC], c[STEPS][VEC], v[STEPS][VEC], g[STEPS][VEC], h[VEC];
-        load_packs<T, VEC, STEPS>(z + l.b * s.zsb + l.d + t0 * s.zst, s.zst, full, left, a);
-        load_packs<T, VEC, STEPS>(x + l.b * s.xsb + l.d + t0 * s.xst, s.xst, full, left, v);
-        load_packs<T, VEC, STEPS>(gh + l.b * s.gsb + l.d + t0 * s.gst, s.gst, full && gh != nullptr, gh != nullptr ? left : 0, g);
+        if constexpr (AHEAD) {
+            if (tile > first) {
+                fetch(tile - 1);
+                stages.wait_but_newest();
+            } else {
+                stages.wait_all();
+            }
+            staged_packs<T, VEC, STEPS>(stages.at(tile, 0), a);
+            staged_packs<T, VEC, STEPS>(stages.at(tile, 1), v);
+            staged_packs<T, VEC, STEPS>(stages.at(tile, 2), g);
+        } else {
+            load_packs<T, VEC, STEPS>(z + l.b * s.zsb + l.d + t0 * s.zst, s.zst, full, left, a);
+            load_packs<T, VEC, STEPS>(x + l.b * s.xsb + l.d + t0 * s.xst, s.xst, full, left, v);
+            load_packs<T, VEC, STEPS>(gh + l.b * s.gsb + l.d + t0 * s.gst, s.gst, full && gh != nullptr, gh != nullptr ? left : 0, g);
+        }
 #pragma unroll
         for (int k = 0; k < VEC; ++k) {
             h[k] = 0.f;
             if (l.in) h[k] = states != nullptr ? states[tile * s.channels + l.c + k] : (h0 != nullptr ? h0[l.c + k] : 0.f);
         }
-        make_gates<VEC, STEPS>(full, left, a, c);
+        make_gates<T, VEC, STEPS>(full, left, a, c);
         float m[VEC];
 #pragma unroll
         for (int k = 0; k < VEC; ++k) m[k] = mu[k];
-        if (s.WT > 1) {
+        if (WT > 1) {
             Map<VEC> run;
             const int buf = (int)(tile & 1), base = l.row - l.wt;
 #pragma unroll
@@ -392,7 +546,8 @@ __global__ void __launch_bounds__(256, VEC == 2 ? 2 : 3) k_scan_bwd(const T *__r
 #pragma unroll
                 for (int k = 0; k < VEC; ++k) h[k] = q.A[k] * h[k] + q.H[k];
             }
-            for (int w = s.WT - 1; w >= 0; --w)
+#pragma unroll
+            for (int w = WT - 1; w >= 0; --w)
 #pragma unroll
                 for (int k = 0; k < VEC; ++k) {
                     if (w == l.wt) m[k] = mu[k];
@@ -414,11 +569,18 @@ __global__ void __launch_bounds__(256, VEC == 2 ? 2 : 3) k_scan_bwd(const T *__r
                 const float lam = g[i][k] + m[k];
                 const float gx = c[i][k] * lam;
                 m[k] = a[i][k] * lam;
-                const bool live = full || i < left;
-                v[i][k] = live ? a[i][k] * gx * v[i][k] : 0.f;
-                g[i][k] = live ? gx : 0.f;
+                v[i][k] = a[i][k] * gx * v[i][k];
+                g[i][k] = gx;
             }
-        if (s.WT == 1)
+        if (!full)
+#pragma unroll
+            for (int i = 0; i < STEPS; ++i)
+#pragma unroll
+                for (int k = 0; k < VEC; ++k) {
+                    v[i][k] = i < left ? v[i][k] : 0.f;
+                    g[i][k] = i < left ? g[i][k] : 0.f;
+                }
+        if (WT == 1)
 #pragma unroll
             for (int k = 0; k < VEC; ++k) mu[k] = m[k];
         const int64_t rest = l.in ? s.T - t0 : 0;
@@ -434,7 +596,7 @@ __global__ void __launch_bounds__(256, VEC == 2 ? 2 : 3) k_scan_bwd(const T *__r
 // pass laid down; VEC only says how many channels a lane takes.
 static int scan_steps(int64_t T) { return T == 1 ? 1 : kScanSteps; }
 
-static ScanDims scan_dims(int64_t B, int64_t T, int64_t D) {
+static ScanDims scan_dims(int64_t B, int64_t T, int64_t D, int ctas_per_sm) {
     ScanDims s{};
     s.B = B, s.T = T, s.D = D, s.channels = B * D;
     const int64_t steps = scan_steps(T);
@@ -443,12 +605,12 @@ static ScanDims scan_dims(int64_t B, int64_t T, int64_t D) {
     while (s.WT < runs && s.WT < kScanMaxWarps) s.WT <<= 1;
     s.WC = 8 / s.WT;
     s.tiles = (runs + s.WT - 1) / s.WT;
-    // Cut the axis when the channels alone do not give every SM a CTA; 4 CTAs of 256 threads an SM is what their registers allow.
+    // Cut the axis when the channels alone do not give every SM a CTA, into as many segments as run at once: one wave.
     const int64_t ctas = (s.channels + 64 * s.WC - 1) / (64 * s.WC);
     const int64_t sms = num_sms();
     int64_t segments = 1;
     if (ctas < sms && s.tiles > 1) {
-        segments = 4 * sms / ctas;
+        segments = ctas_per_sm * sms / ctas;
         if (segments > kScanMaxSegments) segments = kScanMaxSegments;
         if (segments > s.tiles) segments = s.tiles;
     }
@@ -481,17 +643,36 @@ using namespace hgq;
 
 extern "C" size_t hgq_gated_scan_workspace(int64_t B, int64_t T, int64_t D) {
     if (scan_args(B, T, D, HGQ_TYPE_F32) != HGQ_OK || B * D == 0) return 0;
-    const ScanDims s = scan_dims(B, T, D);
-    return s.segments > 1 ? (size_t)s.segments * s.channels * sizeof(float2) : 0;
+    int most = 1;
+    for (int per_sm : {kFwdCtas, kBwdCtas}) {
+        const int n = scan_dims(B, T, D, per_sm).segments;
+        most = n > most ? n : most;
+    }
+    return most > 1 ? (size_t)most * B * D * sizeof(float2) : 0;
 }
 
 extern "C" int64_t hgq_gated_scan_states(int64_t B, int64_t T, int64_t D) {
     if (scan_args(B, T, D, HGQ_TYPE_F32) != HGQ_OK || B * D == 0) return 0;
-    const ScanDims s = scan_dims(B, T, D);
+    const ScanDims s = scan_dims(B, T, D, kFwdCtas);
     return s.tiles > 1 ? s.tiles * s.channels : 0;  // one tile starts from h0 itself
 }
 
 namespace {
+
+// Tiles fetched ahead where a CTA walks more than one and a pack is what an asynchronous copy can move (4 or 8 bytes).
+template <typename T, int VEC>
+constexpr bool kAhead = sizeof(T) * VEC >= 4;
+
+template <typename T, int VEC, int N>
+constexpr size_t kStageBytes = kAhead<T, VEC> ? (size_t)kScanMaxWarps * 2 * N * kScanSteps * 32 * sizeof(T) * VEC : 0;
+
+template <typename K>
+int allow_smem(K kernel, size_t bytes) {
+    if (bytes <= (36u << 10)) return HGQ_OK;  // with at most 12 KB of static shared memory beside it
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+    if (e != cudaSuccess) cudaGetLastError();
+    return (int)e;
+}
 
 template <typename T, int VEC>
 int scan_fwd(const ScanDims &s, const void *x, const void *z, const float *h0, const int32_t *lengths, void *h, float *h_last, float *states,
@@ -499,12 +680,27 @@ int scan_fwd(const ScanDims &s, const void *x, const void *z, const float *h0, c
     const dim3 grid((unsigned)((s.channels + 32 * VEC * s.WC - 1) / (32 * VEC * s.WC)), (unsigned)s.segments);
     const unsigned threads = 32 * s.WT * s.WC;
     const T *px = (const T *)x, *pz = (const T *)z;
-    if (s.segments > 1) {
-        k_scan_fold<T, VEC, kScanSteps><<<grid, threads, 0, st>>>(px, pz, lengths, s, agg);
+    T *ph = (T *)h;
+    constexpr int W = kScanMaxWarps;
+    constexpr bool A = kAhead<T, VEC>;
+    constexpr size_t bytes = kStageBytes<T, VEC, 2>;
+    if (s.segments > 1) {  // more than one tile: WT is kScanMaxWarps
+        auto fold = k_scan_fold<T, VEC, kScanSteps, W, A>;
+        if (int e = allow_smem(fold, bytes)) return e;
+        fold<<<grid, threads, bytes, st>>>(px, pz, lengths, s, agg);
         if (int e = check_launch()) return e;
     }
-    if (s.T == 1) k_scan_fwd<T, VEC, 1><<<grid, threads, 0, st>>>(px, pz, h0, lengths, s, agg, (T *)h, h_last, states);
-    else k_scan_fwd<T, VEC, kScanSteps><<<grid, threads, 0, st>>>(px, pz, h0, lengths, s, agg, (T *)h, h_last, states);
+    if (s.T == 1) {
+        k_scan_fwd<T, VEC, 1, 1, false><<<grid, threads, 0, st>>>(px, pz, h0, lengths, s, agg, ph, h_last, states);
+    } else if (s.tiles_per_segment > 1) {
+        auto fwd = k_scan_fwd<T, VEC, kScanSteps, W, A>;
+        if (int e = allow_smem(fwd, bytes)) return e;
+        fwd<<<grid, threads, bytes, st>>>(px, pz, h0, lengths, s, agg, ph, h_last, states);
+    } else if (s.WT == W) {
+        k_scan_fwd<T, VEC, kScanSteps, W, false><<<grid, threads, 0, st>>>(px, pz, h0, lengths, s, agg, ph, h_last, states);
+    } else {
+        k_scan_fwd<T, VEC, kScanSteps, 0, false><<<grid, threads, 0, st>>>(px, pz, h0, lengths, s, agg, ph, h_last, states);
+    }
     return check_launch();
 }
 
@@ -514,12 +710,28 @@ int scan_bwd(const ScanDims &s, const void *gh, const void *x, const void *z, co
     const dim3 grid((unsigned)((s.channels + 32 * VEC * s.WC - 1) / (32 * VEC * s.WC)), (unsigned)s.segments);
     const unsigned threads = 32 * s.WT * s.WC;
     const T *pg = (const T *)gh, *px = (const T *)x, *pz = (const T *)z;
+    T *pdx = (T *)dx, *pdz = (T *)dz;
+    constexpr int W = kScanMaxWarps;
+    constexpr bool A = kAhead<T, VEC>;
     if (s.segments > 1) {
-        k_scan_bwd_fold<T, VEC, kScanSteps><<<grid, threads, 0, st>>>(pg, pz, lengths, s, agg);
+        constexpr size_t bytes = kStageBytes<T, VEC, 2>;
+        auto fold = k_scan_bwd_fold<T, VEC, kScanSteps, W, A>;
+        if (int e = allow_smem(fold, bytes)) return e;
+        fold<<<grid, threads, bytes, st>>>(pg, pz, lengths, s, agg);
         if (int e = check_launch()) return e;
     }
-    if (s.T == 1) k_scan_bwd<T, VEC, 1><<<grid, threads, 0, st>>>(pg, px, pz, h0, lengths, states, g_last, s, agg, (T *)dx, (T *)dz, dh0);
-    else k_scan_bwd<T, VEC, kScanSteps><<<grid, threads, 0, st>>>(pg, px, pz, h0, lengths, states, g_last, s, agg, (T *)dx, (T *)dz, dh0);
+    if (s.T == 1) {
+        k_scan_bwd<T, VEC, 1, 1, false><<<grid, threads, 0, st>>>(pg, px, pz, h0, lengths, states, g_last, s, agg, pdx, pdz, dh0);
+    } else if (s.tiles_per_segment > 1) {
+        constexpr size_t bytes = kStageBytes<T, VEC, 3>;
+        auto bwd = k_scan_bwd<T, VEC, kScanSteps, W, A>;
+        if (int e = allow_smem(bwd, bytes)) return e;
+        bwd<<<grid, threads, bytes, st>>>(pg, px, pz, h0, lengths, states, g_last, s, agg, pdx, pdz, dh0);
+    } else if (s.WT == W) {
+        k_scan_bwd<T, VEC, kScanSteps, W, false><<<grid, threads, 0, st>>>(pg, px, pz, h0, lengths, states, g_last, s, agg, pdx, pdz, dh0);
+    } else {
+        k_scan_bwd<T, VEC, kScanSteps, 0, false><<<grid, threads, 0, st>>>(pg, px, pz, h0, lengths, states, g_last, s, agg, pdx, pdz, dh0);
+    }
     return check_launch();
 }
 
@@ -545,7 +757,7 @@ extern "C" int hgq_gated_scan_fwd(const void *x, int64_t x_batch, int64_t x_time
     const size_t need = hgq_gated_scan_workspace(B, T, D);
     if (need > 0 && (!workspace || workspace_bytes < need)) return HGQ_ERR_WORKSPACE;
     if (need > 0 && !aligned(workspace, 8)) return HGQ_ERR_ALIGN;
-    ScanDims s = scan_dims(B, T, D);
+    ScanDims s = scan_dims(B, T, D, kFwdCtas);
     s.xsb = x_batch, s.xst = x_time, s.zsb = z_batch, s.zst = z_time;
     if (s.tiles <= 1) states = nullptr;
     cudaStream_t st = (cudaStream_t)stream;
@@ -569,7 +781,7 @@ extern "C" int hgq_gated_scan_bwd(const void *gh, int64_t g_batch, int64_t g_tim
     const size_t need = hgq_gated_scan_workspace(B, T, D);
     if (need > 0 && (!workspace || workspace_bytes < need)) return HGQ_ERR_WORKSPACE;
     if (need > 0 && !aligned(workspace, 8)) return HGQ_ERR_ALIGN;
-    ScanDims s = scan_dims(B, T, D);
+    ScanDims s = scan_dims(B, T, D, kBwdCtas);
     s.xsb = x_batch, s.xst = x_time, s.zsb = z_batch, s.zst = z_time, s.gsb = g_batch, s.gst = g_time;
     s.dxb = dx_batch, s.dxt = dx_time, s.dzb = dz_batch, s.dzt = dz_time;
     if (s.tiles > 1 && !states) return HGQ_ERR_NULL;
