@@ -136,43 +136,63 @@ __device__ __forceinline__ void load_packs(const T *__restrict__ p, int64_t stri
         for (int k = 0; k < VEC; ++k) v[i][k] = scan_float(q[i].v[k]);
 }
 
-// The same through shared memory, fetched a tile ahead: every lane copies and later reads its own packs (no barrier), a copy
-// whose step is not live writes zeros.  Registers would hold the next tile's packs as well, at the price of spills.
-template <typename T, int VEC, int STEPS>
-__device__ __forceinline__ void fetch_packs(ScanPack<T, VEC> *dst, const T *__restrict__ p, int64_t stride, bool full, int64_t left) {
-    constexpr int bytes = sizeof(T) * VEC;
-    static_assert(bytes == 4 || bytes == 8, "copies of 4 or 8 bytes");
-    uint32_t d = (uint32_t)__cvta_generic_to_shared(dst);
-#pragma unroll
-    for (int i = 0; i < STEPS; ++i, d += 32 * bytes, p += stride) {
-        if (full || i < left) asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(d), "l"(p), "n"(bytes) : "memory");
-        else dst[i * 32] = ScanPack<T, VEC>{};
-    }
-}
-
-template <typename T, int VEC, int STEPS>
-__device__ __forceinline__ void staged_packs(const ScanPack<T, VEC> *src, float (&v)[STEPS][VEC]) {
-#pragma unroll
-    for (int i = 0; i < STEPS; ++i) {
-        const ScanPack<T, VEC> q = src[i * 32];
-#pragma unroll
-        for (int k = 0; k < VEC; ++k) v[i][k] = scan_float(q.v[k]);
-    }
-}
-
-// One tile's packs of N sequences, the next tile's on the way while this one's are used.
-template <typename T, int VEC, int STEPS, int N, bool AHEAD>
+// The same through shared memory, fetched a tile ahead: a warp's packs of one sequence are STEPS rows of 32 packs, copied as 16-byte
+// pieces (a quarter to an eighth of the instructions that copies of a lane's own packs take, which cost more issue slots than
+// the recurrence).  A piece lies in one batch row; steps that are not live are filled with zeros.
+template <typename T, int VEC, int STEPS, int N>
 struct Stages {
     using P = ScanPack<T, VEC>;
-    P *base;  // this lane's column of its warp's buffers: [2][N][STEPS][32]
+    static constexpr int kPieces = 32 * (int)sizeof(P) / 16;  // of a row
+    static constexpr int kRows = 32 / kPieces;                // rows that one instruction of the warp copies
+    P *base;        // this warp's buffers: [2][N][STEPS][32]
+    uint32_t dst;   // where this lane's piece of a buffer's first rows goes
+    int row;        // of this lane's piece
+    int64_t b, d, len;
+    bool in;
 
-    __device__ __forceinline__ explicit Stages(unsigned char *smem) {
-        base = reinterpret_cast<P *>(smem) + (threadIdx.x >> 5) * (2 * N * STEPS * 32) + (threadIdx.x & 31);
+    __device__ __forceinline__ Stages(unsigned char *smem, const ScanDims &s, int WT, const int32_t *lengths) {
+        const int w = threadIdx.x >> 5, lane = threadIdx.x & 31, piece = lane % kPieces;
+        base = reinterpret_cast<P *>(smem) + w * (2 * N * STEPS * 32);
+        row = lane / kPieces;
+        dst = (uint32_t)__cvta_generic_to_shared(base) + (uint32_t)(row * kPieces + piece) * 16u;
+        const int64_t c = (((int64_t)blockIdx.x * s.WC + w / WT) * 32) * VEC + piece * (16 / (int)sizeof(T));
+        in = c < s.channels;
+        b = in ? c / s.D : 0;
+        d = in ? c - b * s.D : 0;
+        len = in ? s.T : 0;
+        if (in && lengths != nullptr) {
+            const int64_t n = lengths[b];
+            len = n < 0 ? 0 : (n > s.T ? s.T : n);
+        }
     }
-    __device__ __forceinline__ P *at(int64_t tile, int n) const { return base + ((tile & 1) * N + n) * STEPS * 32; }
+    // p: the tensor, NULL for one of zeros
+    __device__ __forceinline__ void fetch(int64_t tile, int n, const T *__restrict__ p, int64_t batch, int64_t time, int64_t t0) const {
+        const T *src = p + b * batch + d;
+        const int64_t left = p != nullptr ? len - t0 : 0;
+        uint32_t to = dst + (uint32_t)(((tile & 1) * N + n) * STEPS * 32 * (int)sizeof(P));
+#pragma unroll
+        for (int i = 0; i < STEPS; i += kRows, to += 512u) {
+            const bool live = row + i < left;
+            const T *q = live ? src + (t0 + row + i) * time : p;
+            if (p != nullptr) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(q), "r"(live ? 16 : 0) : "memory");
+            else asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(to), "r"(0) : "memory");
+        }
+    }
     static __device__ __forceinline__ void commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-    static __device__ __forceinline__ void wait_but_newest() { asm volatile("cp.async.wait_group 1;" ::: "memory"); }
-    static __device__ __forceinline__ void wait_all() { asm volatile("cp.async.wait_group 0;" ::: "memory"); }
+    static __device__ __forceinline__ void wait(bool next_is_on_the_way) {
+        if (next_is_on_the_way) asm volatile("cp.async.wait_group 1;" ::: "memory");
+        else asm volatile("cp.async.wait_group 0;" ::: "memory");
+        __syncwarp();
+    }
+    __device__ __forceinline__ void values(int64_t tile, int n, float (&v)[STEPS][VEC]) const {
+        const P *src = base + ((tile & 1) * N + n) * STEPS * 32 + (threadIdx.x & 31);
+#pragma unroll
+        for (int i = 0; i < STEPS; ++i) {
+            const P q = src[i * 32];
+#pragma unroll
+            for (int k = 0; k < VEC; ++k) v[i][k] = scan_float(q.v[k]);
+        }
+    }
 };
 
 template <typename T, int VEC, int STEPS>
@@ -221,30 +241,23 @@ __global__ void __launch_bounds__(256) k_scan_fold(const T *__restrict__ x, cons
 #pragma unroll
     for (int k = 0; k < VEC; ++k) A[k] = 1.f, H[k] = 0.f;
     extern __shared__ __align__(16) unsigned char staging[];
-    const Stages<T, VEC, STEPS, 2, AHEAD> stages(staging);
-    [[maybe_unused]] auto fetch = [&](auto tile) {
-        const int64_t t0 = (tile * WT + l.wt) * STEPS, left = l.len - t0;
-        const bool full = __all_sync(0xffffffffu, left >= STEPS);
-        fetch_packs<T, VEC, STEPS>(stages.at(tile, 0), z + l.b * s.zsb + l.d + t0 * s.zst, s.zst, full, left);
-        fetch_packs<T, VEC, STEPS>(stages.at(tile, 1), x + l.b * s.xsb + l.d + t0 * s.xst, s.xst, full, left);
+    const Stages<T, VEC, STEPS, 2> stages(staging, s, WT, lengths);
+    auto fetch = [&](int64_t tile) {
+        const int64_t t0 = (tile * WT + l.wt) * STEPS;
+        stages.fetch(tile, 0, z, s.zsb, s.zst, t0);
+        stages.fetch(tile, 1, x, s.xsb, s.xst, t0);
         stages.commit();
     };
-    if constexpr (AHEAD) {
-        if (first < last) fetch(first);
-    }
+    if (AHEAD && first < last) fetch(first);
     for (int64_t tile = first; tile < last; ++tile) {
         const int64_t t0 = (tile * WT + l.wt) * STEPS, left = l.len - t0;
         const bool full = __all_sync(0xffffffffu, left >= STEPS);
         float a[STEPS][VEC], c[STEPS][VEC], v[STEPS][VEC];
-        if constexpr (AHEAD) {
-            if (tile + 1 < last) {
-                fetch(tile + 1);
-                stages.wait_but_newest();
-            } else {
-                stages.wait_all();
-            }
-            staged_packs<T, VEC, STEPS>(stages.at(tile, 0), a);
-            staged_packs<T, VEC, STEPS>(stages.at(tile, 1), v);
+        if (AHEAD) {
+            if (tile + 1 < last) fetch(tile + 1);
+            stages.wait(tile + 1 < last);
+            stages.values(tile, 0, a);
+            stages.values(tile, 1, v);
         } else {
             load_packs<T, VEC, STEPS>(z + l.b * s.zsb + l.d + t0 * s.zst, s.zst, full, left, a);
             load_packs<T, VEC, STEPS>(x + l.b * s.xsb + l.d + t0 * s.xst, s.xst, full, left, v);
@@ -301,30 +314,23 @@ __global__ void __launch_bounds__(256, VEC == 2 ? kFwdCtas : 4) k_scan_fwd(const
                 carry[k] = q.x * carry[k] + q.y;
             }
     extern __shared__ __align__(16) unsigned char staging[];
-    const Stages<T, VEC, STEPS, 2, AHEAD> stages(staging);
-    [[maybe_unused]] auto fetch = [&](auto tile) {
-        const int64_t t0 = (tile * WT + l.wt) * STEPS, left = l.len - t0;
-        const bool full = __all_sync(0xffffffffu, left >= STEPS);
-        fetch_packs<T, VEC, STEPS>(stages.at(tile, 0), z + l.b * s.zsb + l.d + t0 * s.zst, s.zst, full, left);
-        fetch_packs<T, VEC, STEPS>(stages.at(tile, 1), x + l.b * s.xsb + l.d + t0 * s.xst, s.xst, full, left);
+    const Stages<T, VEC, STEPS, 2> stages(staging, s, WT, lengths);
+    auto fetch = [&](int64_t tile) {
+        const int64_t t0 = (tile * WT + l.wt) * STEPS;
+        stages.fetch(tile, 0, z, s.zsb, s.zst, t0);
+        stages.fetch(tile, 1, x, s.xsb, s.xst, t0);
         stages.commit();
     };
-    if constexpr (AHEAD) {
-        if (first < last) fetch(first);
-    }
+    if (AHEAD && first < last) fetch(first);
     for (int64_t tile = first; tile < last; ++tile) {
         const int64_t t0 = (tile * WT + l.wt) * STEPS, left = l.len - t0;
         const bool full = __all_sync(0xffffffffu, left >= STEPS);
         float a[STEPS][VEC], c[STEPS][VEC], v[STEPS][VEC];
-        if constexpr (AHEAD) {
-            if (tile + 1 < last) {
-                fetch(tile + 1);
-                stages.wait_but_newest();
-            } else {
-                stages.wait_all();
-            }
-            staged_packs<T, VEC, STEPS>(stages.at(tile, 0), a);
-            staged_packs<T, VEC, STEPS>(stages.at(tile, 1), v);
+        if (AHEAD) {
+            if (tile + 1 < last) fetch(tile + 1);
+            stages.wait(tile + 1 < last);
+            stages.values(tile, 0, a);
+            stages.values(tile, 1, v);
         } else {
             load_packs<T, VEC, STEPS>(z + l.b * s.zsb + l.d + t0 * s.zst, s.zst, full, left, a);
             load_packs<T, VEC, STEPS>(x + l.b * s.xsb + l.d + t0 * s.xst, s.xst, full, left, v);
@@ -400,30 +406,23 @@ __global__ void __launch_bounds__(256) k_scan_bwd_fold(const T *__restrict__ gh,
 #pragma unroll
     for (int k = 0; k < VEC; ++k) A[k] = 1.f, L[k] = 0.f;
     extern __shared__ __align__(16) unsigned char staging[];
-    const Stages<T, VEC, STEPS, 2, AHEAD> stages(staging);
-    [[maybe_unused]] auto fetch = [&](auto tile) {
-        const int64_t t0 = (tile * WT + l.wt) * STEPS, left = l.len - t0;
-        const bool full = __all_sync(0xffffffffu, left >= STEPS);
-        fetch_packs<T, VEC, STEPS>(stages.at(tile, 0), z + l.b * s.zsb + l.d + t0 * s.zst, s.zst, full, left);
-        fetch_packs<T, VEC, STEPS>(stages.at(tile, 1), gh + l.b * s.gsb + l.d + t0 * s.gst, s.gst, full && gh != nullptr, gh != nullptr ? left : 0);
+    const Stages<T, VEC, STEPS, 2> stages(staging, s, WT, lengths);
+    auto fetch = [&](int64_t tile) {
+        const int64_t t0 = (tile * WT + l.wt) * STEPS;
+        stages.fetch(tile, 0, z, s.zsb, s.zst, t0);
+        stages.fetch(tile, 1, gh, s.gsb, s.gst, t0);
         stages.commit();
     };
-    if constexpr (AHEAD) {
-        if (first < last) fetch(last - 1);
-    }
+    if (AHEAD && first < last) fetch(last - 1);
     for (int64_t tile = last - 1; tile >= first; --tile) {
         const int64_t t0 = (tile * WT + l.wt) * STEPS, left = l.len - t0;
         const bool full = __all_sync(0xffffffffu, left >= STEPS);
         float a[STEPS][VEC], c[STEPS][VEC], g[STEPS][VEC];
-        if constexpr (AHEAD) {
-            if (tile > first) {
-                fetch(tile - 1);
-                stages.wait_but_newest();
-            } else {
-                stages.wait_all();
-            }
-            staged_packs<T, VEC, STEPS>(stages.at(tile, 0), a);
-            staged_packs<T, VEC, STEPS>(stages.at(tile, 1), g);
+        if (AHEAD) {
+            if (tile > first) fetch(tile - 1);
+            stages.wait(tile > first);
+            stages.values(tile, 0, a);
+            stages.values(tile, 1, g);
         } else {
             load_packs<T, VEC, STEPS>(z + l.b * s.zsb + l.d + t0 * s.zst, s.zst, full, left, a);
             load_packs<T, VEC, STEPS>(gh + l.b * s.gsb + l.d + t0 * s.gst, s.gst, full && gh != nullptr, gh != nullptr ? left : 0, g);
@@ -483,32 +482,25 @@ __global__ void __launch_bounds__(256, VEC == 2 ? kBwdCtas : 3) k_scan_bwd(const
                 mu[k] = q.x * mu[k] + q.y;
             }
     extern __shared__ __align__(16) unsigned char staging[];
-    const Stages<T, VEC, STEPS, 3, AHEAD> stages(staging);
-    [[maybe_unused]] auto fetch = [&](auto tile) {
-        const int64_t t0 = (tile * WT + l.wt) * STEPS, left = l.len - t0;
-        const bool full = __all_sync(0xffffffffu, left >= STEPS);
-        fetch_packs<T, VEC, STEPS>(stages.at(tile, 0), z + l.b * s.zsb + l.d + t0 * s.zst, s.zst, full, left);
-        fetch_packs<T, VEC, STEPS>(stages.at(tile, 1), x + l.b * s.xsb + l.d + t0 * s.xst, s.xst, full, left);
-        fetch_packs<T, VEC, STEPS>(stages.at(tile, 2), gh + l.b * s.gsb + l.d + t0 * s.gst, s.gst, full && gh != nullptr, gh != nullptr ? left : 0);
+    const Stages<T, VEC, STEPS, 3> stages(staging, s, WT, lengths);
+    auto fetch = [&](int64_t tile) {
+        const int64_t t0 = (tile * WT + l.wt) * STEPS;
+        stages.fetch(tile, 0, z, s.zsb, s.zst, t0);
+        stages.fetch(tile, 1, x, s.xsb, s.xst, t0);
+        stages.fetch(tile, 2, gh, s.gsb, s.gst, t0);
         stages.commit();
     };
-    if constexpr (AHEAD) {
-        if (first < last) fetch(last - 1);
-    }
+    if (AHEAD && first < last) fetch(last - 1);
     for (int64_t tile = last - 1; tile >= first; --tile) {
         const int64_t t0 = (tile * WT + l.wt) * STEPS, left = l.len - t0;
         const bool full = __all_sync(0xffffffffu, left >= STEPS);
         float a[STEPS][VEC], c[STEPS][VEC], v[STEPS][VEC], g[STEPS][VEC], h[VEC];
-        if constexpr (AHEAD) {
-            if (tile > first) {
-                fetch(tile - 1);
-                stages.wait_but_newest();
-            } else {
-                stages.wait_all();
-            }
-            staged_packs<T, VEC, STEPS>(stages.at(tile, 0), a);
-            staged_packs<T, VEC, STEPS>(stages.at(tile, 1), v);
-            staged_packs<T, VEC, STEPS>(stages.at(tile, 2), g);
+        if (AHEAD) {
+            if (tile > first) fetch(tile - 1);
+            stages.wait(tile > first);
+            stages.values(tile, 0, a);
+            stages.values(tile, 1, v);
+            stages.values(tile, 2, g);
         } else {
             load_packs<T, VEC, STEPS>(z + l.b * s.zsb + l.d + t0 * s.zst, s.zst, full, left, a);
             load_packs<T, VEC, STEPS>(x + l.b * s.xsb + l.d + t0 * s.xst, s.xst, full, left, v);
@@ -619,13 +611,13 @@ static ScanDims scan_dims(int64_t B, int64_t T, int64_t D, int ctas_per_sm) {
     return s;
 }
 
-// Two neighbouring channels as one access: an even number of features, strides and addresses that keep every pair aligned.
-static bool scan_pairs(int64_t D, size_t size, std::initializer_list<const void *> ptrs, std::initializer_list<int64_t> strides) {
-    if (D % 2 != 0) return false;
+// `n` neighbouring channels as one access: a number of features, strides and addresses that keep every pack aligned.
+static bool scan_packs(int64_t D, size_t size, int n, std::initializer_list<const void *> ptrs, std::initializer_list<int64_t> strides) {
+    if (D % n != 0) return false;
     for (const void *p : ptrs)
-        if (!aligned(p, 2 * size)) return false;
+        if (!aligned(p, n * size)) return false;
     for (int64_t st : strides)
-        if (st % 2 != 0) return false;
+        if (st % n != 0) return false;
     return true;
 }
 
@@ -659,12 +651,8 @@ extern "C" int64_t hgq_gated_scan_states(int64_t B, int64_t T, int64_t D) {
 
 namespace {
 
-// Tiles fetched ahead where a CTA walks more than one and a pack is what an asynchronous copy can move (4 or 8 bytes).
-template <typename T, int VEC>
-constexpr bool kAhead = sizeof(T) * VEC >= 4;
-
 template <typename T, int VEC, int N>
-constexpr size_t kStageBytes = kAhead<T, VEC> ? (size_t)kScanMaxWarps * 2 * N * kScanSteps * 32 * sizeof(T) * VEC : 0;
+constexpr size_t kStageBytes = (size_t)kScanMaxWarps * 2 * N * kScanSteps * 32 * sizeof(T) * VEC;
 
 template <typename K>
 int allow_smem(K kernel, size_t bytes) {
@@ -674,7 +662,10 @@ int allow_smem(K kernel, size_t bytes) {
     return (int)e;
 }
 
-template <typename T, int VEC>
+// What a lane takes of the channels: one, a pair, or a pair out of pieces fetched ahead (the pieces for CTAs that walk several tiles).
+enum ScanAccess { kOne, kPair, kPieces };
+
+template <typename T, int VEC, bool AHEAD>
 int scan_fwd(const ScanDims &s, const void *x, const void *z, const float *h0, const int32_t *lengths, void *h, float *h_last, float *states,
              float2 *agg, cudaStream_t st) {
     const dim3 grid((unsigned)((s.channels + 32 * VEC * s.WC - 1) / (32 * VEC * s.WC)), (unsigned)s.segments);
@@ -682,29 +673,26 @@ int scan_fwd(const ScanDims &s, const void *x, const void *z, const float *h0, c
     const T *px = (const T *)x, *pz = (const T *)z;
     T *ph = (T *)h;
     constexpr int W = kScanMaxWarps;
-    constexpr bool A = kAhead<T, VEC>;
-    constexpr size_t bytes = kStageBytes<T, VEC, 2>;
+    constexpr size_t bytes = AHEAD ? kStageBytes<T, VEC, 2> : 0;
     if (s.segments > 1) {  // more than one tile: WT is kScanMaxWarps
-        auto fold = k_scan_fold<T, VEC, kScanSteps, W, A>;
+        auto fold = k_scan_fold<T, VEC, kScanSteps, W, AHEAD>;
         if (int e = allow_smem(fold, bytes)) return e;
         fold<<<grid, threads, bytes, st>>>(px, pz, lengths, s, agg);
         if (int e = check_launch()) return e;
     }
-    if (s.T == 1) {
-        k_scan_fwd<T, VEC, 1, 1, false><<<grid, threads, 0, st>>>(px, pz, h0, lengths, s, agg, ph, h_last, states);
-    } else if (s.tiles_per_segment > 1) {
-        auto fwd = k_scan_fwd<T, VEC, kScanSteps, W, A>;
+    if (s.WT == W) {
+        auto fwd = k_scan_fwd<T, VEC, kScanSteps, W, AHEAD>;
         if (int e = allow_smem(fwd, bytes)) return e;
         fwd<<<grid, threads, bytes, st>>>(px, pz, h0, lengths, s, agg, ph, h_last, states);
-    } else if (s.WT == W) {
-        k_scan_fwd<T, VEC, kScanSteps, W, false><<<grid, threads, 0, st>>>(px, pz, h0, lengths, s, agg, ph, h_last, states);
+    } else if (s.T == 1) {
+        k_scan_fwd<T, VEC, 1, 1, false><<<grid, threads, 0, st>>>(px, pz, h0, lengths, s, agg, ph, h_last, states);
     } else {
         k_scan_fwd<T, VEC, kScanSteps, 0, false><<<grid, threads, 0, st>>>(px, pz, h0, lengths, s, agg, ph, h_last, states);
     }
     return check_launch();
 }
 
-template <typename T, int VEC>
+template <typename T, int VEC, bool AHEAD>
 int scan_bwd(const ScanDims &s, const void *gh, const void *x, const void *z, const float *h0, const int32_t *lengths, const float *states,
              const float *g_last, void *dx, void *dz, float *dh0, float2 *agg, cudaStream_t st) {
     const dim3 grid((unsigned)((s.channels + 32 * VEC * s.WC - 1) / (32 * VEC * s.WC)), (unsigned)s.segments);
@@ -712,37 +700,43 @@ int scan_bwd(const ScanDims &s, const void *gh, const void *x, const void *z, co
     const T *pg = (const T *)gh, *px = (const T *)x, *pz = (const T *)z;
     T *pdx = (T *)dx, *pdz = (T *)dz;
     constexpr int W = kScanMaxWarps;
-    constexpr bool A = kAhead<T, VEC>;
     if (s.segments > 1) {
-        constexpr size_t bytes = kStageBytes<T, VEC, 2>;
-        auto fold = k_scan_bwd_fold<T, VEC, kScanSteps, W, A>;
+        constexpr size_t bytes = AHEAD ? kStageBytes<T, VEC, 2> : 0;
+        auto fold = k_scan_bwd_fold<T, VEC, kScanSteps, W, AHEAD>;
         if (int e = allow_smem(fold, bytes)) return e;
         fold<<<grid, threads, bytes, st>>>(pg, pz, lengths, s, agg);
         if (int e = check_launch()) return e;
     }
-    if (s.T == 1) {
-        k_scan_bwd<T, VEC, 1, 1, false><<<grid, threads, 0, st>>>(pg, px, pz, h0, lengths, states, g_last, s, agg, pdx, pdz, dh0);
-    } else if (s.tiles_per_segment > 1) {
-        constexpr size_t bytes = kStageBytes<T, VEC, 3>;
-        auto bwd = k_scan_bwd<T, VEC, kScanSteps, W, A>;
+    if (s.WT == W) {
+        constexpr size_t bytes = AHEAD ? kStageBytes<T, VEC, 3> : 0;
+        auto bwd = k_scan_bwd<T, VEC, kScanSteps, W, AHEAD>;
         if (int e = allow_smem(bwd, bytes)) return e;
         bwd<<<grid, threads, bytes, st>>>(pg, px, pz, h0, lengths, states, g_last, s, agg, pdx, pdz, dh0);
-    } else if (s.WT == W) {
-        k_scan_bwd<T, VEC, kScanSteps, W, false><<<grid, threads, 0, st>>>(pg, px, pz, h0, lengths, states, g_last, s, agg, pdx, pdz, dh0);
+    } else if (s.T == 1) {
+        k_scan_bwd<T, VEC, 1, 1, false><<<grid, threads, 0, st>>>(pg, px, pz, h0, lengths, states, g_last, s, agg, pdx, pdz, dh0);
     } else {
         k_scan_bwd<T, VEC, kScanSteps, 0, false><<<grid, threads, 0, st>>>(pg, px, pz, h0, lengths, states, g_last, s, agg, pdx, pdz, dh0);
     }
     return check_launch();
 }
 
-}  // namespace
+template <typename T>
+int scan_fwd_by(ScanAccess how, const ScanDims &s, const void *x, const void *z, const float *h0, const int32_t *lengths, void *h,
+                float *h_last, float *states, float2 *agg, cudaStream_t st) {
+    if (how == kPieces) return scan_fwd<T, 2, true>(s, x, z, h0, lengths, h, h_last, states, agg, st);
+    if (how == kPair) return scan_fwd<T, 2, false>(s, x, z, h0, lengths, h, h_last, states, agg, st);
+    return scan_fwd<T, 1, false>(s, x, z, h0, lengths, h, h_last, states, agg, st);
+}
 
-#define SCAN_DISPATCH(FN, ...)                                                       \
-    do {                                                                             \
-        if (type == HGQ_TYPE_F32) return pairs ? FN<float, 2>(__VA_ARGS__) : FN<float, 1>(__VA_ARGS__); \
-        if (type == HGQ_TYPE_BF16) return pairs ? FN<__nv_bfloat16, 2>(__VA_ARGS__) : FN<__nv_bfloat16, 1>(__VA_ARGS__); \
-        return pairs ? FN<__half, 2>(__VA_ARGS__) : FN<__half, 1>(__VA_ARGS__);      \
-    } while (0)
+template <typename T>
+int scan_bwd_by(ScanAccess how, const ScanDims &s, const void *gh, const void *x, const void *z, const float *h0, const int32_t *lengths,
+                const float *states, const float *g_last, void *dx, void *dz, float *dh0, float2 *agg, cudaStream_t st) {
+    if (how == kPieces) return scan_bwd<T, 2, true>(s, gh, x, z, h0, lengths, states, g_last, dx, dz, dh0, agg, st);
+    if (how == kPair) return scan_bwd<T, 2, false>(s, gh, x, z, h0, lengths, states, g_last, dx, dz, dh0, agg, st);
+    return scan_bwd<T, 1, false>(s, gh, x, z, h0, lengths, states, g_last, dx, dz, dh0, agg, st);
+}
+
+}  // namespace
 
 extern "C" int hgq_gated_scan_fwd(const void *x, int64_t x_batch, int64_t x_time, const void *z, int64_t z_batch, int64_t z_time,
                                   const float *h0, const int32_t *lengths, void *h, float *h_last, float *states, int64_t B, int64_t T,
@@ -762,8 +756,12 @@ extern "C" int hgq_gated_scan_fwd(const void *x, int64_t x_batch, int64_t x_time
     if (s.tiles <= 1) states = nullptr;
     cudaStream_t st = (cudaStream_t)stream;
     float2 *agg = (float2 *)workspace;
-    const bool pairs = scan_pairs(D, size, {x, z, h}, {x_batch, x_time, z_batch, z_time});
-    SCAN_DISPATCH(scan_fwd, s, x, z, h0, lengths, h, h_last, states, agg, st);
+    ScanAccess how = kOne;
+    if (scan_packs(D, size, 2, {x, z, h}, {x_batch, x_time, z_batch, z_time})) how = kPair;
+    if (s.tiles_per_segment > 1 && scan_packs(D, size, (int)(16 / size), {x, z, h}, {x_batch, x_time, z_batch, z_time})) how = kPieces;
+    if (type == HGQ_TYPE_F32) return scan_fwd_by<float>(how, s, x, z, h0, lengths, h, h_last, states, agg, st);
+    if (type == HGQ_TYPE_BF16) return scan_fwd_by<__nv_bfloat16>(how, s, x, z, h0, lengths, h, h_last, states, agg, st);
+    return scan_fwd_by<__half>(how, s, x, z, h0, lengths, h, h_last, states, agg, st);
 }
 
 extern "C" int hgq_gated_scan_bwd(const void *gh, int64_t g_batch, int64_t g_time, const void *x, int64_t x_batch, int64_t x_time,
@@ -788,6 +786,12 @@ extern "C" int hgq_gated_scan_bwd(const void *gh, int64_t g_batch, int64_t g_tim
     if (s.tiles <= 1) states = nullptr;
     cudaStream_t st = (cudaStream_t)stream;
     float2 *agg = (float2 *)workspace;
-    const bool pairs = scan_pairs(D, size, {gh, x, z, dx, dz}, {g_batch, g_time, x_batch, x_time, z_batch, z_time, dx_batch, dx_time, dz_batch, dz_time});
-    SCAN_DISPATCH(scan_bwd, s, gh, x, z, h0, lengths, states, g_last, dx, dz, dh0, agg, st);
+    const std::initializer_list<const void *> ptrs = {gh, x, z, dx, dz};
+    const std::initializer_list<int64_t> strides = {g_batch, g_time, x_batch, x_time, z_batch, z_time, dx_batch, dx_time, dz_batch, dz_time};
+    ScanAccess how = kOne;
+    if (scan_packs(D, size, 2, ptrs, strides)) how = kPair;
+    if (s.tiles_per_segment > 1 && scan_packs(D, size, (int)(16 / size), ptrs, strides)) how = kPieces;
+    if (type == HGQ_TYPE_F32) return scan_bwd_by<float>(how, s, gh, x, z, h0, lengths, states, g_last, dx, dz, dh0, agg, st);
+    if (type == HGQ_TYPE_BF16) return scan_bwd_by<__nv_bfloat16>(how, s, gh, x, z, h0, lengths, states, g_last, dx, dz, dh0, agg, st);
+    return scan_bwd_by<__half>(how, s, gh, x, z, h0, lengths, states, g_last, dx, dz, dh0, agg, st);
 }
