@@ -9,66 +9,13 @@
 // their variance.  All statistics are fp32 per thread, group totals fp32 or fp64; x, gy, y, dx are fp32, bf16 or fp16 and are
 // rounded once, on the way out.  The backward pass recomputes u from x (nothing of y is needed), so a pass moves x and gy in and
 // dx out.
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
-#include <cuda_runtime.h>
-
-#include "hgq_common.cuh"
+#include "groupnorm.cuh"
 
 namespace hgq {
 
 
 
 
-
-__device__ __forceinline__ float to_float(float v) { return v; }
-__device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
-__device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
-__device__ __forceinline__ void from_float(float v, float &o) { o = v; }
-__device__ __forceinline__ void from_float(float v, __nv_bfloat16 &o) { o = __float2bfloat16_rn(v); }
-__device__ __forceinline__ void from_float(float v, __half &o) { o = __float2half_rn(v); }
-
-template <typename T, int VEC>
-struct alignas(sizeof(T) * VEC) Pack {
-    T v[VEC];
-};
-
-template <typename T, int VEC>
-__device__ __forceinline__ void load_pack(const T *p, float (&f)[VEC]) {
-    const Pack<T, VEC> q = *reinterpret_cast<const Pack<T, VEC> *>(p);
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) f[i] = to_float(q.v[i]);
-}
-template <typename T, int VEC>
-__device__ __forceinline__ void store_pack(T *p, const float (&f)[VEC]) {
-    Pack<T, VEC> q;
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) from_float(f[i], q.v[i]);
-    *reinterpret_cast<Pack<T, VEC> *>(p) = q;
-}
-
-// act(u)
-__device__ __forceinline__ float act_value(float u, int act) {
-    switch (act) {
-        case HGQ_ACT_RELU: return u < 0.f ? 0.f : u;  // a NaN stays
-        case HGQ_ACT_SILU: return u / (1.f + expf(-u));
-        case HGQ_ACT_GELU: return 0.5f * u * (1.f + erff(u * 0.70710678118654752f));
-        default: return u;
-    }
-}
-// act'(u); the ReLU's slope at 0 is 0
-__device__ __forceinline__ float act_slope(float u, int act) {
-    switch (act) {
-        case HGQ_ACT_RELU: return u > 0.f ? 1.f : (u <= 0.f ? 0.f : u);
-        case HGQ_ACT_SILU: {
-            const float p = 1.f / (1.f + expf(-u));
-            return p * (1.f + u * (1.f - p));
-        }
-        case HGQ_ACT_GELU:
-            return 0.5f * (1.f + erff(u * 0.70710678118654752f)) + u * expf(-0.5f * u * u) * 0.39894228040143268f;
-        default: return 1.f;
-    }
-}
 
 // ---- any shape: partial statistics, totals, application ---------------------------------------------------------------------
 // A CTA takes a run of rows of one sample and a tile of channels; a thread owns VEC neighbouring channels for all of its rows.
@@ -203,14 +150,14 @@ __global__ void __launch_bounds__(kThreads) k_gn_apply(const T *__restrict__ x, 
         of[i] = beta ? beta[c0 + i] : 0.f;
     }
     const int64_t base = ((b_base + b) * g.S) * g.C + c0;
-#pragma unroll 4
-    for (int64_t r = r0 + ty; r < r1; r += g.TY) {
-        float v[VEC];
-        load_pack<T, VEC>(x + base + r * g.C, v);
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) v[i] = act_value((v[i] - mu[i]) * sc[i] + of[i], act);
-        store_pack<T, VEC>(y + base + r * g.C, v);
-    }
+    GN_FOR_ACT(act, {
+        _Pragma("unroll 4") for (int64_t r = r0 + ty; r < r1; r += g.TY) {
+            float v[VEC];
+            load_pack<T, VEC>(x + base + r * g.C, v);
+            _Pragma("unroll") for (int i = 0; i < VEC; ++i) v[i] = act_value<T, ACT>((v[i] - mu[i]) * sc[i] + of[i]);
+            store_pack<T, VEC>(y + base + r * g.C, v);
+        }
+    })
 }
 
 // Per (sample, chunk, channel): sum of du and of du xhat.
@@ -237,19 +184,19 @@ __global__ void __launch_bounds__(kThreads) k_gn_bwd_stats(const T *__restrict__
             be[i] = beta ? beta[c0 + i] : 0.f;
         }
         const int64_t base = ((b_base + b) * g.S) * g.C + c0;
-#pragma unroll 2
-        for (int64_t r = r0 + ty; r < r1; r += g.TY) {
-            float v[VEC], d[VEC];
-            load_pack<T, VEC>(x + base + r * g.C, v);
-            load_pack<T, VEC>(gy + base + r * g.C, d);
-#pragma unroll
-            for (int i = 0; i < VEC; ++i) {
-                const float xh = (v[i] - mu[i]) * rs[i];
-                const float du = d[i] * act_slope(xh * ga[i] + be[i], act);
-                acc[i] += du;
-                acc[VEC + i] += du * xh;
+        GN_FOR_ACT(act, {
+            _Pragma("unroll 2") for (int64_t r = r0 + ty; r < r1; r += g.TY) {
+                float v[VEC], d[VEC];
+                load_pack<T, VEC>(x + base + r * g.C, v);
+                load_pack<T, VEC>(gy + base + r * g.C, d);
+                _Pragma("unroll") for (int i = 0; i < VEC; ++i) {
+                    const float xh = (v[i] - mu[i]) * rs[i];
+                    const float du = d[i] * act_slope<T, ACT>(xh * ga[i] + be[i]);
+                    acc[i] += du;
+                    acc[VEC + i] += du * xh;
+                }
             }
-        }
+        })
     }
     sum_over_ty<2 * VEC>(acc, sh, g, tx, ty);
     if (active && ty == 0) {
@@ -307,19 +254,19 @@ __global__ void __launch_bounds__(kThreads) k_gn_bwd_apply(const T *__restrict__
         a2[i] = m2[rel];
     }
     const int64_t base = ((b_base + b) * g.S) * g.C + c0;
-#pragma unroll 2
-    for (int64_t r = r0 + ty; r < r1; r += g.TY) {
-        float v[VEC], d[VEC];
-        load_pack<T, VEC>(x + base + r * g.C, v);
-        load_pack<T, VEC>(gy + base + r * g.C, d);
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-            const float xh = (v[i] - mu[i]) * rs[i];
-            const float du = d[i] * act_slope(xh * ga[i] + be[i], act);
-            v[i] = rs[i] * (du * ga[i] - a1[i] - xh * a2[i]);
+    GN_FOR_ACT(act, {
+        _Pragma("unroll 2") for (int64_t r = r0 + ty; r < r1; r += g.TY) {
+            float v[VEC], d[VEC];
+            load_pack<T, VEC>(x + base + r * g.C, v);
+            load_pack<T, VEC>(gy + base + r * g.C, d);
+            _Pragma("unroll") for (int i = 0; i < VEC; ++i) {
+                const float xh = (v[i] - mu[i]) * rs[i];
+                const float du = d[i] * act_slope<T, ACT>(xh * ga[i] + be[i]);
+                v[i] = rs[i] * (du * ga[i] - a1[i] - xh * a2[i]);
+            }
+            store_pack<T, VEC>(dx + base + r * g.C, v);
         }
-        store_pack<T, VEC>(dx + base + r * g.C, v);
-    }
+    })
 }
 
 // Column sums of [rows, C2] in a fixed order: 32 columns x 8 row lanes a CTA, grid.y row blocks (a second launch with one block
@@ -382,17 +329,21 @@ static int gn_vec(const void *a, const void *b, const void *c, int C, int type) 
     return 1;
 }
 
+// Partial sums of a call, for whichever access width its addresses allow.
 static size_t gn_part_floats(int64_t B, int64_t S, int C, int G, int type, bool bwd) {
     const int size = type == HGQ_TYPE_F32 ? 4 : 2;
     const int64_t group = gn_group(B, S, C, bwd ? 2 * size : size);
-    int64_t most = 0;
+    size_t most = 0;
     for (int v : {16 / size, 2, 1}) {
         if (C % v != 0) continue;
         const GnGeom g = gn_geom(group, S, C, G, v);
-        const int64_t n = (int64_t)g.chunks * 2 * C;
-        if (n > most) most = n;
+        const size_t any = (size_t)g.chunks * 2 * C * (size_t)(bwd ? B : group);
+        most = any > most ? any : most;
+        const SlabPlan p = gn_slab_plan(B, S, C, G, type, v, bwd);
+        const size_t slab = p.usable && bwd ? (size_t)p.workers * p.K * 2 * C : 0;
+        most = slab > most ? slab : most;
     }
-    return (size_t)most * (size_t)(bwd ? B : group);
+    return most;
 }
 
 static bool gn_args_ok(int64_t B, int64_t S, int C, int G, int act, int type, int *err) {
@@ -504,6 +455,8 @@ extern "C" int hgq_group_norm_fwd(const void *x, const float *gamma, const float
     if (!workspace || workspace_bytes < hgq_group_norm_workspace(B, S, C, G, type, 0)) return HGQ_ERR_WORKSPACE;
     if (!aligned(workspace, 4)) return HGQ_ERR_ALIGN;
     const int vec = gn_vec(x, y, nullptr, C, type);
+    const SlabPlan plan = gn_slab_plan(B, S, C, G, type, vec, false);
+    if (plan.usable) return gn_slab_fwd(plan, x, gamma, beta, y, mean, rstd, B, S, C, G, eps, activation, type, (cudaStream_t)stream);
     GN_DISPATCH(gn_fwd_any, x, gamma, beta, y, mean, rstd, B, S, C, G, eps, activation, (float *)workspace, (cudaStream_t)stream);
 }
 
@@ -533,6 +486,13 @@ extern "C" int hgq_group_norm_bwd(const void *gy, const void *x, const float *ga
     if (!aligned(workspace, 4)) return HGQ_ERR_ALIGN;
     const int vec = gn_vec(gy, x, dx, C, type);
     float *part = (float *)workspace;
+    const SlabPlan plan = gn_slab_plan(B, S, C, G, type, vec, true);
+    if (plan.usable) {
+        if (int e = gn_slab_bwd(plan, gy, x, gamma, beta, mean, rstd, dx, dgamma != nullptr ? part : nullptr, B, S, C, G, activation, type, st))
+            return e;
+        const int64_t rows = plan.workers * plan.K;
+        return dgamma != nullptr ? gn_colsum(part, rows, C, part + rows * 2 * C, dgamma, dbeta, st) : HGQ_OK;
+    }
     float *m = part + gn_part_floats(B, S, C, G, type, true);
     float *scratch = m + 2 * gn_group(B, S, C, 2 * (int)size) * G;
     GN_DISPATCH(gn_bwd_any, gy, x, gamma, beta, mean, rstd, dx, dgamma, dbeta, B, S, C, G, activation, part, m, scratch, st);

@@ -30,6 +30,7 @@
 
 #include <initializer_list>
 
+#include "fast_sigmoid.cuh"
 #include "hgq_common.cuh"
 
 namespace hgq {
@@ -59,33 +60,6 @@ struct ScanDims {
     int64_t tiles, tiles_per_segment;
     int segments;
 };
-
-// a = sigmoid(z) = 1 / (1 + e) with e = exp(-z), and c = 1 - a = e / (1 + e), each to full relative precision (c is not the
-// difference where a is near 1).  fp32: z is held in [-88, 100], where the gates are 0 and 1; the exponential is 2^(-z log2 e) with
-// the rounding error of the product carried along, the reciprocal's error is one ulp.  bf16 and fp16: z has at most 11 bits and
-// the outputs no more, the product's rounding (|z| 2^-24 of e) is far below both; a closed gate is 2^-126.  A NaN stays.
-template <typename T>
-__device__ __forceinline__ void gates(float z, float &a, float &c) {
-    float e, r;
-    if (sizeof(T) == 4) {
-        asm("max.NaN.f32 %0, %0, 0fC2B00000;" : "+f"(z));
-        asm("min.NaN.f32 %0, %0, 0f42C80000;" : "+f"(z));
-        const float t = z * -1.44269504088896341f;
-        const float lo = fmaf(z, -1.44269504088896341f, -t);
-        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(t));
-        e = fmaf(e, lo * 0.693147180559945309f, e);
-        asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + e));
-        a = r;
-        c = z < 0.f ? 1.f - r : e * r;
-    } else {
-        float t = z * -1.44269504088896341f;
-        asm("min.NaN.f32 %0, %0, 0f42FC0000;" : "+f"(t));  // 126
-        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(t));
-        asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + e));
-        a = r;
-        c = e * r;
-    }
-}
 
 struct Lane {
     int64_t c, b, d;
@@ -212,7 +186,7 @@ __device__ __forceinline__ void make_gates(bool full, int64_t left, float (&a)[S
 #pragma unroll
     for (int i = 0; i < STEPS; ++i)
 #pragma unroll
-        for (int k = 0; k < VEC; ++k) gates<T>(a[i][k], a[i][k], c[i][k]);
+        for (int k = 0; k < VEC; ++k) sigmoid_pair<sizeof(T) == 4>(a[i][k], a[i][k], c[i][k]);
     if (!full) {
 #pragma unroll
         for (int i = 0; i < STEPS; ++i)
