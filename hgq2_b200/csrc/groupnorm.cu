@@ -95,39 +95,50 @@ __global__ void __launch_bounds__(kThreads) k_gn_stats(const T *__restrict__ x, 
     }
 }
 
-__device__ __forceinline__ double warp_sum(double s) {
+// Sum over the PER threads of a total (a warp, or the whole block), the same in all of them.
+template <int PER>
+__device__ __forceinline__ double total_sum(double s, double *sh) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    if (PER > 32) {
+        __syncthreads();
+        if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = s;
+        __syncthreads();
+        s = 0.0;
+        for (int w = 0; w < PER / 32; ++w) s += sh[w];
+    }
     return s;
 }
 
-// A warp per (sample, group): the parts' means and squares joined in fp64.
+// PER threads for each (sample, group): the parts' means and squares joined in fp64.
+template <int PER>
 __global__ void __launch_bounds__(kThreads) k_gn_totals(const float *__restrict__ part, const GnGeom g, int64_t b_base, int64_t pairs, float eps,
                                                         float *__restrict__ mean_out, float *__restrict__ rstd_out) {
-    const int64_t pair = (int64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5);
-    const int lane = threadIdx.x & 31;
+    __shared__ double sh[kThreads / 32];
+    const int64_t pair = (int64_t)blockIdx.x * (kThreads / PER) + threadIdx.x / PER;
+    const int lane = threadIdx.x % PER;
     if (pair >= pairs) return;
     const int64_t b = pair / g.G;
     const int gr = (int)(pair % g.G);
     const float *base = part + b * g.chunks * 2 * g.C + gr * g.Cg;
-    const int64_t items = (int64_t)g.chunks * g.Cg;
+    const int items = g.chunks * g.Cg;
     const double total = (double)g.S * g.Cg;
     double s = 0.0;
-    for (int64_t i = lane; i < items; i += 32) {
-        const int64_t ch = i / g.Cg;
+    for (int i = lane; i < items; i += PER) {
+        const int ch = i / g.Cg;
         const int64_t rows = min(g.S - ch * g.rows_per_chunk, g.rows_per_chunk);
-        s += (double)rows * base[ch * 2 * g.C + i % g.Cg];
+        s += (double)rows * base[(int64_t)ch * 2 * g.C + i % g.Cg];
     }
-    const double mean = warp_sum(s) / total;
+    const double mean = total_sum<PER>(s, sh) / total;
     double q = 0.0;
-    for (int64_t i = lane; i < items; i += 32) {
-        const int64_t ch = i / g.Cg;
+    for (int i = lane; i < items; i += PER) {
+        const int ch = i / g.Cg;
         const int64_t rows = min(g.S - ch * g.rows_per_chunk, g.rows_per_chunk);
-        const float *p = base + ch * 2 * g.C + i % g.Cg;
+        const float *p = base + (int64_t)ch * 2 * g.C + i % g.Cg;
         const double d = p[0] - mean;
         q += p[g.C] + (double)rows * d * d;
     }
-    q = warp_sum(q) / total;
+    q = total_sum<PER>(q, sh) / total;
     if (lane == 0) {
         mean_out[b_base * g.G + pair] = (float)mean;
         rstd_out[b_base * g.G + pair] = (float)(1.0 / sqrt(q + (double)eps));
@@ -206,26 +217,28 @@ __global__ void __launch_bounds__(kThreads) k_gn_bwd_stats(const T *__restrict__
     }
 }
 
-// A warp per (sample, group): the two means of the backward formula, in fp64.
+// PER threads for each (sample, group): the two means of the backward formula, in fp64.
+template <int PER>
 __global__ void __launch_bounds__(kThreads) k_gn_bwd_totals(const float *__restrict__ part, const float *__restrict__ gamma, const GnGeom g,
                                                             int64_t pairs, float *__restrict__ m1, float *__restrict__ m2) {
-    const int64_t pair = (int64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5);
-    const int lane = threadIdx.x & 31;
+    __shared__ double sh[kThreads / 32];
+    const int64_t pair = (int64_t)blockIdx.x * (kThreads / PER) + threadIdx.x / PER;
+    const int lane = threadIdx.x % PER;
     if (pair >= pairs) return;
     const int64_t b = pair / g.G;
     const int gr = (int)(pair % g.G);
     const float *base = part + b * g.chunks * 2 * g.C + gr * g.Cg;
-    const int64_t items = (int64_t)g.chunks * g.Cg;
+    const int items = g.chunks * g.Cg;
     double s1 = 0.0, s2 = 0.0;
-    for (int64_t i = lane; i < items; i += 32) {
-        const int c = (int)(i % g.Cg);
+    for (int i = lane; i < items; i += PER) {
+        const int ch = i / g.Cg, c = i % g.Cg;
         const double ga = gamma ? gamma[gr * g.Cg + c] : 1.f;
-        const float *p = base + (i / g.Cg) * 2 * g.C + c;
+        const float *p = base + (int64_t)ch * 2 * g.C + c;
         s1 += ga * p[0];
         s2 += ga * p[g.C];
     }
-    s1 = warp_sum(s1);
-    s2 = warp_sum(s2);
+    s1 = total_sum<PER>(s1, sh);
+    s2 = total_sum<PER>(s2, sh);
     if (lane == 0) {
         const double total = (double)g.S * g.Cg;
         m1[pair] = (float)(s1 / total);
@@ -291,7 +304,7 @@ __global__ void __launch_bounds__(kThreads) k_gn_colsum(const float *__restrict_
 }
 
 // Samples whose x (and gy) an L2 of 126 MB still holds when the second pass comes back to them.
-constexpr int64_t kGnGroupBytes = 48ll << 20;
+constexpr int64_t kGnGroupBytes = 80ll << 20;
 constexpr int kGnSumBlocks = 64;
 
 static int64_t gn_group(int64_t B, int64_t S, int C, int64_t bytes_per_value) {
@@ -310,7 +323,7 @@ static GnGeom gn_geom(int64_t group, int64_t S, int C, int G, int vec) {
     g.tiles = (cv + kThreads - 1) / kThreads;
     g.TX = (cv + g.tiles - 1) / g.tiles;
     g.TY = kThreads / g.TX;
-    const int64_t target = (int64_t)num_sms() * 8;
+    const int64_t target = (int64_t)num_sms() * 4;
     int64_t chunks = (target + group * g.tiles - 1) / (group * g.tiles);
     const int64_t most = (S + (int64_t)g.TY * 4 - 1) / ((int64_t)g.TY * 4);
     if (chunks > most) chunks = most;
@@ -361,11 +374,14 @@ static int gn_fwd_any(const void *x, const float *gamma, const float *beta, void
     const GnGeom g = gn_geom(group, S, C, G, VEC);
     for (int64_t b0 = 0; b0 < B; b0 += group) {
         const int64_t nb = B - b0 < group ? B - b0 : group, pairs = nb * G;
-        const int64_t ctas = nb * g.chunks * g.tiles, warps = (pairs + kThreads / 32 - 1) / (kThreads / 32);
-        if (ctas > INT32_MAX || warps > INT32_MAX) return HGQ_ERR_SIZE;
+        const int64_t ctas = nb * g.chunks * g.tiles;
+        const bool wide = (int64_t)g.chunks * g.Cg > 256;  // parts of a total: a block for each, or a warp
+        const int64_t sums = wide ? pairs : (pairs + kThreads / 32 - 1) / (kThreads / 32);
+        if (ctas > INT32_MAX || sums > INT32_MAX || (int64_t)g.chunks * g.Cg > INT32_MAX) return HGQ_ERR_SIZE;
         k_gn_stats<T, VEC><<<(unsigned)ctas, kThreads, 0, st>>>((const T *)x, g, b0, part);
         if (int e = check_launch()) return e;
-        k_gn_totals<<<(unsigned)warps, kThreads, 0, st>>>(part, g, b0, pairs, eps, mean, rstd);
+        if (wide) k_gn_totals<kThreads><<<(unsigned)sums, kThreads, 0, st>>>(part, g, b0, pairs, eps, mean, rstd);
+        else k_gn_totals<32><<<(unsigned)sums, kThreads, 0, st>>>(part, g, b0, pairs, eps, mean, rstd);
         if (int e = check_launch()) return e;
         k_gn_apply<T, VEC><<<(unsigned)ctas, kThreads, 0, st>>>((const T *)x, gamma, beta, mean, rstd, g, b0, act, (T *)y);
         if (int e = check_launch()) return e;
@@ -395,13 +411,16 @@ static int gn_bwd_any(const void *gy, const void *x, const float *gamma, const f
     const GnGeom g = gn_geom(group, S, C, G, VEC);
     for (int64_t b0 = 0; b0 < B; b0 += group) {
         const int64_t nb = B - b0 < group ? B - b0 : group, pairs = nb * G;
-        const int64_t ctas = nb * g.chunks * g.tiles, warps = (pairs + kThreads / 32 - 1) / (kThreads / 32);
-        if (ctas > INT32_MAX || warps > INT32_MAX) return HGQ_ERR_SIZE;
+        const int64_t ctas = nb * g.chunks * g.tiles;
+        const bool wide = (int64_t)g.chunks * g.Cg > 256;  // parts of a total: a block for each, or a warp
+        const int64_t sums = wide ? pairs : (pairs + kThreads / 32 - 1) / (kThreads / 32);
+        if (ctas > INT32_MAX || sums > INT32_MAX || (int64_t)g.chunks * g.Cg > INT32_MAX) return HGQ_ERR_SIZE;
         float *p = part + b0 * g.chunks * 2 * C;
         k_gn_bwd_stats<T, VEC><<<(unsigned)ctas, kThreads, 0, st>>>((const T *)gy, (const T *)x, gamma, beta, mean, rstd, g, b0, act, p);
         if (int e = check_launch()) return e;
         if (dx != nullptr) {
-            k_gn_bwd_totals<<<(unsigned)warps, kThreads, 0, st>>>(p, gamma, g, pairs, m, m + group * G);
+            if (wide) k_gn_bwd_totals<kThreads><<<(unsigned)sums, kThreads, 0, st>>>(p, gamma, g, pairs, m, m + group * G);
+            else k_gn_bwd_totals<32><<<(unsigned)sums, kThreads, 0, st>>>(p, gamma, g, pairs, m, m + group * G);
             if (int e = check_launch()) return e;
             k_gn_bwd_apply<T, VEC><<<(unsigned)ctas, kThreads, 0, st>>>((const T *)gy, (const T *)x, gamma, beta, mean, rstd, m, m + group * G, g,
                                                                        b0, act, (T *)dx);

@@ -73,7 +73,7 @@ __device__ __forceinline__ float act_slope(float u) {
 // shape is for the kernels that read twice.
 struct SlabPlan {
     bool usable;
-    bool multi;     // a thread's pack spans several groups
+    int groups_of_pack;  // numbers that a pack adds to: one a group where packs and groups nest, else one a channel
     int vec;        // channels a thread takes at once
     int R;          // packs of one tensor that a thread holds
     int K;          // CTAs of a cluster that share a slab's rows

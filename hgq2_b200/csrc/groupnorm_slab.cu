@@ -4,11 +4,11 @@
 // packs of VEC neighbouring channels in registers from the one read to the write.  The statistics are two block reductions (mean,
 // then centred squares: data whose mean is large against its spread keep their variance), joined over the cluster through
 // distributed shared memory in rank order.  Small samples share a CTA.  Registers rather than shared memory hold the data because
-// every value is used by the thread that loaded it; what crosses threads is one number a pack (a pack that spans several groups:
-// one a channel).
+// every value is used by the thread that loaded it; what crosses threads is one number a pack (one a group that the pack touches).
+// The CTAs are resident and walk over the samples.
 //
-// Backward: the CTAs are resident and walk over the samples, so that dgamma and dbeta stay in registers until the end (one row of
-// partial sums a CTA, added up in a fixed order by a second launch).  du gamma is kept in fp32 in place of gy between the two uses.
+// Backward: dgamma and dbeta add up in shared memory, a place for each thread, until the end (one row of partial sums a CTA, added
+// up in a fixed order by a second launch).  du gamma is kept in fp32 in place of gy between its two uses.
 #include <cooperative_groups.h>
 
 #include "groupnorm.cuh"
@@ -25,9 +25,14 @@ constexpr int kMaxPairs = 512;  // (sample, group) pairs of a CTA
 struct SlabArgs {
     int64_t B, S, items, workers;
     int C, G, Cg, Cs, Gs, slabs, TX, TY, K, subs, rows;
-    int width;    // reduction entries of a thread row: TX (one a pack) or TX VEC (one a channel)
-    int per_row;  // of them that belong to one group
-    FastDiv by_per_row;
+    int per_row;  // neighbouring threads of a row that belong to one group (one a pack), or 1
+    // Totals over a (sample, group).  `bits`: all extents are powers of two, so that the threads of one total differ exactly in
+    // certain bits of their index: those of lane_bits meet in shuffles, those of warp_bits through shared memory.
+    bool bits;
+    unsigned lane_bits, warp_bits;
+    // Otherwise: entries in shared memory, [TY][width], per_group of a row to one group.
+    int width, per_group;
+    FastDiv by_per_group;
 };
 
 // Where a thread works: its channels, its sample among the CTA's and its first row.
@@ -60,52 +65,121 @@ __device__ __forceinline__ SlabPlace slab_place(const SlabArgs &a, int vec) {
     return p;
 }
 
-// Sums over the (sample of the CTA, group) pairs.  entries: [TY][width] in shared memory, complete; out[pair] = the pair's sum, by a
-// power of two of neighbouring lanes each, all pairs at once where they are few.  Every thread of the block calls it.
-template <int N>
-__device__ __forceinline__ void pair_sums(const float *entries, int stride, float *out, int out_stride, const SlabArgs &a, const SlabPlace &p) {
-    const int pairs = a.subs * p.groups;
-    const int rows = a.subs > 1 ? (int)a.S : a.TY;
-    const int n = rows * a.per_row;
-    int lanes = 32;
-    while (lanes > 1 && (lanes * pairs > kSlabThreads || lanes > n)) lanes >>= 1;
-    const int at_once = kSlabThreads / lanes, l = threadIdx.x % lanes, first = threadIdx.x / lanes;
-    for (int base = 0; base < pairs; base += at_once) {
-        const int pair = base + first;
-        float s[N];
+// What a CTA needs to add up N sets of NG numbers a thread over the threads of each (sample, group).
+template <int NG, int N>
+struct SumSpace {
+    float entries[N * NG * kSlabThreads];
+    float pair[2][N][kMaxPairs];  // by turns
+    float all[N][kMaxPairs];      // over the cluster
+};
+
+// v: in, a thread's numbers (one a group that its pack touches; NG == VEC: one a channel), out, the totals of their groups, over the
+// cluster.  pair_of: the (sample of the CTA, group) of each.  Every thread of the block calls it, `turn` alternating.
+template <int NG, int N>
+__device__ __forceinline__ void group_totals(float (&v)[N][NG], SumSpace<NG, N> &sh, int turn, const int (&pair_of)[NG], const SlabArgs &a,
+                                             const SlabPlace &p) {
+    const int tid = threadIdx.x;
+    if (a.bits) {
+        for (unsigned o = 1; o < 32; o <<= 1)
+            if (a.lane_bits & o)
 #pragma unroll
-        for (int k = 0; k < N; ++k) s[k] = 0.f;
-        if (pair < pairs) {
-            const int sub = a.subs > 1 ? pair / p.groups : 0, g = pair - sub * p.groups;
-            const float *e = entries + (sub * rows) * a.width + g * a.per_row;
-            for (int j = l; j < n; j += lanes) {
-                const int r = (int)fastdiv((uint32_t)j, a.by_per_row), c = j - r * a.per_row;
+                for (int k = 0; k < N; ++k)
 #pragma unroll
-                for (int k = 0; k < N; ++k) s[k] += e[k * stride + r * a.width + c];
-            }
+                    for (int i = 0; i < NG; ++i) v[k][i] += __shfl_xor_sync(0xffffffffu, v[k][i], o);
+        if (a.warp_bits != 0) {
+            float *e = sh.entries;
+            if ((tid & a.lane_bits) == 0)
+#pragma unroll
+                for (int k = 0; k < N; ++k)
+#pragma unroll
+                    for (int i = 0; i < NG; ++i) e[(k * NG + i) * kSlabThreads + tid] = v[k][i];
+            __syncthreads();
+            const int base = tid & ~(int)(a.lane_bits | a.warp_bits);
+#pragma unroll
+            for (int k = 0; k < N; ++k)
+#pragma unroll
+                for (int i = 0; i < NG; ++i) v[k][i] = 0.f;
+            // the subsets of warp_bits in ascending order
+            unsigned w = 0;
+            do {
+#pragma unroll
+                for (int k = 0; k < N; ++k)
+#pragma unroll
+                    for (int i = 0; i < NG; ++i) v[k][i] += e[(k * NG + i) * kSlabThreads + (base | w)];
+                w = (w - a.warp_bits) & a.warp_bits;
+            } while (w != 0);
         }
-        for (int o = lanes >> 1; o > 0; o >>= 1)
+        if (a.K > 1 && p.in && (tid & (a.lane_bits | a.warp_bits)) == 0)
 #pragma unroll
-            for (int k = 0; k < N; ++k) s[k] += __shfl_xor_sync(0xffffffffu, s[k], o);
-        if (pair < pairs && l == 0)
+            for (int k = 0; k < N; ++k)
 #pragma unroll
-            for (int k = 0; k < N; ++k) out[k * out_stride + pair] = s[k];
+                for (int i = 0; i < NG; ++i) sh.pair[turn][k][pair_of[i]] = v[k][i];
+        if (a.K == 1) {
+            if (a.warp_bits != 0) __syncthreads();  // the entries are free again
+            return;
+        }
+    } else {
+        const int pairs = a.subs * p.groups, rows = a.subs > 1 ? (int)a.S : a.TY, n = rows * a.per_group;
+        if (p.ty < a.TY)
+#pragma unroll
+            for (int k = 0; k < N; ++k)
+#pragma unroll
+                for (int i = 0; i < NG; ++i) sh.entries[k * NG * kSlabThreads + p.ty * a.width + p.tx * NG + i] = v[k][i];
+        __syncthreads();
+        // a power of two of neighbouring lanes for each pair, all pairs at once where they are few
+        int lanes = 32;
+        while (lanes > 1 && (lanes * pairs > kSlabThreads || lanes > n)) lanes >>= 1;
+        const int at_once = kSlabThreads / lanes, l = tid & (lanes - 1), first = tid / lanes;
+        for (int base = 0; base < pairs; base += at_once) {
+            const int pair = base + first;
+            float s[N];
+#pragma unroll
+            for (int k = 0; k < N; ++k) s[k] = 0.f;
+            if (pair < pairs) {
+                const int sub = a.subs > 1 ? pair / p.groups : 0, g = pair - sub * p.groups;
+                const float *e = sh.entries + (sub * rows) * a.width + g * a.per_group;
+                for (int j = l; j < n; j += lanes) {
+                    const int r = (int)fastdiv((uint32_t)j, a.by_per_group), c = j - r * a.per_group;
+#pragma unroll
+                    for (int k = 0; k < N; ++k) s[k] += e[k * NG * kSlabThreads + r * a.width + c];
+                }
+            }
+            for (int o = lanes >> 1; o > 0; o >>= 1)
+#pragma unroll
+                for (int k = 0; k < N; ++k) s[k] += __shfl_xor_sync(0xffffffffu, s[k], o);
+            if (pair < pairs && l == 0)
+#pragma unroll
+                for (int k = 0; k < N; ++k) sh.pair[turn][k][pair] = s[k];
+        }
     }
+    if (a.K > 1) {
+        // the CTAs' totals in rank order; each CTA's of this turn stay until the next turn's barrier
+        cg::cluster_group cluster = cg::this_cluster();
+        cluster.sync();
+        const int pairs = a.subs * p.groups;
+        for (int i = tid; i < pairs; i += kSlabThreads)
+#pragma unroll
+            for (int k = 0; k < N; ++k) {
+                float t = 0.f;
+                for (int r = 0; r < a.K; ++r) t += *cluster.map_shared_rank(&sh.pair[turn][k][i], r);
+                sh.all[k][i] = t;
+            }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < N; ++k)
+#pragma unroll
+        for (int i = 0; i < NG; ++i) v[k][i] = a.K > 1 ? sh.all[k][pair_of[i]] : sh.pair[turn][k][pair_of[i]];
 }
 
-// One thread's contributions (VEC channel sums) into the entries: one a pack or one a channel.
-template <int VEC, bool MULTI>
-__device__ __forceinline__ void put_entries(float *entries, const float (&v)[VEC], const SlabArgs &a, const SlabPlace &p) {
-    if (p.ty >= a.TY) return;
-    float *e = entries + p.ty * a.width;
-    if (MULTI) {
+// The channels of a pack as the NG groups they belong to.
+template <int VEC, int NG>
+__device__ __forceinline__ void join_channels(const float (&c)[VEC], float (&g)[NG]) {
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) e[p.tx * VEC + i] = v[i];
-    } else {
-        float s = v[0];
+    for (int i = 0; i < NG; ++i) {
+        g[i] = c[i * (VEC / NG)];
 #pragma unroll
-        for (int i = 1; i < VEC; ++i) s += v[i];
-        e[p.tx] = s;
+        for (int j = 1; j < VEC / NG; ++j) g[i] += c[i * (VEC / NG) + j];
     }
 }
 
@@ -152,38 +226,40 @@ struct Held {
     }
 };
 
-template <typename T, int VEC, int R, bool MULTI>
+template <typename T, int VEC, int R, int NG>
 __global__ void __launch_bounds__(kSlabThreads, R * VEC >= 64 ? 2 : (R * VEC >= 32 ? 3 : 4))
     k_gn_slab_fwd(const T *__restrict__ x, const float *__restrict__ gamma, const float *__restrict__ beta, const SlabArgs a, float eps, int act,
                   T *__restrict__ y, float *__restrict__ mean_out, float *__restrict__ rstd_out) {
-    __shared__ float entries[kSlabThreads * (MULTI ? VEC : 1)];
-    __shared__ float local[2][kMaxPairs], total[2][kMaxPairs];
+    constexpr int W = VEC / NG;  // channels of a pack in one group
+    __shared__ SumSpace<NG, 1> sh;
     const SlabPlace p = slab_place(a, VEC);
     const int c0 = p.slab * a.Cs + p.tx * VEC;
-    const int pairs = a.subs * p.groups;
     const float inv_n = 1.f / ((float)a.S * (float)a.Cg);
     float ga[VEC], be[VEC];
-    int pair_of[MULTI ? VEC : 1];
+    int pair_of[NG], group_of[NG];
 #pragma unroll
     for (int i = 0; i < VEC; ++i) {
         ga[i] = p.in && gamma != nullptr ? gamma[c0 + i] : 1.f;
         be[i] = p.in && beta != nullptr ? beta[c0 + i] : 0.f;
-        if (MULTI || i == 0) pair_of[i] = p.in ? p.sub * p.groups + (p.tx * VEC + i) / a.Cg : 0;
     }
+#pragma unroll
+    for (int i = 0; i < NG; ++i) {
+        group_of[i] = p.in ? (p.tx * VEC + i * W) / a.Cg : 0;
+        pair_of[i] = (p.in ? p.sub : 0) * p.groups + group_of[i];
+    }
+    const int64_t step = (int64_t)a.TY * a.C, end = a.subs > 1 ? a.S : min(a.S, (int64_t)(p.rank + 1) * a.rows);
+    const int64_t row = (int64_t)p.rank * a.rows + p.row;
+    unsigned rows_mask = 0;
+#pragma unroll
+    for (int j = 0; j < R; ++j)
+        if (row + j * a.TY < end && (j == 0 || a.subs == 1)) rows_mask |= 1u << j;
     for (int64_t item = p.worker; item < a.items; item += a.workers) {
         const int64_t b = item * a.subs + p.sub;
-        const int64_t row = (int64_t)p.rank * a.rows + p.row;
-        unsigned mask = 0;
-        if (p.in && b < a.B) {
-            const int64_t end = a.subs > 1 ? a.S : min(a.S, (int64_t)(p.rank + 1) * a.rows);
-#pragma unroll
-            for (int j = 0; j < R; ++j)
-                if (row + j * a.TY < end && (j == 0 || a.subs == 1)) mask |= 1u << j;
-        }
-        const int64_t base = (b * a.S + row) * a.C + c0, step = (int64_t)a.TY * a.C;
+        const unsigned mask = p.in && b < a.B ? rows_mask : 0;
+        const int64_t base = (b * a.S + row) * a.C + c0;
         Held<T, VEC, R> h;
         h.load(x + base, step, mask);
-        float s[VEC];
+        float s[VEC], mu[1][NG], rs[1][NG];
 #pragma unroll
         for (int i = 0; i < VEC; ++i) s[i] = 0.f;
 #pragma unroll
@@ -193,65 +269,41 @@ __global__ void __launch_bounds__(kSlabThreads, R * VEC >= 64 ? 2 : (R * VEC >= 
 #pragma unroll
             for (int i = 0; i < VEC; ++i) s[i] += v[i];
         }
-        // mean, then centred squares
-        float mu[MULTI ? VEC : 1], rs[MULTI ? VEC : 1];
+        join_channels<VEC, NG>(s, mu[0]);
+        group_totals<NG, 1>(mu, sh, 0, pair_of, a, p);
 #pragma unroll
-        for (int phase = 0; phase < 2; ++phase) {
-            put_entries<VEC, MULTI>(entries, s, a, p);
-            __syncthreads();
-            pair_sums<1>(entries, 0, local[phase], 0, a, p);
-            if (a.K > 1) {
-                cg::cluster_group cluster = cg::this_cluster();
-                cluster.sync();
-                for (int i = threadIdx.x; i < pairs; i += kSlabThreads) {
-                    float t = 0.f;
-                    for (int k = 0; k < a.K; ++k) t += *cluster.map_shared_rank(&local[phase][i], k);
-                    total[phase][i] = t;
+        for (int i = 0; i < NG; ++i) mu[0][i] *= inv_n;
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) s[i] = 0.f;
+#pragma unroll
+        for (int j = 0; j < R; ++j)
+            if (mask >> j & 1) {
+                float v[VEC];
+                h.values(j, v);
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) {
+                    const float d = v[i] - mu[0][i / W];
+                    s[i] += d * d;
                 }
-            } else {
-                __syncthreads();
             }
-            const float *sums = a.K > 1 ? total[phase] : local[phase];
-            if (a.K > 1) __syncthreads();
-            if (phase == 0) {
+        join_channels<VEC, NG>(s, rs[0]);
+        group_totals<NG, 1>(rs, sh, 1, pair_of, a, p);
 #pragma unroll
-                for (int i = 0; i < (MULTI ? VEC : 1); ++i) mu[i] = sums[pair_of[i]] * inv_n;
-#pragma unroll
-                for (int i = 0; i < VEC; ++i) s[i] = 0.f;
-#pragma unroll
-                for (int j = 0; j < R; ++j)
-                    if (mask >> j & 1) {
-                        float v[VEC];
-                        h.values(j, v);
-#pragma unroll
-                        for (int i = 0; i < VEC; ++i) {
-                            const float d = v[i] - mu[MULTI ? i : 0];
-                            s[i] += d * d;
-                        }
-                    }
-            } else {
-#pragma unroll
-                for (int i = 0; i < (MULTI ? VEC : 1); ++i) rs[i] = 1.f / sqrtf(sums[pair_of[i]] * inv_n + eps);
-                if (p.rank == 0)
-                    for (int i = threadIdx.x; i < pairs; i += kSlabThreads) {
-                        const int sub = i / p.groups;
-                        const int64_t bb = item * a.subs + sub;
-                        if (bb < a.B) {
-                            const int64_t o = bb * a.G + p.slab * a.Gs + (i - sub * p.groups);
-                            mean_out[o] = (a.K > 1 ? total[0][i] : local[0][i]) * inv_n;
-                            rstd_out[o] = 1.f / sqrtf(sums[i] * inv_n + eps);
-                        }
-                    }
+        for (int i = 0; i < NG; ++i) {
+            rs[0][i] = 1.f / sqrtf(rs[0][i] * inv_n + eps);
+            // the first thread of each (sample, group): the first row's first pack of it
+            if (p.in && b < a.B && p.rank == 0 && p.row == 0 && (p.tx * VEC + i * W) % a.Cg == 0) {
+                const int64_t o = b * a.G + p.slab * a.Gs + group_of[i];
+                mean_out[o] = mu[0][i];
+                rstd_out[o] = rs[0][i];
             }
         }
         GN_FOR_ACT(act, {
             _Pragma("unroll") for (int j = 0; j < R; ++j) if (mask >> j & 1) {
                 float v[VEC];
                 h.values(j, v);
-                _Pragma("unroll") for (int i = 0; i < VEC; ++i) {
-                    const int m = MULTI ? i : 0;
-                    v[i] = act_value<T, ACT>((v[i] - mu[m]) * (rs[m] * ga[i]) + be[i]);
-                }
+                _Pragma("unroll") for (int i = 0; i < VEC; ++i)
+                    v[i] = act_value<T, ACT>((v[i] - mu[0][i / W]) * (rs[0][i / W] * ga[i]) + be[i]);
                 store_pack<T, VEC>(y + base + j * step, v);
             }
         })
@@ -259,55 +311,52 @@ __global__ void __launch_bounds__(kSlabThreads, R * VEC >= 64 ? 2 : (R * VEC >= 
     if (a.K > 1) cg::this_cluster().sync();  // no CTA leaves while another may still read its sums
 }
 
-template <typename T, int VEC, int R, bool MULTI>
+template <typename T, int VEC, int R, int NG>
 __global__ void __launch_bounds__(kSlabThreads, 2)
     k_gn_slab_bwd(const T *__restrict__ gy, const T *__restrict__ x, const float *__restrict__ gamma, const float *__restrict__ beta,
                   const float *__restrict__ mean, const float *__restrict__ rstd, const SlabArgs a, int act, T *__restrict__ dx,
                   float *__restrict__ part) {
-    constexpr int kEntries = kSlabThreads * (MULTI ? VEC : 1);
-    __shared__ float entries[2 * kEntries];
-    __shared__ float local[2][2 * kMaxPairs], total[2][2 * kMaxPairs];
+    constexpr int W = VEC / NG;
+    __shared__ SumSpace<NG, 2> sh;
     __shared__ float acc[2 * VEC][kSlabThreads];  // du and du xhat of this thread's channels, over all of the CTA's samples
     const SlabPlace p = slab_place(a, VEC);
     const int c0 = p.slab * a.Cs + p.tx * VEC;
-    const int pairs = a.subs * p.groups;
     const float inv_n = 1.f / ((float)a.S * (float)a.Cg);
     float ga[VEC], be[VEC];
-    int pair_of[MULTI ? VEC : 1], group_of[MULTI ? VEC : 1];
+    int pair_of[NG], group_of[NG];
 #pragma unroll
     for (int i = 0; i < VEC; ++i) {
         ga[i] = p.in && gamma != nullptr ? gamma[c0 + i] : 1.f;
         be[i] = p.in && beta != nullptr ? beta[c0 + i] : 0.f;
         acc[i][threadIdx.x] = acc[VEC + i][threadIdx.x] = 0.f;
-        if (MULTI || i == 0) {
-            group_of[i] = p.in ? (p.tx * VEC + i) / a.Cg : 0;
-            pair_of[i] = (p.in ? p.sub : 0) * p.groups + group_of[i];
-        }
     }
+#pragma unroll
+    for (int i = 0; i < NG; ++i) {
+        group_of[i] = p.in ? (p.tx * VEC + i * W) / a.Cg : 0;
+        pair_of[i] = (p.in ? p.sub : 0) * p.groups + group_of[i];
+    }
+    const int64_t step = (int64_t)a.TY * a.C, end = a.subs > 1 ? a.S : min(a.S, (int64_t)(p.rank + 1) * a.rows);
+    const int64_t row = (int64_t)p.rank * a.rows + p.row;
+    unsigned rows_mask = 0;
+#pragma unroll
+    for (int j = 0; j < R; ++j)
+        if (row + j * a.TY < end && (j == 0 || a.subs == 1)) rows_mask |= 1u << j;
     int turn = 0;
     for (int64_t item = p.worker; item < a.items; item += a.workers, turn ^= 1) {
         const int64_t b = item * a.subs + p.sub;
-        const int64_t row = (int64_t)p.rank * a.rows + p.row;
-        unsigned mask = 0;
-        float mu[MULTI ? VEC : 1], rs[MULTI ? VEC : 1];
-#pragma unroll
-        for (int i = 0; i < (MULTI ? VEC : 1); ++i) mu[i] = rs[i] = 0.f;
-        if (p.in && b < a.B) {
-            const int64_t end = a.subs > 1 ? a.S : min(a.S, (int64_t)(p.rank + 1) * a.rows);
-#pragma unroll
-            for (int j = 0; j < R; ++j)
-                if (row + j * a.TY < end && (j == 0 || a.subs == 1)) mask |= 1u << j;
-#pragma unroll
-            for (int i = 0; i < (MULTI ? VEC : 1); ++i) {
-                const int64_t o = b * a.G + p.slab * a.Gs + group_of[i];
-                mu[i] = mean[o];
-                rs[i] = rstd[o];
-            }
-        }
-        const int64_t base = (b * a.S + row) * a.C + c0, step = (int64_t)a.TY * a.C;
+        const bool in = p.in && b < a.B;
+        const unsigned mask = in ? rows_mask : 0;
+        const int64_t base = (b * a.S + row) * a.C + c0;
         Held<T, VEC, R> h, hg;
         h.load(x + base, step, mask);
         hg.load(gy + base, step, mask);
+        float mu[NG], rs[NG];
+#pragma unroll
+        for (int i = 0; i < NG; ++i) {
+            const int64_t o = b * a.G + p.slab * a.Gs + group_of[i];
+            mu[i] = in ? mean[o] : 0.f;
+            rs[i] = in ? rstd[o] : 0.f;
+        }
         float t[R][VEC], du_[VEC], dux[VEC];  // t: du gamma
 #pragma unroll
         for (int i = 0; i < VEC; ++i) du_[i] = dux[i] = 0.f;
@@ -317,8 +366,7 @@ __global__ void __launch_bounds__(kSlabThreads, 2)
                 h.values(j, v);
                 hg.values(j, d);
                 _Pragma("unroll") for (int i = 0; i < VEC; ++i) {
-                    const int m = MULTI ? i : 0;
-                    const float xh = (v[i] - mu[m]) * rs[m];
+                    const float xh = (v[i] - mu[i / W]) * rs[i / W];
                     const float du = d[i] * act_slope<T, ACT>(xh * ga[i] + be[i]);
                     du_[i] += du;
                     dux[i] += du * xh;
@@ -326,40 +374,22 @@ __global__ void __launch_bounds__(kSlabThreads, 2)
                 }
             }
         })
-        float w1[VEC], w2[VEC];
 #pragma unroll
         for (int i = 0; i < VEC; ++i) {
             acc[i][threadIdx.x] += du_[i];
             acc[VEC + i][threadIdx.x] += dux[i];
-            w1[i] = du_[i] * ga[i];
-            w2[i] = dux[i] * ga[i];
+            du_[i] *= ga[i];
+            dux[i] *= ga[i];
         }
         if (dx == nullptr) continue;  // the parameters' gradients alone
-        put_entries<VEC, MULTI>(entries, w1, a, p);
-        put_entries<VEC, MULTI>(entries + kEntries, w2, a, p);
-        __syncthreads();
-        pair_sums<2>(entries, kEntries, local[turn], kMaxPairs, a, p);
-        const float *sums = local[turn];
-        if (a.K > 1) {
-            cg::cluster_group cluster = cg::this_cluster();
-            cluster.sync();
-            for (int i = threadIdx.x; i < pairs; i += kSlabThreads) {
-                float t1 = 0.f, t2 = 0.f;
-                for (int k = 0; k < a.K; ++k) {
-                    t1 += *cluster.map_shared_rank(&local[turn][i], k);
-                    t2 += *cluster.map_shared_rank(&local[turn][kMaxPairs + i], k);
-                }
-                total[turn][i] = t1;
-                total[turn][kMaxPairs + i] = t2;
-            }
-            sums = total[turn];
-        }
-        __syncthreads();
-        float m1[MULTI ? VEC : 1], m2[MULTI ? VEC : 1];
+        float m[2][NG];
+        join_channels<VEC, NG>(du_, m[0]);
+        join_channels<VEC, NG>(dux, m[1]);
+        group_totals<NG, 2>(m, sh, turn, pair_of, a, p);
 #pragma unroll
-        for (int i = 0; i < (MULTI ? VEC : 1); ++i) {
-            m1[i] = sums[pair_of[i]] * inv_n;
-            m2[i] = sums[kMaxPairs + pair_of[i]] * inv_n;
+        for (int i = 0; i < NG; ++i) {
+            m[0][i] *= inv_n;
+            m[1][i] *= inv_n;
         }
 #pragma unroll
         for (int j = 0; j < R; ++j)
@@ -368,9 +398,8 @@ __global__ void __launch_bounds__(kSlabThreads, 2)
                 h.values(j, v);
 #pragma unroll
                 for (int i = 0; i < VEC; ++i) {
-                    const int m = MULTI ? i : 0;
-                    const float xh = (v[i] - mu[m]) * rs[m];
-                    v[i] = rs[m] * (t[j][i] - m1[m] - xh * m2[m]);
+                    const float xh = (v[i] - mu[i / W]) * rs[i / W];
+                    v[i] = rs[i / W] * (t[j][i] - m[0][i / W] - xh * m[1][i / W]);
                 }
                 store_pack<T, VEC>(dx + base + j * step, v);
             }
@@ -406,7 +435,7 @@ SlabPlan gn_slab_plan(int64_t B, int64_t S, int C, int G, int type, int vec, boo
     const int Cg = C / G, size = type == HGQ_TYPE_F32 ? 4 : 2;
     const int most = slab_most(type, vec, backward);
     p.vec = vec;
-    p.multi = Cg % vec != 0;
+    p.groups_of_pack = Cg % vec == 0 ? 1 : (vec % Cg == 0 ? vec / Cg : vec);
     // whole groups whose channels are whole packs
     int unit = Cg;
     while (unit % vec != 0) unit += Cg;  // at most vec groups
@@ -442,13 +471,11 @@ SlabPlan gn_slab_plan(int64_t B, int64_t S, int C, int G, int type, int vec, boo
     p.R = need <= 1 ? 1 : (need <= 4 && most != 16 ? 4 : most);
     p.items = (B + p.subs - 1) / p.subs;
     if (p.items * p.slabs * p.K > INT32_MAX) return p;
-    p.workers = p.items;
-    if (backward) {
-        // resident CTAs: two an SM; a cluster's CTAs are placed together
-        int64_t n = (int64_t)num_sms() * 2 / ((int64_t)p.K * p.slabs);
-        if (n < 1) n = 1;
-        if (p.workers > n) p.workers = n;
-    }
+    // resident CTAs, by their registers: what a CTA sets up once (places, scale and offset) is spread over its samples
+    const int held = p.R * vec;
+    int64_t n = (int64_t)num_sms() * (backward || held >= 64 ? 2 : (held >= 32 ? 3 : 4)) / ((int64_t)p.K * p.slabs);
+    if (n < 1) n = 1;
+    p.workers = p.items < n ? p.items : n;
     p.usable = true;
     return p;
 }
@@ -458,9 +485,20 @@ static SlabArgs slab_args(const SlabPlan &p, int64_t B, int64_t S, int C, int G)
     a.B = B, a.S = S, a.items = p.items, a.workers = p.workers;
     a.C = C, a.G = G, a.Cg = C / G, a.Cs = p.Cs, a.Gs = p.Gs, a.slabs = p.slabs, a.TX = p.TX, a.TY = p.TY, a.K = p.K, a.subs = p.subs,
     a.rows = p.rows;
-    a.width = p.multi ? p.TX * p.vec : p.TX;
-    a.per_row = p.multi ? a.Cg : a.Cg / p.vec;
-    a.by_per_row = make_fastdiv((uint32_t)a.per_row);
+    a.per_row = a.Cg % p.vec == 0 ? a.Cg / p.vec : 1;
+    // one number a pack where it lies in one group, else one a group it touches or one a channel
+    const int ng = p.groups_of_pack;
+    a.width = p.TX * ng;
+    a.per_group = ng == 1 ? a.per_row : (ng * a.Cg == p.vec ? 1 : a.Cg);
+    a.by_per_group = make_fastdiv((uint32_t)a.per_group);
+    auto pow2 = [](int64_t v) { return v > 0 && (v & (v - 1)) == 0; };
+    // thread index, from the low bit: packs of a group, groups, rows of a sample, samples
+    a.bits = pow2(p.TX) && pow2(a.per_row) && p.TX * p.TY == kSlabThreads && C % p.Cs == 0 && (p.subs == 1 || pow2(S)) &&
+             (ng == 1 ? a.Cg % p.vec == 0 : ng * a.Cg == p.vec);
+    const unsigned rows = p.subs > 1 ? (unsigned)S : (unsigned)p.TY;
+    const unsigned bits = (unsigned)(a.per_row - 1) | ((rows - 1) * (unsigned)p.TX);
+    a.lane_bits = bits & 31u;
+    a.warp_bits = bits & ~31u;
     return a;
 }
 
@@ -488,20 +526,22 @@ template <typename T, int VEC, int R>
 static int slab_fwd(const SlabPlan &p, const SlabArgs &a, const void *x, const float *gamma, const float *beta, void *y, float *mean, float *rstd,
                     float eps, int act, cudaStream_t st) {
     const int64_t ctas = p.workers * p.slabs * p.K;
-    if (VEC > 1 && p.multi)
-        return launch_clusters(k_gn_slab_fwd<T, VEC, R, true>, ctas, p.K, st, (const T *)x, gamma, beta, a, eps, act, (T *)y, mean, rstd);
-    return launch_clusters(k_gn_slab_fwd<T, VEC, R, false>, ctas, p.K, st, (const T *)x, gamma, beta, a, eps, act, (T *)y, mean, rstd);
+    auto kernel = k_gn_slab_fwd<T, VEC, R, 1>;
+    if (VEC > 1 && p.groups_of_pack == 2) kernel = k_gn_slab_fwd<T, VEC, R, (VEC > 1 ? 2 : 1)>;
+    if (VEC > 4 && p.groups_of_pack == 4) kernel = k_gn_slab_fwd<T, VEC, R, (VEC > 4 ? 4 : VEC)>;
+    if (VEC > 2 && p.groups_of_pack == VEC) kernel = k_gn_slab_fwd<T, VEC, R, VEC>;
+    return launch_clusters(kernel, ctas, p.K, st, (const T *)x, gamma, beta, a, eps, act, (T *)y, mean, rstd);
 }
 
 template <typename T, int VEC, int R>
 static int slab_bwd(const SlabPlan &p, const SlabArgs &a, const void *gy, const void *x, const float *gamma, const float *beta, const float *mean,
                     const float *rstd, int act, void *dx, float *part, cudaStream_t st) {
     const int64_t ctas = p.workers * p.slabs * p.K;
-    if (VEC > 1 && p.multi)
-        return launch_clusters(k_gn_slab_bwd<T, VEC, R, true>, ctas, p.K, st, (const T *)gy, (const T *)x, gamma, beta, mean, rstd, a, act,
-                               (T *)dx, part);
-    return launch_clusters(k_gn_slab_bwd<T, VEC, R, false>, ctas, p.K, st, (const T *)gy, (const T *)x, gamma, beta, mean, rstd, a, act, (T *)dx,
-                           part);
+    auto kernel = k_gn_slab_bwd<T, VEC, R, 1>;
+    if (VEC > 1 && p.groups_of_pack == 2) kernel = k_gn_slab_bwd<T, VEC, R, (VEC > 1 ? 2 : 1)>;
+    if (VEC > 4 && p.groups_of_pack == 4) kernel = k_gn_slab_bwd<T, VEC, R, (VEC > 4 ? 4 : VEC)>;
+    if (VEC > 2 && p.groups_of_pack == VEC) kernel = k_gn_slab_bwd<T, VEC, R, VEC>;
+    return launch_clusters(kernel, ctas, p.K, st, (const T *)gy, (const T *)x, gamma, beta, mean, rstd, a, act, (T *)dx, part);
 }
 
 #define SLAB_DISPATCH(FN, FULL_MOST, ...)                                              \
