@@ -80,7 +80,8 @@ struct SlabPlan {
     int slabs;      // along the channels; Cs channels (whole groups) each, the last one may have fewer
     int Cs, Gs;
     int TX, TY;     // threads along channels and along rows
-    int subs;       // samples a CTA works on at once (small ones)
+    int subs;       // samples a CTA works on at once (small ones), TYs thread rows each
+    int TYs;
     int rows;       // of one CTA
     int64_t items;  // ceil(B / subs)
     int64_t workers;

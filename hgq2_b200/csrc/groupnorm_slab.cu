@@ -25,6 +25,7 @@ constexpr int kMaxPairs = 512;  // (sample, group) pairs of a CTA
 struct SlabArgs {
     int64_t B, S, items, workers;
     int C, G, Cg, Cs, Gs, slabs, TX, TY, K, subs, rows;
+    int TYs;  // thread rows of one sample: TY / subs
     int per_row;  // neighbouring threads of a row that belong to one group (one a pack), or 1
     // Totals over a (sample, group).  `bits`: all extents are powers of two, so that the threads of one total differ exactly in
     // certain bits of their index: those of lane_bits meet in shuffles, those of warp_bits through shared memory.
@@ -54,14 +55,9 @@ __device__ __forceinline__ SlabPlace slab_place(const SlabArgs &a, int vec) {
     p.tx = threadIdx.x % a.TX;
     p.ty = threadIdx.x / a.TX;
     p.in = p.ty < a.TY && p.tx * vec < p.channels;
-    if (a.subs > 1) {
-        p.sub = p.ty / (int)a.S;
-        p.row = p.ty % (int)a.S;
-        p.in = p.in && p.sub < a.subs;
-    } else {
-        p.sub = 0;
-        p.row = p.ty;
-    }
+    p.sub = a.subs > 1 ? p.ty / a.TYs : 0;
+    p.row = a.subs > 1 ? p.ty - p.sub * a.TYs : p.ty;
+    p.in = p.in && p.sub < a.subs;
     return p;
 }
 
@@ -80,6 +76,7 @@ __device__ __forceinline__ void group_totals(float (&v)[N][NG], SumSpace<NG, N> 
                                              const SlabPlace &p) {
     const int tid = threadIdx.x;
     if (a.bits) {
+#pragma unroll
         for (unsigned o = 1; o < 32; o <<= 1)
             if (a.lane_bits & o)
 #pragma unroll
@@ -99,15 +96,23 @@ __device__ __forceinline__ void group_totals(float (&v)[N][NG], SumSpace<NG, N> 
             for (int k = 0; k < N; ++k)
 #pragma unroll
                 for (int i = 0; i < NG; ++i) v[k][i] = 0.f;
-            // the subsets of warp_bits in ascending order
-            unsigned w = 0;
-            do {
+            if (a.warp_bits == kSlabThreads - 32) {  // all warps: the same sums in the same order, unrolled
 #pragma unroll
-                for (int k = 0; k < N; ++k)
+                for (int w = 0; w < kSlabWarps; ++w)
 #pragma unroll
-                    for (int i = 0; i < NG; ++i) v[k][i] += e[(k * NG + i) * kSlabThreads + (base | w)];
-                w = (w - a.warp_bits) & a.warp_bits;
-            } while (w != 0);
+                    for (int k = 0; k < N; ++k)
+#pragma unroll
+                        for (int i = 0; i < NG; ++i) v[k][i] += e[(k * NG + i) * kSlabThreads + base + w * 32];
+            } else {
+                unsigned w = 0;  // the subsets of warp_bits in ascending order
+                do {
+#pragma unroll
+                    for (int k = 0; k < N; ++k)
+#pragma unroll
+                        for (int i = 0; i < NG; ++i) v[k][i] += e[(k * NG + i) * kSlabThreads + (base | w)];
+                    w = (w - a.warp_bits) & a.warp_bits;
+                } while (w != 0);
+            }
         }
         if (a.K > 1 && p.in && (tid & (a.lane_bits | a.warp_bits)) == 0)
 #pragma unroll
@@ -119,7 +124,7 @@ __device__ __forceinline__ void group_totals(float (&v)[N][NG], SumSpace<NG, N> 
             return;
         }
     } else {
-        const int pairs = a.subs * p.groups, rows = a.subs > 1 ? (int)a.S : a.TY, n = rows * a.per_group;
+        const int pairs = a.subs * p.groups, rows = a.TYs, n = rows * a.per_group;
         if (p.ty < a.TY)
 #pragma unroll
             for (int k = 0; k < N; ++k)
@@ -237,6 +242,7 @@ __global__ void __launch_bounds__(kSlabThreads, R * VEC >= 64 ? 2 : (R * VEC >= 
     const float inv_n = 1.f / ((float)a.S * (float)a.Cg);
     float ga[VEC], be[VEC];
     int pair_of[NG], group_of[NG];
+    unsigned writes = 0;
 #pragma unroll
     for (int i = 0; i < VEC; ++i) {
         ga[i] = p.in && gamma != nullptr ? gamma[c0 + i] : 1.f;
@@ -246,13 +252,15 @@ __global__ void __launch_bounds__(kSlabThreads, R * VEC >= 64 ? 2 : (R * VEC >= 
     for (int i = 0; i < NG; ++i) {
         group_of[i] = p.in ? (p.tx * VEC + i * W) / a.Cg : 0;
         pair_of[i] = (p.in ? p.sub : 0) * p.groups + group_of[i];
+        // the first thread of each (sample, group) writes its statistics: the first row's first pack of it
+        if (p.in && p.rank == 0 && p.row == 0 && (p.tx * VEC + i * W) % a.Cg == 0) writes |= 1u << i;
     }
-    const int64_t step = (int64_t)a.TY * a.C, end = a.subs > 1 ? a.S : min(a.S, (int64_t)(p.rank + 1) * a.rows);
+    const int64_t step = (int64_t)a.TYs * a.C, end = min(a.S, (int64_t)(p.rank + 1) * a.rows);
     const int64_t row = (int64_t)p.rank * a.rows + p.row;
     unsigned rows_mask = 0;
 #pragma unroll
     for (int j = 0; j < R; ++j)
-        if (row + j * a.TY < end && (j == 0 || a.subs == 1)) rows_mask |= 1u << j;
+        if (row + j * a.TYs < end) rows_mask |= 1u << j;
     for (int64_t item = p.worker; item < a.items; item += a.workers) {
         const int64_t b = item * a.subs + p.sub;
         const unsigned mask = p.in && b < a.B ? rows_mask : 0;
@@ -290,9 +298,8 @@ __global__ void __launch_bounds__(kSlabThreads, R * VEC >= 64 ? 2 : (R * VEC >= 
         group_totals<NG, 1>(rs, sh, 1, pair_of, a, p);
 #pragma unroll
         for (int i = 0; i < NG; ++i) {
-            rs[0][i] = 1.f / sqrtf(rs[0][i] * inv_n + eps);
-            // the first thread of each (sample, group): the first row's first pack of it
-            if (p.in && b < a.B && p.rank == 0 && p.row == 0 && (p.tx * VEC + i * W) % a.Cg == 0) {
+            rs[0][i] = rsqrtf(rs[0][i] * inv_n + eps);
+            if ((writes >> i & 1) && b < a.B) {
                 const int64_t o = b * a.G + p.slab * a.Gs + group_of[i];
                 mean_out[o] = mu[0][i];
                 rstd_out[o] = rs[0][i];
@@ -335,12 +342,12 @@ __global__ void __launch_bounds__(kSlabThreads, 2)
         group_of[i] = p.in ? (p.tx * VEC + i * W) / a.Cg : 0;
         pair_of[i] = (p.in ? p.sub : 0) * p.groups + group_of[i];
     }
-    const int64_t step = (int64_t)a.TY * a.C, end = a.subs > 1 ? a.S : min(a.S, (int64_t)(p.rank + 1) * a.rows);
+    const int64_t step = (int64_t)a.TYs * a.C, end = min(a.S, (int64_t)(p.rank + 1) * a.rows);
     const int64_t row = (int64_t)p.rank * a.rows + p.row;
     unsigned rows_mask = 0;
 #pragma unroll
     for (int j = 0; j < R; ++j)
-        if (row + j * a.TY < end && (j == 0 || a.subs == 1)) rows_mask |= 1u << j;
+        if (row + j * a.TYs < end) rows_mask |= 1u << j;
     int turn = 0;
     for (int64_t item = p.worker; item < a.items; item += a.workers, turn ^= 1) {
         const int64_t b = item * a.subs + p.sub;
@@ -456,18 +463,25 @@ SlabPlan gn_slab_plan(int64_t B, int64_t S, int C, int G, int type, int vec, boo
     }
     p.Gs = p.Cs / Cg;
     p.slabs = (G + p.Gs - 1) / p.Gs;
+    // As few thread rows for a sample as hold it (what a total costs is a matter of threads, not of values): the CTA's others take
+    // other samples, if there are enough of them to give every SM two CTAs.
     p.subs = 1;
     p.K = 1;
-    if (2 * S <= p.TY) {
-        p.subs = p.TY / (int)S;
-        if (p.subs > B) p.subs = (int)B;
-        if (p.subs > kMaxPairs / p.Gs) p.subs = kMaxPairs / p.Gs;
-        if (p.subs < 1) p.subs = 1;
+    p.TYs = p.TY;
+    if (S <= (int64_t)p.TY * most) {
+        int rows = 1;
+        while ((int64_t)rows * most < S) rows <<= 1;
+        while (rows < p.TY && (B * rows < (int64_t)num_sms() * 2 * p.TY || p.TY / rows > kMaxPairs / p.Gs)) rows <<= 1;
+        if (2 * rows <= p.TY) {
+            p.TYs = rows;
+            p.subs = p.TY / rows;
+            if (p.subs > B) p.subs = (int)B;
+        }
     }
-    const int64_t packs = (S + p.TY - 1) / p.TY;  // a thread would hold with one CTA
+    const int64_t packs = (S + p.TYs - 1) / p.TYs;  // a thread would hold with one CTA
     while (packs > (int64_t)most * p.K) p.K <<= 1;
     p.rows = (int)((S + p.K - 1) / p.K);
-    const int need = (p.rows + p.TY - 1) / p.TY;
+    const int need = (p.rows + p.TYs - 1) / p.TYs;
     p.R = need <= 1 ? 1 : (need <= 4 && most != 16 ? 4 : most);
     p.items = (B + p.subs - 1) / p.subs;
     if (p.items * p.slabs * p.K > INT32_MAX) return p;
@@ -484,7 +498,7 @@ static SlabArgs slab_args(const SlabPlan &p, int64_t B, int64_t S, int C, int G)
     SlabArgs a{};
     a.B = B, a.S = S, a.items = p.items, a.workers = p.workers;
     a.C = C, a.G = G, a.Cg = C / G, a.Cs = p.Cs, a.Gs = p.Gs, a.slabs = p.slabs, a.TX = p.TX, a.TY = p.TY, a.K = p.K, a.subs = p.subs,
-    a.rows = p.rows;
+    a.rows = p.rows, a.TYs = p.TYs;
     a.per_row = a.Cg % p.vec == 0 ? a.Cg / p.vec : 1;
     // one number a pack where it lies in one group, else one a group it touches or one a channel
     const int ng = p.groups_of_pack;
@@ -493,10 +507,9 @@ static SlabArgs slab_args(const SlabPlan &p, int64_t B, int64_t S, int C, int G)
     a.by_per_group = make_fastdiv((uint32_t)a.per_group);
     auto pow2 = [](int64_t v) { return v > 0 && (v & (v - 1)) == 0; };
     // thread index, from the low bit: packs of a group, groups, rows of a sample, samples
-    a.bits = pow2(p.TX) && pow2(a.per_row) && p.TX * p.TY == kSlabThreads && C % p.Cs == 0 && (p.subs == 1 || pow2(S)) &&
+    a.bits = pow2(p.TX) && pow2(a.per_row) && p.TX * p.TY == kSlabThreads && C % p.Cs == 0 &&
              (ng == 1 ? a.Cg % p.vec == 0 : ng * a.Cg == p.vec);
-    const unsigned rows = p.subs > 1 ? (unsigned)S : (unsigned)p.TY;
-    const unsigned bits = (unsigned)(a.per_row - 1) | ((rows - 1) * (unsigned)p.TX);
+    const unsigned bits = (unsigned)(a.per_row - 1) | ((unsigned)(p.TYs - 1) * (unsigned)p.TX);
     a.lane_bits = bits & 31u;
     a.warp_bits = bits & ~31u;
     return a;
