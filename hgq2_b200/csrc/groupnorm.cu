@@ -37,6 +37,16 @@ __device__ __forceinline__ bool gn_place(const GnGeom &g, int64_t blk, int &b_re
     return ty < g.TY && c0 < g.C;
 }
 
+// Rows in flight at once, by the registers that a pack and its sums take.
+constexpr int kGnRows = 8, kGnApplyRows = 4, kGnBwdRows = 4;
+
+// Which of the rows r, r + TY, ... are before `end`.
+template <int ROWS>
+__device__ __forceinline__ unsigned rows_left(int64_t r, int64_t end, int TY) {
+    const int64_t n = (end - r + TY - 1) / TY;  // r < end
+    return n >= ROWS ? (1u << ROWS) - 1 : (1u << (int)n) - 1;
+}
+
 // Sum over ty of N values a thread; the result is in the threads of ty == 0.  `sh` has blockDim.x * N floats.
 template <int N>
 __device__ __forceinline__ void sum_over_ty(float (&v)[N], float *sh, const GnGeom &g, int tx, int ty) {
@@ -67,19 +77,26 @@ __global__ void __launch_bounds__(kThreads) k_gn_stats(const T *__restrict__ x, 
     float acc[2 * VEC], k[VEC];
 #pragma unroll
     for (int i = 0; i < VEC; ++i) acc[i] = acc[VEC + i] = k[i] = 0.f;
+    const int64_t step = (int64_t)g.TY * g.C;
     if (active) {
         const T *base = x + ((b_base + b) * g.S) * g.C + c0;
         load_pack<T, VEC>(base + r0 * g.C, k);
-#pragma unroll 4
-        for (int64_t r = r0 + ty; r < r1; r += g.TY) {
-            float v[VEC];
-            load_pack<T, VEC>(base + r * g.C, v);
+        for (int64_t r = r0 + ty; r < r1; r += (int64_t)kGnRows * g.TY) {
+            Held<T, VEC, kGnRows> h;
+            const unsigned mask = rows_left<kGnRows>(r, r1, g.TY);
+            h.load(base + r * g.C, step, mask);
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) {
-                const float d = v[i] - k[i];
-                acc[i] += d;
-                acc[VEC + i] += d * d;
-            }
+            for (int j = 0; j < kGnRows; ++j)
+                if (mask >> j & 1) {
+                    float v[VEC];
+                    h.values(j, v);
+#pragma unroll
+                    for (int i = 0; i < VEC; ++i) {
+                        const float d = v[i] - k[i];
+                        acc[i] += d;
+                        acc[VEC + i] += d * d;
+                    }
+                }
         }
     }
     sum_over_ty<2 * VEC>(acc, sh, g, tx, ty);
@@ -160,13 +177,18 @@ __global__ void __launch_bounds__(kThreads) k_gn_apply(const T *__restrict__ x, 
         sc[i] = rstd[pair] * (gamma ? gamma[c0 + i] : 1.f);
         of[i] = beta ? beta[c0 + i] : 0.f;
     }
-    const int64_t base = ((b_base + b) * g.S) * g.C + c0;
+    const int64_t base = ((b_base + b) * g.S) * g.C + c0, step = (int64_t)g.TY * g.C;
     GN_FOR_ACT(act, {
-        _Pragma("unroll 4") for (int64_t r = r0 + ty; r < r1; r += g.TY) {
-            float v[VEC];
-            load_pack<T, VEC>(x + base + r * g.C, v);
-            _Pragma("unroll") for (int i = 0; i < VEC; ++i) v[i] = act_value<T, ACT>((v[i] - mu[i]) * sc[i] + of[i]);
-            store_pack<T, VEC>(y + base + r * g.C, v);
+        for (int64_t r = r0 + ty; r < r1; r += (int64_t)kGnApplyRows * g.TY) {
+            Held<T, VEC, kGnApplyRows> h;
+            const unsigned mask = rows_left<kGnApplyRows>(r, r1, g.TY);
+            h.load(x + base + r * g.C, step, mask);
+            _Pragma("unroll") for (int j = 0; j < kGnApplyRows; ++j) if (mask >> j & 1) {
+                float v[VEC];
+                h.values(j, v);
+                _Pragma("unroll") for (int i = 0; i < VEC; ++i) v[i] = act_value<T, ACT>((v[i] - mu[i]) * sc[i] + of[i]);
+                store_pack<T, VEC>(y + base + r * g.C + j * step, v);
+            }
         }
     })
 }
@@ -194,17 +216,23 @@ __global__ void __launch_bounds__(kThreads) k_gn_bwd_stats(const T *__restrict__
             ga[i] = gamma ? gamma[c0 + i] : 1.f;
             be[i] = beta ? beta[c0 + i] : 0.f;
         }
-        const int64_t base = ((b_base + b) * g.S) * g.C + c0;
+        const int64_t base = ((b_base + b) * g.S) * g.C + c0, step = (int64_t)g.TY * g.C;
         GN_FOR_ACT(act, {
-            _Pragma("unroll 2") for (int64_t r = r0 + ty; r < r1; r += g.TY) {
-                float v[VEC], d[VEC];
-                load_pack<T, VEC>(x + base + r * g.C, v);
-                load_pack<T, VEC>(gy + base + r * g.C, d);
-                _Pragma("unroll") for (int i = 0; i < VEC; ++i) {
-                    const float xh = (v[i] - mu[i]) * rs[i];
-                    const float du = d[i] * act_slope<T, ACT>(xh * ga[i] + be[i]);
-                    acc[i] += du;
-                    acc[VEC + i] += du * xh;
+            for (int64_t r = r0 + ty; r < r1; r += (int64_t)kGnBwdRows * g.TY) {
+                Held<T, VEC, kGnBwdRows> h, hg;
+                const unsigned mask = rows_left<kGnBwdRows>(r, r1, g.TY);
+                h.load(x + base + r * g.C, step, mask);
+                hg.load(gy + base + r * g.C, step, mask);
+                _Pragma("unroll") for (int j = 0; j < kGnBwdRows; ++j) if (mask >> j & 1) {
+                    float v[VEC], d[VEC];
+                    h.values(j, v);
+                    hg.values(j, d);
+                    _Pragma("unroll") for (int i = 0; i < VEC; ++i) {
+                        const float xh = (v[i] - mu[i]) * rs[i];
+                        const float du = d[i] * act_slope<T, ACT>(xh * ga[i] + be[i]);
+                        acc[i] += du;
+                        acc[VEC + i] += du * xh;
+                    }
                 }
             }
         })
@@ -266,18 +294,24 @@ __global__ void __launch_bounds__(kThreads) k_gn_bwd_apply(const T *__restrict__
         a1[i] = m1[rel];
         a2[i] = m2[rel];
     }
-    const int64_t base = ((b_base + b) * g.S) * g.C + c0;
+    const int64_t base = ((b_base + b) * g.S) * g.C + c0, step = (int64_t)g.TY * g.C;
     GN_FOR_ACT(act, {
-        _Pragma("unroll 2") for (int64_t r = r0 + ty; r < r1; r += g.TY) {
-            float v[VEC], d[VEC];
-            load_pack<T, VEC>(x + base + r * g.C, v);
-            load_pack<T, VEC>(gy + base + r * g.C, d);
-            _Pragma("unroll") for (int i = 0; i < VEC; ++i) {
-                const float xh = (v[i] - mu[i]) * rs[i];
-                const float du = d[i] * act_slope<T, ACT>(xh * ga[i] + be[i]);
-                v[i] = rs[i] * (du * ga[i] - a1[i] - xh * a2[i]);
+        for (int64_t r = r0 + ty; r < r1; r += (int64_t)kGnBwdRows * g.TY) {
+            Held<T, VEC, kGnBwdRows> h, hg;
+            const unsigned mask = rows_left<kGnBwdRows>(r, r1, g.TY);
+            h.load(x + base + r * g.C, step, mask);
+            hg.load(gy + base + r * g.C, step, mask);
+            _Pragma("unroll") for (int j = 0; j < kGnBwdRows; ++j) if (mask >> j & 1) {
+                float v[VEC], d[VEC];
+                h.values(j, v);
+                hg.values(j, d);
+                _Pragma("unroll") for (int i = 0; i < VEC; ++i) {
+                    const float xh = (v[i] - mu[i]) * rs[i];
+                    const float du = d[i] * act_slope<T, ACT>(xh * ga[i] + be[i]);
+                    v[i] = rs[i] * (du * ga[i] - a1[i] - xh * a2[i]);
+                }
+                store_pack<T, VEC>(dx + base + r * g.C + j * step, v);
             }
-            store_pack<T, VEC>(dx + base + r * g.C, v);
         }
     })
 }
@@ -336,7 +370,7 @@ static GnGeom gn_geom(int64_t group, int64_t S, int C, int G, int vec) {
 static int gn_vec(const void *a, const void *b, const void *c, int C, int type) {
     const int size = type == HGQ_TYPE_F32 ? 4 : 2;
     const int full = 16 / size;
-    for (int v : {full, 2}) {
+    for (int v : {full, 4, 2}) {
         if (C % v == 0 && aligned(a, (size_t)v * size) && aligned(b, (size_t)v * size) && aligned(c, (size_t)v * size)) return v;
     }
     return 1;
@@ -347,7 +381,7 @@ static size_t gn_part_floats(int64_t B, int64_t S, int C, int G, int type, bool 
     const int size = type == HGQ_TYPE_F32 ? 4 : 2;
     const int64_t group = gn_group(B, S, C, bwd ? 2 * size : size);
     size_t most = 0;
-    for (int v : {16 / size, 2, 1}) {
+    for (int v : {16 / size, 4, 2, 1}) {
         if (C % v != 0) continue;
         const GnGeom g = gn_geom(group, S, C, G, v);
         const size_t any = (size_t)g.chunks * 2 * C * (size_t)(bwd ? B : group);
@@ -453,10 +487,12 @@ extern "C" size_t hgq_group_norm_workspace(int64_t B, int64_t S, int C, int G, i
         }                                                                                             \
         if (type == HGQ_TYPE_BF16) {                                                                  \
             if (vec == 8) return FN<__nv_bfloat16, 8>(__VA_ARGS__);                                   \
+            if (vec == 4) return FN<__nv_bfloat16, 4>(__VA_ARGS__);                                   \
             if (vec == 2) return FN<__nv_bfloat16, 2>(__VA_ARGS__);                                   \
             return FN<__nv_bfloat16, 1>(__VA_ARGS__);                                                 \
         }                                                                                             \
         if (vec == 8) return FN<__half, 8>(__VA_ARGS__);                                              \
+        if (vec == 4) return FN<__half, 4>(__VA_ARGS__);                                              \
         if (vec == 2) return FN<__half, 2>(__VA_ARGS__);                                              \
         return FN<__half, 1>(__VA_ARGS__);                                                            \
     } while (0)

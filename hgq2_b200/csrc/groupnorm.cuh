@@ -69,6 +69,67 @@ __device__ __forceinline__ float act_slope(float u) {
         default: { constexpr int ACT = HGQ_ACT_NONE; __VA_ARGS__; break; }           \
     }
 
+// Packs stay in their own type until they are used, as whole words (16-bit halves in registers of their own would double them).
+template <int BYTES> struct Words { using type = uint16_t; };
+template <> struct Words<4> { using type = uint32_t; };
+template <> struct Words<8> { using type = uint2; };
+template <> struct Words<16> { using type = uint4; };
+
+__device__ __forceinline__ void unpack_word(uint32_t w, float &lo, float &hi, const __nv_bfloat16 *) {
+    lo = __uint_as_float(w << 16);
+    hi = __uint_as_float(w & 0xffff0000u);
+}
+__device__ __forceinline__ void unpack_word(uint32_t w, float &lo, float &hi, const __half *) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w));
+    lo = f.x;
+    hi = f.y;
+}
+
+template <typename T, int VEC, int R>
+struct Held {
+    static constexpr int kBytes = (int)sizeof(T) * VEC;
+    using W = typename Words<kBytes>::type;
+    W q[R];
+
+    __device__ __forceinline__ void load(const T *p, int64_t step, unsigned mask) {
+#pragma unroll
+        for (int j = 0; j < R; ++j) {
+            q[j] = W{};
+            if (mask >> j & 1) q[j] = *reinterpret_cast<const W *>(p + j * step);
+        }
+    }
+    // The same a sample ahead: 16-byte packs are copied to this thread's places in shared memory while the sample before is worked
+    // on (its own packs: no barrier), and taken from there.
+    static constexpr bool kAhead = kBytes == 16;
+    static constexpr int kStageBytes = kAhead ? R * kThreads * 16 : 0;
+    static __device__ __forceinline__ void fetch(unsigned char *stage, const T *p, int64_t step, unsigned mask) {
+        uint32_t d = (uint32_t)__cvta_generic_to_shared(stage) + threadIdx.x * 16;
+#pragma unroll
+        for (int j = 0; j < R; ++j, d += kThreads * 16)
+            if (mask >> j & 1) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(d), "l"(p + j * step) : "memory");
+    }
+    static __device__ __forceinline__ void arrived() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+    __device__ __forceinline__ void take(const unsigned char *stage, unsigned mask) {
+#pragma unroll
+        for (int j = 0; j < R; ++j) {
+            q[j] = W{};
+            if (mask >> j & 1) q[j] = reinterpret_cast<const W *>(stage)[j * kThreads + threadIdx.x];
+        }
+    }
+    __device__ __forceinline__ void values(int j, float (&v)[VEC]) const {
+        if constexpr (kBytes == 2) {
+            v[0] = to_float(*reinterpret_cast<const T *>(&q[j]));
+        } else {
+            const uint32_t *w = reinterpret_cast<const uint32_t *>(&q[j]);
+#pragma unroll
+            for (int k = 0; k < kBytes / 4; ++k) {
+                if constexpr (sizeof(T) == 4) v[k] = __uint_as_float(w[k]);
+                else unpack_word(w[k], v[2 * k], v[2 * k + 1], (const T *)nullptr);
+            }
+        }
+    }
+};
+
 // Samples (or slabs of their channels) that fit on chip: how a call is cut up for the one-read kernels.  usable == false: the
 // shape is for the kernels that read twice.
 struct SlabPlan {
@@ -85,6 +146,7 @@ struct SlabPlan {
     int rows;       // of one CTA
     int64_t items;  // ceil(B / subs)
     int64_t workers;
+    bool ahead;     // forward: the next sample is fetched while this one is worked on
 };
 
 SlabPlan gn_slab_plan(int64_t B, int64_t S, int C, int G, int type, int vec, bool backward);

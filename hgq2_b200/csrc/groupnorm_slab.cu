@@ -17,9 +17,9 @@ namespace hgq {
 
 namespace cg = cooperative_groups;
 
-constexpr int kSlabThreads = 256;
+constexpr int kSlabThreads = kThreads;
 constexpr int kSlabWarps = kSlabThreads / 32;
-constexpr int kMaxCluster = 8;
+constexpr int kMaxCluster = 2;  // clusters of 4 and 8 wait for one another longer than a second read from L2 takes
 constexpr int kMaxPairs = 512;  // (sample, group) pairs of a CTA
 
 struct SlabArgs {
@@ -188,51 +188,11 @@ __device__ __forceinline__ void join_channels(const float (&c)[VEC], float (&g)[
     }
 }
 
-// Packs stay in their own type until they are used, as whole words (16-bit halves in registers of their own would double them).
-template <int BYTES> struct Words { using type = uint16_t; };
-template <> struct Words<4> { using type = uint32_t; };
-template <> struct Words<8> { using type = uint2; };
-template <> struct Words<16> { using type = uint4; };
+// CTAs an SM, by the registers that the held packs take.
+constexpr int slab_fwd_ctas(int values, bool ahead) { return ahead ? (values >= 32 ? 2 : 3) : (values >= 64 ? 2 : (values >= 32 ? 3 : 4)); }
 
-__device__ __forceinline__ void unpack_word(uint32_t w, float &lo, float &hi, const __nv_bfloat16 *) {
-    lo = __uint_as_float(w << 16);
-    hi = __uint_as_float(w & 0xffff0000u);
-}
-__device__ __forceinline__ void unpack_word(uint32_t w, float &lo, float &hi, const __half *) {
-    const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w));
-    lo = f.x;
-    hi = f.y;
-}
-
-template <typename T, int VEC, int R>
-struct Held {
-    static constexpr int kBytes = (int)sizeof(T) * VEC;
-    using W = typename Words<kBytes>::type;
-    W q[R];
-
-    __device__ __forceinline__ void load(const T *p, int64_t step, unsigned mask) {
-#pragma unroll
-        for (int j = 0; j < R; ++j) {
-            q[j] = W{};
-            if (mask >> j & 1) q[j] = *reinterpret_cast<const W *>(p + j * step);
-        }
-    }
-    __device__ __forceinline__ void values(int j, float (&v)[VEC]) const {
-        if constexpr (kBytes == 2) {
-            v[0] = to_float(*reinterpret_cast<const T *>(&q[j]));
-        } else {
-            const uint32_t *w = reinterpret_cast<const uint32_t *>(&q[j]);
-#pragma unroll
-            for (int k = 0; k < kBytes / 4; ++k) {
-                if constexpr (sizeof(T) == 4) v[k] = __uint_as_float(w[k]);
-                else unpack_word(w[k], v[2 * k], v[2 * k + 1], (const T *)nullptr);
-            }
-        }
-    }
-};
-
-template <typename T, int VEC, int R, int NG>
-__global__ void __launch_bounds__(kSlabThreads, R * VEC >= 64 ? 2 : (R * VEC >= 32 ? 3 : 4))
+template <typename T, int VEC, int R, int NG, bool AHEAD>
+__global__ void __launch_bounds__(kSlabThreads, slab_fwd_ctas(R * VEC, AHEAD))
     k_gn_slab_fwd(const T *__restrict__ x, const float *__restrict__ gamma, const float *__restrict__ beta, const SlabArgs a, float eps, int act,
                   T *__restrict__ y, float *__restrict__ mean_out, float *__restrict__ rstd_out) {
     constexpr int W = VEC / NG;  // channels of a pack in one group
@@ -261,12 +221,22 @@ __global__ void __launch_bounds__(kSlabThreads, R * VEC >= 64 ? 2 : (R * VEC >= 
 #pragma unroll
     for (int j = 0; j < R; ++j)
         if (row + j * a.TYs < end) rows_mask |= 1u << j;
+    using H = Held<T, VEC, R>;
+    extern __shared__ __align__(16) unsigned char stage[];
+    auto mask_of = [&](int64_t item) { return p.in && item < a.items && item * a.subs + p.sub < a.B ? rows_mask : 0u; };
+    auto base_of = [&](int64_t item) { return ((item * a.subs + p.sub) * a.S + row) * a.C + c0; };
+    if (AHEAD) H::fetch(stage, x + base_of(p.worker), step, mask_of(p.worker));
     for (int64_t item = p.worker; item < a.items; item += a.workers) {
         const int64_t b = item * a.subs + p.sub;
-        const unsigned mask = p.in && b < a.B ? rows_mask : 0;
-        const int64_t base = (b * a.S + row) * a.C + c0;
-        Held<T, VEC, R> h;
-        h.load(x + base, step, mask);
+        const unsigned mask = mask_of(item);
+        const int64_t base = base_of(item);
+        H h;
+        if (AHEAD) {
+            H::arrived();
+            h.take(stage, mask);
+        } else {
+            h.load(x + base, step, mask);
+        }
         float s[VEC], mu[1][NG], rs[1][NG];
 #pragma unroll
         for (int i = 0; i < VEC; ++i) s[i] = 0.f;
@@ -278,6 +248,8 @@ __global__ void __launch_bounds__(kSlabThreads, R * VEC >= 64 ? 2 : (R * VEC >= 
             for (int i = 0; i < VEC; ++i) s[i] += v[i];
         }
         join_channels<VEC, NG>(s, mu[0]);
+        // every value has been used by now: the places are free for the next sample
+        if (AHEAD) H::fetch(stage, x + base_of(item + a.workers), step, mask_of(item + a.workers));
         group_totals<NG, 1>(mu, sh, 0, pair_of, a, p);
 #pragma unroll
         for (int i = 0; i < NG; ++i) mu[0][i] *= inv_n;
@@ -433,6 +405,7 @@ __global__ void __launch_bounds__(kSlabThreads, 2)
 // Packs a thread holds: enough of them that a CTA has 16 to 32 KB of a tensor in flight.
 static int slab_most(int type, int vec, bool backward) {
     const int size = type == HGQ_TYPE_F32 ? 4 : 2;
+    if (vec * size == 8 && vec == 4) return 8;
     if (vec * size < 16) return 16;  // narrow packs: many of them
     return backward && type != HGQ_TYPE_F32 ? 4 : 8;
 }
@@ -486,8 +459,8 @@ SlabPlan gn_slab_plan(int64_t B, int64_t S, int C, int G, int type, int vec, boo
     p.items = (B + p.subs - 1) / p.subs;
     if (p.items * p.slabs * p.K > INT32_MAX) return p;
     // resident CTAs, by their registers: what a CTA sets up once (places, scale and offset) is spread over its samples
-    const int held = p.R * vec;
-    int64_t n = (int64_t)num_sms() * (backward || held >= 64 ? 2 : (held >= 32 ? 3 : 4)) / ((int64_t)p.K * p.slabs);
+    p.ahead = !backward && p.K == 1 && vec * size == 16;
+    int64_t n = (int64_t)num_sms() * (backward ? 2 : slab_fwd_ctas(p.R * vec, p.ahead)) / ((int64_t)p.K * p.slabs);
     if (n < 1) n = 1;
     p.workers = p.items < n ? p.items : n;
     p.usable = true;
@@ -516,10 +489,18 @@ static SlabArgs slab_args(const SlabPlan &p, int64_t B, int64_t S, int C, int G)
 }
 
 template <typename... Params, typename... Args>
-static int launch_clusters(void (*kernel)(Params...), int64_t ctas, int K, cudaStream_t st, Args... args) {
+static int launch_clusters(void (*kernel)(Params...), int64_t ctas, int K, size_t smem, cudaStream_t st, Args... args) {
+    if (smem > 0) {  // beside up to 36 KB of static shared memory
+        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+        if (e != cudaSuccess) {
+            cudaGetLastError();
+            return (int)e;
+        }
+    }
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((unsigned)ctas);
     cfg.blockDim = dim3(kSlabThreads);
+    cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -539,11 +520,15 @@ template <typename T, int VEC, int R>
 static int slab_fwd(const SlabPlan &p, const SlabArgs &a, const void *x, const float *gamma, const float *beta, void *y, float *mean, float *rstd,
                     float eps, int act, cudaStream_t st) {
     const int64_t ctas = p.workers * p.slabs * p.K;
-    auto kernel = k_gn_slab_fwd<T, VEC, R, 1>;
-    if (VEC > 1 && p.groups_of_pack == 2) kernel = k_gn_slab_fwd<T, VEC, R, (VEC > 1 ? 2 : 1)>;
-    if (VEC > 4 && p.groups_of_pack == 4) kernel = k_gn_slab_fwd<T, VEC, R, (VEC > 4 ? 4 : VEC)>;
-    if (VEC > 2 && p.groups_of_pack == VEC) kernel = k_gn_slab_fwd<T, VEC, R, VEC>;
-    return launch_clusters(kernel, ctas, p.K, st, (const T *)x, gamma, beta, a, eps, act, (T *)y, mean, rstd);
+    constexpr bool can = Held<T, VEC, R>::kAhead;
+    const size_t smem = p.ahead ? Held<T, VEC, R>::kStageBytes : 0;
+#define SLAB_FWD(NG) (p.ahead ? k_gn_slab_fwd<T, VEC, R, NG, can> : k_gn_slab_fwd<T, VEC, R, NG, false>)
+    auto kernel = SLAB_FWD(1);
+    if (VEC > 1 && p.groups_of_pack == 2) kernel = SLAB_FWD((VEC > 1 ? 2 : 1));
+    if (VEC > 4 && p.groups_of_pack == 4) kernel = SLAB_FWD((VEC > 4 ? 4 : VEC));
+    if (VEC > 2 && p.groups_of_pack == VEC) kernel = SLAB_FWD(VEC);
+#undef SLAB_FWD
+    return launch_clusters(kernel, ctas, p.K, smem, st, (const T *)x, gamma, beta, a, eps, act, (T *)y, mean, rstd);
 }
 
 template <typename T, int VEC, int R>
@@ -554,7 +539,7 @@ static int slab_bwd(const SlabPlan &p, const SlabArgs &a, const void *gy, const 
     if (VEC > 1 && p.groups_of_pack == 2) kernel = k_gn_slab_bwd<T, VEC, R, (VEC > 1 ? 2 : 1)>;
     if (VEC > 4 && p.groups_of_pack == 4) kernel = k_gn_slab_bwd<T, VEC, R, (VEC > 4 ? 4 : VEC)>;
     if (VEC > 2 && p.groups_of_pack == VEC) kernel = k_gn_slab_bwd<T, VEC, R, VEC>;
-    return launch_clusters(kernel, ctas, p.K, st, (const T *)gy, (const T *)x, gamma, beta, mean, rstd, a, act, (T *)dx, part);
+    return launch_clusters(kernel, ctas, p.K, 0, st, (const T *)gy, (const T *)x, gamma, beta, mean, rstd, a, act, (T *)dx, part);
 }
 
 #define SLAB_DISPATCH(FN, FULL_MOST, ...)                                              \
@@ -577,6 +562,9 @@ static int slab_bwd(const SlabPlan &p, const SlabArgs &a, const void *gy, const 
         if (p.vec == 8 && p.R == 1) return FN<T, 8, 1>(__VA_ARGS__);     \
         if (p.vec == 8 && p.R == 4) return FN<T, 8, 4>(__VA_ARGS__);     \
         if (p.vec == 8) return FN<T, 8, FULL_MOST>(__VA_ARGS__);         \
+        if (p.vec == 4 && p.R == 1) return FN<T, 4, 1>(__VA_ARGS__);     \
+        if (p.vec == 4 && p.R == 4) return FN<T, 4, 4>(__VA_ARGS__);     \
+        if (p.vec == 4) return FN<T, 4, 8>(__VA_ARGS__);                 \
         if (p.vec == 2 && p.R == 1) return FN<T, 2, 1>(__VA_ARGS__);     \
         if (p.vec == 2) return FN<T, 2, 16>(__VA_ARGS__);                \
         if (p.R == 1) return FN<T, 1, 1>(__VA_ARGS__);                   \
