@@ -20,6 +20,10 @@ namespace hgq {
 // ---- any shape: partial statistics, totals, application ---------------------------------------------------------------------
 // A CTA takes a run of rows of one sample and a tile of channels; a thread owns VEC neighbouring channels for all of its rows.
 
+// Rows in flight at once, by the registers that a pack and its sums take.
+constexpr int kGnRows = 8, kGnApplyRows = 4, kGnBwdRows = 4;
+constexpr int kGnFwdCtas = 3, kGnBwdCtas = 2;  // CTAs an SM
+
 struct GnGeom {
     int64_t S, rows_per_chunk;
     int C, G, Cg, TX, TY, tiles, chunks;
@@ -36,9 +40,6 @@ __device__ __forceinline__ bool gn_place(const GnGeom &g, int64_t blk, int &b_re
     c0 = (tile * g.TX + tx) * VEC;
     return ty < g.TY && c0 < g.C;
 }
-
-// Rows in flight at once, by the registers that a pack and its sums take.
-constexpr int kGnRows = 8, kGnApplyRows = 4, kGnBwdRows = 4;
 
 // Which of the rows r, r + TY, ... are before `end`.
 template <int ROWS>
@@ -69,7 +70,7 @@ __device__ __forceinline__ void sum_over_ty(float (&v)[N], float *sh, const GnGe
 // a large mean costs no digits as long as rows of one channel lie within a few spreads of one another; the totals' step is exact
 // about the rest.
 template <typename T, int VEC>
-__global__ void __launch_bounds__(kThreads) k_gn_stats(const T *__restrict__ x, const GnGeom g, int64_t b_base, float *__restrict__ part) {
+__global__ void __launch_bounds__(kThreads, kGnFwdCtas) k_gn_stats(const T *__restrict__ x, const GnGeom g, int64_t b_base, float *__restrict__ part) {
     __shared__ float sh[kThreads * 2 * VEC];
     int b, chunk, c0, tx, ty;
     const bool active = gn_place<VEC>(g, blockIdx.x, b, chunk, c0, tx, ty);
@@ -163,7 +164,7 @@ __global__ void __launch_bounds__(kThreads) k_gn_totals(const float *__restrict_
 }
 
 template <typename T, int VEC>
-__global__ void __launch_bounds__(kThreads) k_gn_apply(const T *__restrict__ x, const float *__restrict__ gamma, const float *__restrict__ beta,
+__global__ void __launch_bounds__(kThreads, kGnFwdCtas) k_gn_apply(const T *__restrict__ x, const float *__restrict__ gamma, const float *__restrict__ beta,
                                                        const float *__restrict__ mean, const float *__restrict__ rstd, const GnGeom g,
                                                        int64_t b_base, int act, T *__restrict__ y) {
     int b, chunk, c0, tx, ty;
@@ -195,7 +196,7 @@ __global__ void __launch_bounds__(kThreads) k_gn_apply(const T *__restrict__ x, 
 
 // Per (sample, chunk, channel): sum of du and of du xhat.
 template <typename T, int VEC>
-__global__ void __launch_bounds__(kThreads) k_gn_bwd_stats(const T *__restrict__ gy, const T *__restrict__ x, const float *__restrict__ gamma,
+__global__ void __launch_bounds__(kThreads, kGnBwdCtas) k_gn_bwd_stats(const T *__restrict__ gy, const T *__restrict__ x, const float *__restrict__ gamma,
                                                            const float *__restrict__ beta, const float *__restrict__ mean,
                                                            const float *__restrict__ rstd, const GnGeom g, int64_t b_base, int act,
                                                            float *__restrict__ part) {
@@ -275,7 +276,7 @@ __global__ void __launch_bounds__(kThreads) k_gn_bwd_totals(const float *__restr
 }
 
 template <typename T, int VEC>
-__global__ void __launch_bounds__(kThreads) k_gn_bwd_apply(const T *__restrict__ gy, const T *__restrict__ x, const float *__restrict__ gamma,
+__global__ void __launch_bounds__(kThreads, kGnBwdCtas) k_gn_bwd_apply(const T *__restrict__ gy, const T *__restrict__ x, const float *__restrict__ gamma,
                                                            const float *__restrict__ beta, const float *__restrict__ mean,
                                                            const float *__restrict__ rstd, const float *__restrict__ m1,
                                                            const float *__restrict__ m2, const GnGeom g, int64_t b_base, int act,
@@ -350,15 +351,15 @@ static int64_t gn_group(int64_t B, int64_t S, int C, int64_t bytes_per_value) {
     return groups > 0 ? (B + groups - 1) / groups : 1;
 }
 
-static GnGeom gn_geom(int64_t group, int64_t S, int C, int G, int vec) {
+// ctas_per_sm: how many of the call's CTAs an SM holds (their registers): one wave of them, so that no few stragglers follow it.
+static GnGeom gn_geom(int64_t group, int64_t S, int C, int G, int vec, int ctas_per_sm) {
     GnGeom g;
     g.S = S, g.C = C, g.G = G, g.Cg = C / G;
     const int cv = C / vec;
     g.tiles = (cv + kThreads - 1) / kThreads;
     g.TX = (cv + g.tiles - 1) / g.tiles;
     g.TY = kThreads / g.TX;
-    const int64_t target = (int64_t)num_sms() * 4;
-    int64_t chunks = (target + group * g.tiles - 1) / (group * g.tiles);
+    int64_t chunks = (int64_t)num_sms() * ctas_per_sm / (group * g.tiles);
     const int64_t most = (S + (int64_t)g.TY * 4 - 1) / ((int64_t)g.TY * 4);
     if (chunks > most) chunks = most;
     if (chunks < 1) chunks = 1;
@@ -383,7 +384,7 @@ static size_t gn_part_floats(int64_t B, int64_t S, int C, int G, int type, bool 
     size_t most = 0;
     for (int v : {16 / size, 4, 2, 1}) {
         if (C % v != 0) continue;
-        const GnGeom g = gn_geom(group, S, C, G, v);
+        const GnGeom g = gn_geom(group, S, C, G, v, bwd ? kGnBwdCtas : kGnFwdCtas);
         const size_t any = (size_t)g.chunks * 2 * C * (size_t)(bwd ? B : group);
         most = any > most ? any : most;
         const SlabPlan p = gn_slab_plan(B, S, C, G, type, v, bwd);
@@ -405,7 +406,7 @@ template <typename T, int VEC>
 static int gn_fwd_any(const void *x, const float *gamma, const float *beta, void *y, float *mean, float *rstd, int64_t B, int64_t S, int C,
                       int G, float eps, int act, float *part, cudaStream_t st) {
     const int64_t group = gn_group(B, S, C, sizeof(T));
-    const GnGeom g = gn_geom(group, S, C, G, VEC);
+    const GnGeom g = gn_geom(group, S, C, G, VEC, kGnFwdCtas);
     for (int64_t b0 = 0; b0 < B; b0 += group) {
         const int64_t nb = B - b0 < group ? B - b0 : group, pairs = nb * G;
         const int64_t ctas = nb * g.chunks * g.tiles;
@@ -442,7 +443,7 @@ static int gn_bwd_any(const void *gy, const void *x, const float *gamma, const f
                       float *dgamma, float *dbeta, int64_t B, int64_t S, int C, int G, int act, float *part, float *m, float *scratch,
                       cudaStream_t st) {
     const int64_t group = gn_group(B, S, C, 2 * sizeof(T));
-    const GnGeom g = gn_geom(group, S, C, G, VEC);
+    const GnGeom g = gn_geom(group, S, C, G, VEC, kGnBwdCtas);
     for (int64_t b0 = 0; b0 < B; b0 += group) {
         const int64_t nb = B - b0 < group ? B - b0 : group, pairs = nb * G;
         const int64_t ctas = nb * g.chunks * g.tiles;
