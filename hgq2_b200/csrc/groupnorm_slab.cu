@@ -402,18 +402,23 @@ __global__ void __launch_bounds__(kSlabThreads, 2)
 
 // ---- host ---------------------------------------------------------------------------------------------------------------------
 
-// Packs a thread holds: enough of them that a CTA has 16 to 32 KB of a tensor in flight.
-static int slab_most(int type, int vec, bool backward) {
-    const int size = type == HGQ_TYPE_F32 ? 4 : 2;
-    if (vec * size == 8 && vec == 4) return 8;
-    if (vec * size < 16) return 16;  // narrow packs: many of them
-    return backward && type != HGQ_TYPE_F32 ? 4 : 8;
+// Packs of one tensor that a thread holds: usually (what leaves two or three CTAs an SM), and at most, where that saves a cluster.
+static void slab_held(int type, int vec, bool backward, int &usual, int &most) {
+    const bool half = type != HGQ_TYPE_F32;
+    const int bytes = vec * (half ? 2 : 4);
+    if (bytes == 16) {
+        usual = backward && half ? 4 : 8;
+        most = backward || half ? usual : 16;
+    } else {
+        usual = most = half && vec == 4 ? 8 : 16;  // narrow packs: many of them
+    }
 }
 
 SlabPlan gn_slab_plan(int64_t B, int64_t S, int C, int G, int type, int vec, bool backward) {
     SlabPlan p{};
     const int Cg = C / G, size = type == HGQ_TYPE_F32 ? 4 : 2;
-    const int most = slab_most(type, vec, backward);
+    int usual, most;
+    slab_held(type, vec, backward, usual, most);
     p.vec = vec;
     p.groups_of_pack = Cg % vec == 0 ? 1 : (vec % Cg == 0 ? vec / Cg : vec);
     // whole groups whose channels are whole packs
@@ -441,9 +446,9 @@ SlabPlan gn_slab_plan(int64_t B, int64_t S, int C, int G, int type, int vec, boo
     p.subs = 1;
     p.K = 1;
     p.TYs = p.TY;
-    if (S <= (int64_t)p.TY * most) {
+    if (S <= (int64_t)p.TY * usual) {
         int rows = 1;
-        while ((int64_t)rows * most < S) rows <<= 1;
+        while ((int64_t)rows * usual < S) rows <<= 1;
         while (rows < p.TY && (B * rows < (int64_t)num_sms() * 2 * p.TY || p.TY / rows > kMaxPairs / p.Gs)) rows <<= 1;
         if (2 * rows <= p.TY) {
             p.TYs = rows;
@@ -455,7 +460,8 @@ SlabPlan gn_slab_plan(int64_t B, int64_t S, int C, int G, int type, int vec, boo
     while (packs > (int64_t)most * p.K) p.K <<= 1;
     p.rows = (int)((S + p.K - 1) / p.K);
     const int need = (p.rows + p.TYs - 1) / p.TYs;
-    p.R = need <= 1 ? 1 : (need <= 4 && most != 16 ? 4 : most);
+    if (vec * size >= 8 && vec >= 4) p.R = need <= 1 ? 1 : (need <= 4 ? 4 : (need <= 8 ? 8 : 16));
+    else p.R = need <= 1 ? 1 : 16;
     p.items = (B + p.subs - 1) / p.subs;
     if (p.items * p.slabs * p.K > INT32_MAX) return p;
     // resident CTAs, by their registers: what a CTA sets up once (places, scale and offset) is spread over its samples
@@ -542,26 +548,27 @@ static int slab_bwd(const SlabPlan &p, const SlabArgs &a, const void *gy, const 
     return launch_clusters(kernel, ctas, p.K, 0, st, (const T *)gy, (const T *)x, gamma, beta, mean, rstd, a, act, (T *)dx, part);
 }
 
-#define SLAB_DISPATCH(FN, FULL_MOST, ...)                                              \
+#define SLAB_DISPATCH(FN, MOST, HALF_MOST, ...)                                              \
     do {                                                                               \
         if (type == HGQ_TYPE_F32) {                                                    \
             if (p.vec == 4 && p.R == 1) return FN<float, 4, 1>(__VA_ARGS__);           \
             if (p.vec == 4 && p.R == 4) return FN<float, 4, 4>(__VA_ARGS__);           \
-            if (p.vec == 4) return FN<float, 4, 8>(__VA_ARGS__);                       \
+            if (p.vec == 4 && p.R == 8) return FN<float, 4, 8>(__VA_ARGS__);           \
+            if (p.vec == 4) return FN<float, 4, MOST>(__VA_ARGS__);                    \
             if (p.vec == 2 && p.R == 1) return FN<float, 2, 1>(__VA_ARGS__);           \
             if (p.vec == 2) return FN<float, 2, 16>(__VA_ARGS__);                      \
             if (p.R == 1) return FN<float, 1, 1>(__VA_ARGS__);                         \
             return FN<float, 1, 16>(__VA_ARGS__);                                      \
         }                                                                              \
-        if (type == HGQ_TYPE_BF16) SLAB_HALF(FN, FULL_MOST, __nv_bfloat16, __VA_ARGS__); \
-        SLAB_HALF(FN, FULL_MOST, __half, __VA_ARGS__);                                 \
+        if (type == HGQ_TYPE_BF16) SLAB_HALF(FN, HALF_MOST, __nv_bfloat16, __VA_ARGS__); \
+        SLAB_HALF(FN, HALF_MOST, __half, __VA_ARGS__);                                 \
     } while (0)
 
-#define SLAB_HALF(FN, FULL_MOST, T, ...)                                 \
+#define SLAB_HALF(FN, HALF_MOST, T, ...)                                 \
     do {                                                                 \
         if (p.vec == 8 && p.R == 1) return FN<T, 8, 1>(__VA_ARGS__);     \
         if (p.vec == 8 && p.R == 4) return FN<T, 8, 4>(__VA_ARGS__);     \
-        if (p.vec == 8) return FN<T, 8, FULL_MOST>(__VA_ARGS__);         \
+        if (p.vec == 8) return FN<T, 8, HALF_MOST>(__VA_ARGS__);         \
         if (p.vec == 4 && p.R == 1) return FN<T, 4, 1>(__VA_ARGS__);     \
         if (p.vec == 4 && p.R == 4) return FN<T, 4, 4>(__VA_ARGS__);     \
         if (p.vec == 4) return FN<T, 4, 8>(__VA_ARGS__);                 \
@@ -574,13 +581,13 @@ static int slab_bwd(const SlabPlan &p, const SlabArgs &a, const void *gy, const 
 int gn_slab_fwd(const SlabPlan &p, const void *x, const float *gamma, const float *beta, void *y, float *mean, float *rstd, int64_t B,
                 int64_t S, int C, int G, float eps, int act, int type, cudaStream_t st) {
     const SlabArgs a = slab_args(p, B, S, C, G);
-    SLAB_DISPATCH(slab_fwd, 8, p, a, x, gamma, beta, y, mean, rstd, eps, act, st);
+    SLAB_DISPATCH(slab_fwd, 16, 8, p, a, x, gamma, beta, y, mean, rstd, eps, act, st);
 }
 
 int gn_slab_bwd(const SlabPlan &p, const void *gy, const void *x, const float *gamma, const float *beta, const float *mean,
                 const float *rstd, void *dx, float *part, int64_t B, int64_t S, int C, int G, int act, int type, cudaStream_t st) {
     const SlabArgs a = slab_args(p, B, S, C, G);
-    SLAB_DISPATCH(slab_bwd, 4, p, a, gy, x, gamma, beta, mean, rstd, act, dx, part, st);
+    SLAB_DISPATCH(slab_bwd, 8, 4, p, a, gy, x, gamma, beta, mean, rstd, act, dx, part, st);
 }
 
 }  // namespace hgq
