@@ -23,6 +23,7 @@ FLAG_TRAINING = 1
 FLAG_ZERO_NONPOS = 2
 FLAG_ABSMAX_ACCUMULATE = 4
 ADAMW_BLOCK = 256  # HGQ_ADAMW_BLOCK
+ADAMW_CHUNK = 2048  # HGQ_ADAMW_CHUNK
 
 
 class HGQError(RuntimeError):
@@ -253,9 +254,10 @@ def ptr(t) -> int | None:
 
 
 def stream_handle() -> int:
+    """Handle of the current device's current stream (without the Stream object that torch.cuda.current_stream() builds)."""
     import torch
 
-    return torch.cuda.current_stream().cuda_stream
+    return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
 
 
 def require_cuda(*tensors) -> None:

@@ -14,9 +14,9 @@
 // Every product and sum that leads to a code is written as a single IEEE operation (no contraction), so the codes are a
 // function of the inputs alone and not of how the compiler schedules the expression.
 //
-// A block is a warp's unit of work (8 elements a lane): per-block maxima are warp reductions and nothing is shared between
-// warps.  The (tensor, block) table is built once by the caller; gradient addresses, which change from step to step, travel in
-// the kernel's parameters, so a step copies nothing to the device and a captured graph keeps its own.
+// A CTA takes 8 neighbouring blocks of a tensor (a chunk) at a time, a block a warp (8 elements a lane): maxima are warp reductions and
+// nothing is shared between warps.  The (tensor, chunk) table is built once by the caller; gradient addresses, which change from step
+// to step, travel in the kernel's parameters, so a step copies nothing to the device and a captured graph keeps its own.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
@@ -27,9 +27,10 @@
 namespace hgq {
 
 constexpr int kAdamBlock = HGQ_ADAMW_BLOCK;
-constexpr int kAdamWarps = 8;
+constexpr int kAdamWarps = HGQ_ADAMW_CHUNK / HGQ_ADAMW_BLOCK;
 constexpr int kAdamMaxTensors = 512;  // gradient addresses in one launch's parameters (4.6 KB)
-constexpr int kNormCtasPerSm = 4;
+constexpr int kNormCtasPerSm = 8;
+constexpr int kAdamCtas32 = 3, kAdamCtas8 = 3;  // CTAs an SM, by registers
 
 struct GradTable {
     const void *p[kAdamMaxTensors];
@@ -41,39 +42,68 @@ struct AdamScalars {
     float f_b1, f_1mb1, f_b2, f_1mb2, eps, grad_scale;
 };
 
+// Element j of a lane: VEC, 8 neighbours a lane (whole sectors of memory); otherwise every 32nd.
 template <bool VEC>
 __device__ __forceinline__ int elem_of(int j, int lane) {
-    return VEC ? (j >> 2) * 128 + lane * 4 + (j & 3) : j * 32 + lane;
+    return VEC ? lane * 8 + j : j * 32 + lane;
 }
 
-// 8 values of a lane from an array of `type` at p (already at the block's first element); elements >= count read as 0.
+__device__ __forceinline__ void unpack8(const uint4 q, int type, float (&v)[8]) {
+    const uint32_t u[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        if (type == HGQ_TYPE_BF16) {
+            v[2 * k] = __uint_as_float(u[k] << 16);
+            v[2 * k + 1] = __uint_as_float(u[k] & 0xffff0000u);
+        } else {
+            const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&u[k]));
+            v[2 * k] = f.x;
+            v[2 * k + 1] = f.y;
+        }
+    }
+}
+__device__ __forceinline__ void quad(const float4 q, float *v) { v[0] = q.x, v[1] = q.y, v[2] = q.z, v[3] = q.w; }
+
+// e4m3 codes: 8 of a lane.  Decoding is exact (every e4m3 value is an fp16 value).
+__device__ __forceinline__ void decode8(const uint2 q, float (&v)[8]) {
+    const uint32_t u[2] = {q.x, q.y};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        const __half2_raw r = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(u[k >> 1] >> (16 * (k & 1))), __NV_E4M3);
+        const float2 f = __half22float2(__half2(r));
+        v[2 * k] = f.x;
+        v[2 * k + 1] = f.y;
+    }
+}
+// The values are on the e4m3 grid already (or NaN), so the conversion rounds nothing.
+__device__ __forceinline__ uint2 encode8(const float (&v)[8]) {
+    uint32_t u[2] = {0, 0};
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+        u[k >> 1] |= (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(v[2 * k], v[2 * k + 1]), __NV_SATFINITE, __NV_E4M3) << (16 * (k & 1));
+    return make_uint2(u[0], u[1]);
+}
+
+// 8 values of a lane from an array of `type` at p (already at the block's first element); elements >= count read as 0.  VEC: p is
+// aligned to 4 elements, WIDE to 8 fp32.
 template <bool VEC>
-__device__ __forceinline__ void load_any(const void *p, int type, int lane, int count, float (&v)[8]) {
+__device__ __forceinline__ void load_any(const void *p, int type, int lane, int count, bool wide, float (&v)[8]) {
     if (VEC) {
         if (type == HGQ_TYPE_F32) {
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const float4 q = __ldcs(reinterpret_cast<const float4 *>(p) + h * 32 + lane);
-                v[4 * h] = q.x, v[4 * h + 1] = q.y, v[4 * h + 2] = q.z, v[4 * h + 3] = q.w;
+            const float *f = reinterpret_cast<const float *>(p) + lane * 8;
+            if (wide) {
+                asm volatile("ld.global.v8.f32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                             : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7])
+                             : "l"(f)
+                             : "memory");
+            } else {
+                quad(reinterpret_cast<const float4 *>(f)[0], v);
+                quad(reinterpret_cast<const float4 *>(f)[1], v + 4);
             }
         } else {
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const uint2 q = __ldcs(reinterpret_cast<const uint2 *>(p) + h * 32 + lane);
-                const uint32_t u[2] = {q.x, q.y};
-#pragma unroll
-                for (int k = 0; k < 2; ++k) {
-                    float2 f;
-                    if (type == HGQ_TYPE_BF16) {
-                        f.x = __uint_as_float(u[k] << 16);
-                        f.y = __uint_as_float(u[k] & 0xffff0000u);
-                    } else {
-                        f = __half22float2(*reinterpret_cast<const __half2 *>(&u[k]));
-                    }
-                    v[4 * h + 2 * k] = f.x;
-                    v[4 * h + 2 * k + 1] = f.y;
-                }
-            }
+            const uint2 *h = reinterpret_cast<const uint2 *>(p) + lane * 2;
+            const uint2 a = h[0], b = h[1];
+            unpack8(make_uint4(a.x, a.y, b.x, b.y), type, v);
         }
     } else {
 #pragma unroll
@@ -90,28 +120,31 @@ __device__ __forceinline__ void load_any(const void *p, int type, int lane, int 
 }
 
 template <bool VEC>
-__device__ __forceinline__ void store_any(void *p, int type, int lane, int count, const float (&v)[8]) {
+__device__ __forceinline__ void store_any(void *p, int type, int lane, int count, bool wide, const float (&v)[8]) {
     if (VEC) {
         if (type == HGQ_TYPE_F32) {
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
-                __stcs(reinterpret_cast<float4 *>(p) + h * 32 + lane, make_float4(v[4 * h], v[4 * h + 1], v[4 * h + 2], v[4 * h + 3]));
-        } else {
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                uint32_t u[2];
-#pragma unroll
-                for (int k = 0; k < 2; ++k) {
-                    if (type == HGQ_TYPE_BF16) {
-                        const __nv_bfloat162 q = __floats2bfloat162_rn(v[4 * h + 2 * k], v[4 * h + 2 * k + 1]);
-                        u[k] = *reinterpret_cast<const uint32_t *>(&q);
-                    } else {
-                        const __half2 q = __floats2half2_rn(v[4 * h + 2 * k], v[4 * h + 2 * k + 1]);
-                        u[k] = *reinterpret_cast<const uint32_t *>(&q);
-                    }
-                }
-                __stcs(reinterpret_cast<uint2 *>(p) + h * 32 + lane, make_uint2(u[0], u[1]));
+            float *f = reinterpret_cast<float *>(p) + lane * 8;
+            if (wide) {
+                stcs8(f, v);
+            } else {
+                reinterpret_cast<float4 *>(f)[0] = make_float4(v[0], v[1], v[2], v[3]);
+                reinterpret_cast<float4 *>(f)[1] = make_float4(v[4], v[5], v[6], v[7]);
             }
+        } else {
+            uint32_t u[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                if (type == HGQ_TYPE_BF16) {
+                    const __nv_bfloat162 q = __floats2bfloat162_rn(v[2 * k], v[2 * k + 1]);
+                    u[k] = *reinterpret_cast<const uint32_t *>(&q);
+                } else {
+                    const __half2 q = __floats2half2_rn(v[2 * k], v[2 * k + 1]);
+                    u[k] = *reinterpret_cast<const uint32_t *>(&q);
+                }
+            }
+            uint2 *h = reinterpret_cast<uint2 *>(p) + lane * 2;
+            h[0] = make_uint2(u[0], u[1]);
+            h[1] = make_uint2(u[2], u[3]);
         }
     } else {
 #pragma unroll
@@ -126,21 +159,10 @@ __device__ __forceinline__ void store_any(void *p, int type, int lane, int count
     }
 }
 
-// e4m3 codes: 8 of a lane.  Decoding is exact (every e4m3 value is an fp16 value).
 template <bool VEC>
 __device__ __forceinline__ void load_codes(const uint8_t *p, int lane, int count, float (&v)[8]) {
     if (VEC) {
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const uint32_t q = __ldcs(reinterpret_cast<const uint32_t *>(p) + h * 32 + lane);
-#pragma unroll
-            for (int k = 0; k < 2; ++k) {
-                const __half2_raw r = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(q >> (16 * k)), __NV_E4M3);
-                const float2 f = __half22float2(__half2(r));
-                v[4 * h + 2 * k] = f.x;
-                v[4 * h + 2 * k + 1] = f.y;
-            }
-        }
+        decode8(reinterpret_cast<const uint2 *>(p)[lane], v);
     } else {
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
@@ -151,19 +173,10 @@ __device__ __forceinline__ void load_codes(const uint8_t *p, int lane, int count
     }
 }
 
-// The values are on the e4m3 grid already (or NaN), so the conversion rounds nothing.
 template <bool VEC>
 __device__ __forceinline__ void store_codes(uint8_t *p, int lane, int count, const float (&v)[8]) {
     if (VEC) {
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            uint32_t q = 0;
-#pragma unroll
-            for (int k = 0; k < 2; ++k)
-                q |= (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(v[4 * h + 2 * k], v[4 * h + 2 * k + 1]), __NV_SATFINITE, __NV_E4M3)
-                     << (16 * k);
-            __stcs(reinterpret_cast<uint32_t *>(p) + h * 32 + lane, q);
-        }
+        __stcs(reinterpret_cast<uint2 *>(p) + lane, encode8(v));
     } else {
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
@@ -185,10 +198,11 @@ __device__ __forceinline__ uint32_t dither_bits(uint32_t place, uint32_t step) {
 }
 
 // u in [0, 256] to the e4m3 grid (3 mantissa bits above 2^-6, steps of 2^-9 below), up with probability (distance below) / step.
+template <bool LOW>  // LOW: u may lie below 2^-6
 __device__ __forceinline__ float dithered_e4m3(float u, uint32_t d16) {
-    const bool low = u < 0x1p-6f;
+    const bool low = LOW && u < 0x1p-6f;
     float y = low ? __fadd_rn(u, 0x1p-6f) : u;
-    y = __uint_as_float((__float_as_uint(y) + (d16 << 4)) & 0xfff00000u);
+    y = __uint_as_float((__float_as_uint(y) + d16 * 16u) & 0xfff00000u);
     return low ? __fsub_rn(y, 0x1p-6f) : y;
 }
 
@@ -204,24 +218,36 @@ __device__ __forceinline__ float warp_max(float v) {  // of non-negative numbers
 // The scaled gradient as the moments see it, before clipping.
 __device__ __forceinline__ float scaled_grad(float g, float grad_scale, float l1) { return __fadd_rn(__fmul_rn(g, grad_scale), l1); }
 
+// The tensor that a CTA is at.  It is the same for all of its threads, and found from the CTA's number alone: branches on it are
+// uniform to the compiler too.
+struct Current {
+    hgq_adamw_tensor t;
+    const char *g;
+    int gtype, index;
+    float kept;     // 1 - lr decay
+    bool clamps;    // has a constraint
+    bool scales;    // gradient scale, regulariser or clipping
+    bool aligned;   // addresses that 4 elements at a time can be read from
+    bool wide_g, wide_w;  // 8 fp32 at a time
+};
+
+// VEC: the whole block of 256; otherwise element by element.
 template <int BITS, bool VEC>
-__device__ __forceinline__ void adamw_block(const hgq_adamw_tensor &T, const void *gp, int gtype, int64_t base, int count, int lane,
-                                            void *m_, void *v_, float *m_scale, float *v_scale, const AdamScalars &a, float alpha,
-                                            float coef, uint32_t step) {
-    const int gsize = gtype == HGQ_TYPE_F32 ? 4 : 2;
-    const int wsize = T.w_type == HGQ_TYPE_F32 ? 4 : 2;
-    const int64_t so = T.offset + base;
-    float *const wm = T.master != nullptr ? T.master + base : reinterpret_cast<float *>(T.w) + base;
+__device__ __forceinline__ void adamw_block(const Current &T, int64_t base, int count, int lane, void *m_, void *v_,
+                                            float *m_scale, float *v_scale, const AdamScalars &a, float alpha, float coef, uint32_t step) {
+    const int gsize = T.gtype == HGQ_TYPE_F32 ? 4 : 2;
+    const int64_t so = T.t.offset + base;
+    float *const wm = (T.t.master != nullptr ? T.t.master : reinterpret_cast<float *>(T.t.w)) + base;
     float g[8], w[8], m[8], v[8];
-    load_any<VEC>(reinterpret_cast<const char *>(gp) + base * gsize, gtype, lane, count, g);
-    load_any<VEC>(wm, HGQ_TYPE_F32, lane, count, w);
+    load_any<VEC>(T.g + base * gsize, T.gtype, lane, count, T.wide_g, g);
+    load_any<VEC>(wm, HGQ_TYPE_F32, lane, count, T.wide_w, w);
     if (BITS == 32) {
-        load_any<VEC>(reinterpret_cast<float *>(m_) + so, HGQ_TYPE_F32, lane, count, m);
-        load_any<VEC>(reinterpret_cast<float *>(v_) + so, HGQ_TYPE_F32, lane, count, v);
+        load_any<VEC>(reinterpret_cast<float *>(m_) + so, HGQ_TYPE_F32, lane, count, true, m);
+        load_any<VEC>(reinterpret_cast<float *>(v_) + so, HGQ_TYPE_F32, lane, count, true, v);
     } else {
+        const float sm = m_scale[so / kAdamBlock], sv = v_scale[so / kAdamBlock];
         load_codes<VEC>(reinterpret_cast<uint8_t *>(m_) + so, lane, count, m);
         load_codes<VEC>(reinterpret_cast<uint8_t *>(v_) + so, lane, count, v);
-        const float sm = m_scale[so / kAdamBlock], sv = v_scale[so / kAdamBlock];
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
             m[j] = __fmul_rn(m[j], sm);
@@ -229,87 +255,116 @@ __device__ __forceinline__ void adamw_block(const hgq_adamw_tensor &T, const voi
             v[j] = __fmul_rn(r, r);
         }
     }
-    const float kept = (float)(1.0 - a.lr * T.decay);
-    float top_m = 0.f, top_r = 0.f;
-    const float l1 = T.l1;
+    if (T.scales) {
+        const float l1 = T.t.l1;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            g[j] = scaled_grad(g[j], a.grad_scale, l1);
+            if (a.clipnorm > 0.0) g[j] = __fmul_rn(g[j], coef);
+        }
+    }
+    // of the block: largest and least sizes (NaN passes by), and a sum that is not zero when a moment is not finite
+    float top_m = 0.f, top_r = 0.f, least_m = INFINITY, least_r = INFINITY, odd_sum = 0.f;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-        float ge = scaled_grad(g[j], a.grad_scale, l1);
-        if (a.clipnorm > 0.0) ge = __fmul_rn(ge, coef);
-        m[j] = __fadd_rn(__fmul_rn(m[j], a.f_b1), __fmul_rn(ge, a.f_1mb1));
-        v[j] = __fadd_rn(__fmul_rn(v[j], a.f_b2), __fmul_rn(__fmul_rn(ge, ge), a.f_1mb2));
+        m[j] = __fadd_rn(__fmul_rn(m[j], a.f_b1), __fmul_rn(g[j], a.f_1mb1));
+        v[j] = __fadd_rn(__fmul_rn(v[j], a.f_b2), __fmul_rn(__fmul_rn(g[j], g[j]), a.f_1mb2));
         const float root = __fsqrt_rn(v[j]);
-        float we = __fsub_rn(__fmul_rn(w[j], kept), __fdiv_rn(__fmul_rn(alpha, m[j]), __fadd_rn(root, a.eps)));
-        we = we < T.lo ? T.lo : we;
-        we = we > T.hi ? T.hi : we;
-        w[j] = we;
+        // the step is a few bits of w: the fast quotient (2 ulp) is far below what is left of it
+        w[j] = __fsub_rn(__fmul_rn(w[j], T.kept), __fdividef(__fmul_rn(alpha, m[j]), __fadd_rn(root, a.eps)));
         if (BITS == 8) {
-            // lanes beyond the tensor's end hold l1-driven values that are not part of the block
-            if (!VEC && elem_of<VEC>(j, lane) >= count) m[j] = 0.f, v[j] = 0.f;
-            else v[j] = root;
+            v[j] = root;
+            // lanes beyond the tensor's end hold values driven by the regulariser that are not part of the block
+            if (!VEC && elem_of<VEC>(j, lane) >= count) m[j] = v[j] = 0.f;
+            top_m = fmaxf(top_m, fabsf(m[j]));
+            top_r = fmaxf(top_r, v[j]);
+            least_m = fminf(least_m, fabsf(m[j]));
+            least_r = fminf(least_r, v[j]);
+            odd_sum = fmaf(m[j], 0.f, fmaf(v[j], 0.f, odd_sum));
+        }
+    }
+    if (T.clamps) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {  // a NaN stays
+            w[j] = w[j] < T.t.lo ? T.t.lo : w[j];
+            w[j] = w[j] > T.t.hi ? T.t.hi : w[j];
+        }
+    }
+    store_any<VEC>(wm, HGQ_TYPE_F32, lane, count, T.wide_w, w);
+    if (T.t.master != nullptr) store_any<VEC>(reinterpret_cast<char *>(T.t.w) + base * (T.t.w_type == HGQ_TYPE_F32 ? 4 : 2), T.t.w_type, lane, count, false, w);
+    if (BITS == 32) {
+        store_any<VEC>(reinterpret_cast<float *>(m_) + so, HGQ_TYPE_F32, lane, count, true, m);
+        store_any<VEC>(reinterpret_cast<float *>(v_) + so, HGQ_TYPE_F32, lane, count, true, v);
+        return;
+    }
+    const bool odd = __any_sync(0xffffffffu, odd_sum != 0.f);
+    if (odd) {  // the scale is that of the finite moments; the others are kept as NaN (e4m3 has no infinity)
+        top_m = top_r = 0.f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
             top_m = fmaxf(top_m, finite_size(m[j]));
             top_r = fmaxf(top_r, finite_size(v[j]));
         }
     }
-    store_any<VEC>(wm, HGQ_TYPE_F32, lane, count, w);
-    if (T.master != nullptr) store_any<VEC>(reinterpret_cast<char *>(T.w) + base * wsize, T.w_type, lane, count, w);
-    if (BITS == 32) {
-        store_any<VEC>(reinterpret_cast<float *>(m_) + so, HGQ_TYPE_F32, lane, count, m);
-        store_any<VEC>(reinterpret_cast<float *>(v_) + so, HGQ_TYPE_F32, lane, count, v);
-        return;
-    }
-    top_m = fmaxf(warp_max(top_m), 0x1p-100f);
-    top_r = fmaxf(warp_max(top_r), 0x1p-100f);
-    const float inv_m = __fdiv_rn(256.f, top_m), inv_r = __fdiv_rn(256.f, top_r);
+    const float fm = fmaxf(warp_max(top_m), 0x1p-100f), fr = fmaxf(warp_max(top_r), 0x1p-100f);
+    const float inv_m = __fdiv_rn(256.f, fm), inv_r = __fdiv_rn(256.f, fr);
+    float um[8], ur[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-        const uint32_t d = dither_bits((uint32_t)(so + elem_of<VEC>(j, lane)), step);
-        const float sm = fabsf(m[j]), sr = v[j];
-        const float cm = copysignf(dithered_e4m3(__fmul_rn(sm, inv_m), d & 0xffffu), m[j]);
-        float cr = dithered_e4m3(__fmul_rn(sr, inv_r), d >> 16);
-        if (sr > 0.f && cr == 0.f) cr = 0x1p-9f;
-        // a moment that is not finite is kept as NaN (e4m3 has no infinity)
-        m[j] = sm <= 3.402823466e38f ? cm : __int_as_float(0x7fc00000);
-        v[j] = sr <= 3.402823466e38f ? cr : __int_as_float(0x7fc00000);
+        um[j] = __fmul_rn(fabsf(m[j]), inv_m);
+        ur[j] = __fmul_rn(v[j], inv_r);
+    }
+    const float least = fminf(__fmul_rn(least_m, inv_m), __fmul_rn(least_r, inv_r));
+    if (!odd && __all_sync(0xffffffffu, least >= 0x1p-6f)) {  // the usual block: no code below the normal range
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const uint32_t d = dither_bits((uint32_t)(so + elem_of<VEC>(j, lane)), step);
+            m[j] = copysignf(dithered_e4m3<false>(um[j], d & 0xffffu), m[j]);
+            v[j] = dithered_e4m3<false>(ur[j], d >> 16);
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const uint32_t d = dither_bits((uint32_t)(so + elem_of<VEC>(j, lane)), step);
+            const float cm = copysignf(dithered_e4m3<true>(um[j], d & 0xffffu), m[j]);
+            float cr = dithered_e4m3<true>(ur[j], d >> 16);
+            if (v[j] > 0.f && cr == 0.f) cr = 0x1p-9f;
+            const float nan = __int_as_float(0x7fc00000);
+            m[j] = fabsf(m[j]) <= 3.402823466e38f ? cm : nan;
+            v[j] = v[j] <= 3.402823466e38f ? cr : nan;
+        }
     }
     store_codes<VEC>(reinterpret_cast<uint8_t *>(m_) + so, lane, count, m);
     store_codes<VEC>(reinterpret_cast<uint8_t *>(v_) + so, lane, count, v);
     if (lane == 0) {
-        m_scale[so / kAdamBlock] = top_m * (1.f / 256.f);
-        v_scale[so / kAdamBlock] = top_r * (1.f / 256.f);
+        m_scale[so / kAdamBlock] = fm * (1.f / 256.f);
+        v_scale[so / kAdamBlock] = fr * (1.f / 256.f);
     }
-}
-
-__device__ __forceinline__ bool block_is_vector(const hgq_adamw_tensor &T, const void *gp, int gtype, int count) {
-    uintptr_t bits = (uintptr_t)T.master;
-    if (T.master != nullptr) bits |= (uintptr_t)T.w << 1;  // 8-byte groups of the 16-bit copy
-    else bits |= (uintptr_t)T.w;
-    bits |= gtype == HGQ_TYPE_F32 ? (uintptr_t)gp : (uintptr_t)gp << 1;
-    return count == kAdamBlock && (bits & 15) == 0;
 }
 
 // Sum of squares of the scaled gradients, one fp64 partial a CTA (fixed assignment of blocks to warps: the sum does not depend
 // on scheduling).
 __global__ void __launch_bounds__(kAdamWarps * 32) k_grad_norm(const __grid_constant__ GradTable G, const hgq_adamw_tensor *__restrict__ tensors,
-                                                               const int2 *__restrict__ blocks, int64_t n_blocks, int first_tensor,
+                                                               const int2 *__restrict__ chunks, int64_t n_chunks, int first_tensor,
                                                                float grad_scale, double *__restrict__ part) {
     __shared__ double red[kAdamWarps];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     double s = 0.0;
-    for (int64_t b = (int64_t)blockIdx.x * kAdamWarps + warp; b < n_blocks; b += (int64_t)gridDim.x * kAdamWarps) {
-        const int2 it = __ldg(blocks + b);
+    for (int64_t c = blockIdx.x; c < n_chunks; c += gridDim.x) {
+        const int2 it = chunks[c];
         const void *gp = G.p[it.x - first_tensor];
         if (gp == nullptr) continue;
         const int gtype = G.type[it.x - first_tensor];
-        const int64_t base = (int64_t)it.y * kAdamBlock, n = tensors[it.x].n;
+        const int64_t base = (int64_t)it.y * HGQ_ADAMW_CHUNK + warp * kAdamBlock, n = tensors[it.x].n;
+        if (base >= n) continue;
         const int count = (int)(n - base < kAdamBlock ? n - base : kAdamBlock);
         const float l1 = tensors[it.x].l1;
         const int gsize = gtype == HGQ_TYPE_F32 ? 4 : 2;
         const char *p = reinterpret_cast<const char *>(gp) + base * gsize;
         float g[8];
         const bool vec = count == kAdamBlock && ((uintptr_t)gp & (uintptr_t)(4 * gsize - 1)) == 0;
-        if (vec) load_any<true>(p, gtype, lane, count, g);
-        else load_any<false>(p, gtype, lane, count, g);
+        if (vec) load_any<true>(p, gtype, lane, count, ((uintptr_t)gp & 31) == 0, g);
+        else load_any<false>(p, gtype, lane, count, false, g);
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
             const double ge = (double)scaled_grad(g[j], grad_scale, l1);
@@ -328,8 +383,8 @@ __global__ void __launch_bounds__(kAdamWarps * 32) k_grad_norm(const __grid_cons
 }
 
 template <int BITS>
-__global__ void __launch_bounds__(kAdamWarps * 32) k_adamw(const __grid_constant__ GradTable G, const hgq_adamw_tensor *__restrict__ tensors,
-                                                           const int2 *__restrict__ blocks, int64_t n_blocks, int first_tensor,
+__global__ void __launch_bounds__(kAdamWarps * 32, BITS == 32 ? kAdamCtas32 : kAdamCtas8) k_adamw(const __grid_constant__ GradTable G, const hgq_adamw_tensor *__restrict__ tensors,
+                                                           const int2 *__restrict__ chunks, int64_t n_chunks, int first_tensor,
                                                            void *m, void *v, float *m_scale, float *v_scale, const AdamScalars a,
                                                            const double *__restrict__ part, int n_part, long long *step,
                                                            unsigned *ticket, int last_launch) {
@@ -358,18 +413,35 @@ __global__ void __launch_bounds__(kAdamWarps * 32) k_adamw(const __grid_constant
     }
     __syncthreads();
     const float alpha = s_alpha, coef = s_coef;
-    for (int64_t b = (int64_t)blockIdx.x * kAdamWarps + warp; b < n_blocks; b += (int64_t)gridDim.x * kAdamWarps) {
-        const int2 it = __ldg(blocks + b);
-        const void *gp = G.p[it.x - first_tensor];
-        if (gp == nullptr) continue;  // no gradient this step: the tensor and its states stay as they are
-        const int gtype = G.type[it.x - first_tensor];
-        const hgq_adamw_tensor T = tensors[it.x];
-        const int64_t base = (int64_t)it.y * kAdamBlock;
-        const int count = (int)(T.n - base < kAdamBlock ? T.n - base : kAdamBlock);
-        if (block_is_vector(T, gp, gtype, count))
-            adamw_block<BITS, true>(T, gp, gtype, base, count, lane, m, v, m_scale, v_scale, a, alpha, coef, (uint32_t)t);
+    Current T;
+    T.index = -1;
+    for (int64_t c = blockIdx.x; c < n_chunks; c += gridDim.x) {
+        const int2 it = chunks[c];
+        if (it.x != T.index) {
+            T.index = it.x;
+            T.t = tensors[it.x];
+            T.g = reinterpret_cast<const char *>(G.p[it.x - first_tensor]);
+            T.gtype = G.type[it.x - first_tensor];
+            T.kept = (float)(1.0 - a.lr * T.t.decay);
+            T.clamps = !(T.t.lo == -INFINITY && T.t.hi == INFINITY);
+            T.scales = a.clipnorm > 0.0 || a.grad_scale != 1.f || T.t.l1 != 0.f;
+            uintptr_t bits = (uintptr_t)T.t.master;
+            if (T.t.master != nullptr) bits |= (uintptr_t)T.t.w << 1;  // 8-byte groups of the 16-bit copy
+            else bits |= (uintptr_t)T.t.w;
+            bits |= T.gtype == HGQ_TYPE_F32 ? (uintptr_t)T.g : (uintptr_t)T.g << 1;
+            T.aligned = (bits & 15) == 0;
+            T.wide_g = ((uintptr_t)T.g & 31) == 0;
+            T.wide_w = ((uintptr_t)(T.t.master != nullptr ? (void *)T.t.master : T.t.w) & 31) == 0;
+        }
+        if (T.g == nullptr) continue;  // no gradient this step: the tensor and its states stay as they are
+        const int64_t base = (int64_t)it.y * HGQ_ADAMW_CHUNK + warp * kAdamBlock;
+        const int64_t left = T.t.n - base;
+        if (left <= 0) continue;
+        if (T.aligned && left >= kAdamBlock)
+            adamw_block<BITS, true>(T, base, kAdamBlock, lane, m, v, m_scale, v_scale, a, alpha, coef, (uint32_t)t);
         else
-            adamw_block<BITS, false>(T, gp, gtype, base, count, lane, m, v, m_scale, v_scale, a, alpha, coef, (uint32_t)t);
+            adamw_block<BITS, false>(T, base, (int)(left < kAdamBlock ? left : kAdamBlock), lane, m, v, m_scale, v_scale, a, alpha, coef,
+                                     (uint32_t)t);
     }
     if (last_launch && threadIdx.x == 0) {
         // every CTA has read the step number before it takes a ticket; the last one advances it
@@ -390,18 +462,18 @@ extern "C" size_t hgq_adamw_workspace(int64_t n_tensors) {
     return (size_t)launches * num_sms() * kNormCtasPerSm * sizeof(double);
 }
 
-extern "C" int hgq_adamw_step(const hgq_adamw_tensor *tensors, int64_t n_tensors, const int32_t *blocks, const int64_t *first_block,
+extern "C" int hgq_adamw_step(const hgq_adamw_tensor *tensors, int64_t n_tensors, const int32_t *chunks, const int64_t *first_chunk,
                               const void *const *grads, const uint8_t *grad_types, int state_bits, void *m, void *v, float *m_scale,
                               float *v_scale, double lr, double beta1, double beta2, double eps, double grad_scale, double clipnorm,
                               long long *step, unsigned *ticket, void *workspace, size_t workspace_bytes, void *stream) {
     if (n_tensors < 0 || n_tensors > INT32_MAX) return HGQ_ERR_SIZE;
     if (state_bits != 32 && state_bits != 8) return HGQ_ERR_MODE;
-    if (!tensors || !blocks || !first_block || !grads || !grad_types || !m || !v || !step || !ticket) return HGQ_ERR_NULL;
+    if (!tensors || !chunks || !first_chunk || !grads || !grad_types || !m || !v || !step || !ticket) return HGQ_ERR_NULL;
     if (state_bits == 8 && (!m_scale || !v_scale)) return HGQ_ERR_NULL;
-    if (!aligned(m, 16) || !aligned(v, 16) || !aligned(blocks, 8) || !aligned(tensors, 8) || !aligned(step, 8)) return HGQ_ERR_ALIGN;
+    if (!aligned(m, 32) || !aligned(v, 32) || !aligned(chunks, 8) || !aligned(tensors, 8) || !aligned(step, 8)) return HGQ_ERR_ALIGN;
     if (n_tensors == 0) return HGQ_OK;
     for (int64_t i = 0; i < n_tensors; ++i) {
-        if (first_block[i + 1] < first_block[i]) return HGQ_ERR_SIZE;
+        if (first_chunk[i + 1] < first_chunk[i]) return HGQ_ERR_SIZE;
         if (grad_types[i] > HGQ_TYPE_F16) return HGQ_ERR_MODE;
         if (grads[i] != nullptr && !aligned(grads[i], grad_types[i] == HGQ_TYPE_F32 ? 4 : 2)) return HGQ_ERR_ALIGN;
     }
@@ -422,23 +494,21 @@ extern "C" int hgq_adamw_step(const hgq_adamw_tensor *tensors, int64_t n_tensors
             const bool last = t0 + cnt == n_tensors;
             GradTable G;
             for (int i = 0; i < cnt; ++i) G.p[i] = grads[t0 + i], G.type[i] = grad_types[t0 + i];
-            const int64_t b0 = first_block[t0], nb = first_block[t0 + cnt] - b0;
-            if (nb == 0 && !(pass == 1 && last)) continue;
-            const int2 *bt = reinterpret_cast<const int2 *>(blocks) + b0;
-            int64_t ctas = (nb + kAdamWarps - 1) / kAdamWarps;
+            const int64_t c0 = first_chunk[t0], nc = first_chunk[t0 + cnt] - c0;
+            if (nc == 0 && !(pass == 1 && last)) continue;
+            const int2 *ct = reinterpret_cast<const int2 *>(chunks) + c0;
+            int64_t ctas = nc;
             if (pass == 0) {
                 if (ctas > (int64_t)sms * kNormCtasPerSm) ctas = (int64_t)sms * kNormCtasPerSm;
-                k_grad_norm<<<(unsigned)ctas, kAdamWarps * 32, 0, st>>>(G, tensors, bt, nb, (int)t0, a.grad_scale, part + n_part);
+                k_grad_norm<<<(unsigned)ctas, kAdamWarps * 32, 0, st>>>(G, tensors, ct, nc, (int)t0, a.grad_scale, part + n_part);
                 n_part += (int)ctas;
             } else {
                 if (ctas < 1) ctas = 1;  // nothing to update, but the step is counted
-                if (ctas > (int64_t)sms * 8) ctas = (int64_t)sms * 8;
-                if (state_bits == 32)
-                    k_adamw<32><<<(unsigned)ctas, kAdamWarps * 32, 0, st>>>(G, tensors, bt, nb, (int)t0, m, v, m_scale, v_scale, a, part,
-                                                                          n_part, step, ticket, last ? 1 : 0);
-                else
-                    k_adamw<8><<<(unsigned)ctas, kAdamWarps * 32, 0, st>>>(G, tensors, bt, nb, (int)t0, m, v, m_scale, v_scale, a, part,
-                                                                         n_part, step, ticket, last ? 1 : 0);
+                const int resident = sms * (state_bits == 32 ? kAdamCtas32 : kAdamCtas8);
+                if (ctas > resident) ctas = resident;
+                auto kernel = state_bits == 32 ? k_adamw<32> : k_adamw<8>;
+                kernel<<<(unsigned)ctas, kAdamWarps * 32, 0, st>>>(G, tensors, ct, nc, (int)t0, m, v, m_scale, v_scale, a, part, n_part, step,
+                                                                      ticket, last ? 1 : 0);
             }
             if (int e = check_launch()) return e;
         }

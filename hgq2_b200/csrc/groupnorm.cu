@@ -377,19 +377,17 @@ static int gn_vec(const void *a, const void *b, const void *c, int C, int type) 
     return 1;
 }
 
-// Partial sums of a call, for whichever access width its addresses allow.
+// Partial sums of a call, for whichever access width its addresses allow (the one-read forward pass has none).
 static size_t gn_part_floats(int64_t B, int64_t S, int C, int G, int type, bool bwd) {
     const int size = type == HGQ_TYPE_F32 ? 4 : 2;
     const int64_t group = gn_group(B, S, C, bwd ? 2 * size : size);
     size_t most = 0;
     for (int v : {16 / size, 4, 2, 1}) {
         if (C % v != 0) continue;
-        const GnGeom g = gn_geom(group, S, C, G, v, bwd ? kGnBwdCtas : kGnFwdCtas);
-        const size_t any = (size_t)g.chunks * 2 * C * (size_t)(bwd ? B : group);
-        most = any > most ? any : most;
         const SlabPlan p = gn_slab_plan(B, S, C, G, type, v, bwd);
-        const size_t slab = p.usable && bwd ? (size_t)p.workers * p.K * 2 * C : 0;
-        most = slab > most ? slab : most;
+        const GnGeom g = gn_geom(group, S, C, G, v, bwd ? kGnBwdCtas : kGnFwdCtas);
+        const size_t n = !p.usable ? (size_t)g.chunks * 2 * C * (size_t)(bwd ? B : group) : (bwd ? (size_t)p.workers * p.K * 2 * C : 0);
+        most = n > most ? n : most;
     }
     return most;
 }
@@ -508,10 +506,10 @@ extern "C" int hgq_group_norm_fwd(const void *x, const float *gamma, const float
     const size_t size = type == HGQ_TYPE_F32 ? 4 : 2;
     if (!aligned(x, size) || !aligned(y, size) || !aligned(gamma, 4) || !aligned(beta, 4) || !aligned(mean, 4) || !aligned(rstd, 4))
         return HGQ_ERR_ALIGN;
-    if (!workspace || workspace_bytes < hgq_group_norm_workspace(B, S, C, G, type, 0)) return HGQ_ERR_WORKSPACE;
-    if (!aligned(workspace, 4)) return HGQ_ERR_ALIGN;
     const int vec = gn_vec(x, y, nullptr, C, type);
     const SlabPlan plan = gn_slab_plan(B, S, C, G, type, vec, false);
+    if (!plan.usable && (!workspace || workspace_bytes < hgq_group_norm_workspace(B, S, C, G, type, 0))) return HGQ_ERR_WORKSPACE;
+    if (!aligned(workspace, 4)) return HGQ_ERR_ALIGN;
     if (plan.usable) return gn_slab_fwd(plan, x, gamma, beta, y, mean, rstd, B, S, C, G, eps, activation, type, (cudaStream_t)stream);
     GN_DISPATCH(gn_fwd_any, x, gamma, beta, y, mean, rstd, B, S, C, G, eps, activation, (float *)workspace, (cudaStream_t)stream);
 }

@@ -7,6 +7,7 @@ These functions are the seam between the Python mirror of the reference interfac
 from __future__ import annotations
 
 from array import array
+from contextlib import nullcontext
 
 import torch
 
@@ -30,12 +31,20 @@ def workspace(nbytes: int, device: torch.device, slot: int = 0) -> torch.Tensor 
         # its memory back to the driver while this graph's kernels still hold the address.
         return torch.empty(nbytes, dtype=torch.uint8, device=device)
     dev = device.index if device.index is not None else torch.cuda.current_device()
-    key = (dev, slot, torch.cuda.current_stream(dev).cuda_stream)
+    key = (dev, slot, torch._C._cuda_getCurrentRawStream(dev))
     ws = _workspaces.get(key)
     if ws is None or ws.numel() < nbytes:
         ws = torch.empty(max(nbytes, 1 << 20), dtype=torch.uint8, device=device)
         _workspaces[key] = ws
     return ws
+
+
+_here = nullcontext()
+
+
+def on_device(device: torch.device):
+    """``torch.cuda.device(device)``, at no cost where it is the current one already."""
+    return _here if torch._C._cuda_getDevice() == device.index else torch.cuda.device(device)
 
 
 def _modes(round_mode: str, overflow_mode: str) -> tuple[int, int]:
@@ -698,10 +707,10 @@ def adamw_step(opt, grads, grad_scale: float = 1.0) -> None:
     addresses, types = array('Q', ptrs), bytes(kinds)
     clip = opt.global_clipnorm or 0.0
     eight = opt.state_bits == 8
-    with torch.cuda.device(dev):
+    with on_device(dev):
         ws = workspace(lib().hgq_adamw_workspace(n), dev, slot=7) if clip else None
         st = lib().hgq_adamw_step(
-            ptr(opt._table), n, ptr(opt._blocks), opt._first_block.ctypes.data, addresses.buffer_info()[0], types, opt.state_bits,
+            ptr(opt._table), n, ptr(opt._chunks), opt._first_chunk.ctypes.data, addresses.buffer_info()[0], types, opt.state_bits,
             ptr(opt.m), ptr(opt.r if eight else opt.v), ptr(opt.m_scale) if eight else None, ptr(opt.r_scale) if eight else None,
             opt.lr, opt.b1, opt.b2, opt.eps, grad_scale, clip, ptr(opt.step_count), ptr(opt._ticket), ptr(ws),
             ws.numel() if ws is not None else 0, stream_handle())
@@ -735,9 +744,9 @@ def group_norm_fwd(x, gamma, beta, groups: int, eps: float = 1e-3, activation: s
     x = x.contiguous()
     gamma, beta = (p if p is None else p.contiguous() for p in (gamma, beta))
     y = torch.empty_like(x)
-    stats = torch.empty((2, B, groups), dtype=torch.float32, device=x.device)
-    mean, rstd = stats[0], stats[1]
-    with torch.cuda.device(x.device):
+    mean = torch.empty((B, groups), dtype=torch.float32, device=x.device)
+    rstd = torch.empty_like(mean)
+    with on_device(x.device):
         ws = workspace(lib().hgq_group_norm_workspace(B, S, C, groups, kind, 0), x.device, slot=8)
         st = lib().hgq_group_norm_fwd(ptr(x), ptr(gamma), ptr(beta), ptr(y), ptr(mean), ptr(rstd), B, S, C, groups, eps, act, kind,
                                       ptr(ws), ws.numel() if ws is not None else 0, stream_handle())
@@ -769,7 +778,7 @@ def group_norm_bwd(gy, x, gamma, beta, mean, rstd, groups: int, activation: str 
     if want_params:
         dgamma = out_dgamma if out_dgamma is not None else torch.empty(C, dtype=torch.float32, device=x.device)
         dbeta = out_dbeta if out_dbeta is not None else torch.empty(C, dtype=torch.float32, device=x.device)
-    with torch.cuda.device(x.device):
+    with on_device(x.device):
         ws = workspace(lib().hgq_group_norm_workspace(B, S, C, groups, kind, 1), x.device, slot=8)
         st = lib().hgq_group_norm_bwd(ptr(gy), ptr(x), ptr(gamma), ptr(beta), ptr(mean), ptr(rstd), ptr(dx), ptr(dgamma), ptr(dbeta), B,
                                       S, C, groups, act, kind, ptr(ws), ws.numel() if ws is not None else 0, stream_handle())
@@ -820,7 +829,7 @@ def gated_scan_fwd(x, z, h0=None, lengths=None, want_states: bool = False):
     h = torch.empty((B, T, D), dtype=x.dtype, device=dev)
     h_last = torch.empty((B, D), dtype=torch.float32, device=dev)
     L = lib()
-    with torch.cuda.device(dev):
+    with on_device(dev):
         states = torch.empty(L.hgq_gated_scan_states(B, T, D), dtype=torch.float32, device=dev) if want_states else None
         ws = workspace(L.hgq_gated_scan_workspace(B, T, D), dev, slot=9)
         st = L.hgq_gated_scan_fwd(ptr(x), x.stride(0), x.stride(1), ptr(z), z.stride(0), z.stride(1), ptr(h0), ptr(lengths), ptr(h),
@@ -845,7 +854,7 @@ def gated_scan_bwd(gh, x, z, h0=None, lengths=None, states=None, g_last=None, wa
     if g_last is not None:
         g_last = _scan_state(g_last, B, D, dev, 'the gradient of h_last')
     L = lib()
-    with torch.cuda.device(dev):
+    with on_device(dev):
         n = L.hgq_gated_scan_states(B, T, D)
         if n and (states is None or states.numel() != n or states.dtype != torch.float32 or states.device != dev):
             raise ValueError('states must be what gated_scan_fwd(..., want_states=True) returned for these inputs')

@@ -197,12 +197,13 @@ class FusedAdamW:
         self.masters = [None if w.dtype == torch.float32 else w.float() for w in self.tensors]
         block = _lib.ADAMW_BLOCK
         self._numels, self._shapes = [w.numel() for w in self.tensors], [w.shape for w in self.tensors]
-        counts = [-(-n // block) for n in self._numels]
+        ends = np.cumsum([-(-n // block) * block for n in self._numels])
+        self.offsets = [0, *map(int, ends[:-1])]
+        total = int(ends[-1])
+        counts = [-(-n // _lib.ADAMW_CHUNK) for n in self._numels]
         first = np.zeros(len(items) + 1, dtype=np.int64)
         np.cumsum(counts, out=first[1:])
-        self._first_block = first
-        self.offsets = [int(f) * block for f in first[:-1]]
-        total = int(first[-1]) * block
+        self._first_chunk = first
         table = (_lib.AdamWTensor * len(items))()
         for i, (t, v) in enumerate(zip(table, items)):
             w, master = self.tensors[i], self.masters[i]
@@ -213,7 +214,7 @@ class FusedAdamW:
         pairs = np.empty((int(first[-1]), 2), dtype=np.int32)
         pairs[:, 0] = np.repeat(np.arange(len(items), dtype=np.int32), counts)
         pairs[:, 1] = np.arange(int(first[-1])) - np.repeat(first[:-1], counts)
-        self._table, self._blocks = torch.from_numpy(raw).to(dev), torch.from_numpy(pairs).to(dev)
+        self._table, self._chunks = torch.from_numpy(raw).to(dev), torch.from_numpy(pairs).to(dev)
         kind = torch.float32 if state_bits == 32 else torch.float8_e4m3fn
         self.m = torch.zeros(total, dtype=torch.uint8 if state_bits == 8 else kind, device=dev).view(kind)
         second = torch.zeros_like(self.m.view(torch.uint8) if state_bits == 8 else self.m).view(kind)
@@ -235,7 +236,8 @@ class FusedAdamW:
 
     def moments(self, i: int) -> tuple[torch.Tensor, torch.Tensor]:
         """The fp32 values of tensor ``i``'s first and second moment (for inspection; 8-bit states are decoded)."""
-        a, b = self.offsets[i], int(self._first_block[i + 1]) * _lib.ADAMW_BLOCK
+        a = self.offsets[i]
+        b = a - (-self._numels[i] // _lib.ADAMW_BLOCK) * _lib.ADAMW_BLOCK
         shape = self.tensors[i].shape
         if self.state_bits == 32:
             m, v = self.m[a:b], self.v[a:b]

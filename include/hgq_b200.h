@@ -424,7 +424,8 @@ int hgq_adam_step(float *w, const float *g, float *m, float *v, const float *lo,
 
 /* ---- AdamW over a list of tensors ----------------------------------------------------------- */
 
-#define HGQ_ADAMW_BLOCK 256 /* consecutive elements of one tensor that share a scale of the 8-bit states */
+#define HGQ_ADAMW_BLOCK 256  /* consecutive elements of one tensor that share a scale of the 8-bit states */
+#define HGQ_ADAMW_CHUNK 2048 /* consecutive elements of one tensor that a CTA takes at a time */
 
 /* One tensor of the list; the array lives in DEVICE memory. */
 typedef struct {
@@ -444,17 +445,17 @@ typedef struct {
  *   g' = (g grad_scale + l1) c,  c = min(clipnorm / |g grad_scale + l1| over all tensors, 1), or 1 if clipnorm <= 0
  *   m = b1 m + (1 - b1) g';  v = b2 v + (1 - b2) g'^2;  alpha = lr sqrt(1 - b2^t) / (1 - b1^t)
  *   w = clamp(w (1 - lr decay) - alpha m / (sqrt(v) + eps), lo, hi)
- * blocks: DEVICE array of (tensor, block of that tensor) pairs of int32, the tensors in order, ceil(n / 256) each; first_block:
+ * chunks: DEVICE array of (tensor, chunk of that tensor) pairs of int32, the tensors in order, ceil(n / 2048) each; first_chunk:
  * HOST array of n_tensors + 1 positions in it.  grads / grad_types: HOST arrays, one entry per tensor (read before the call
  * returns; a captured graph keeps the addresses); a NULL gradient leaves its tensor and states untouched.
- * state_bits 32: m and v are fp32 arrays.  state_bits 8: m and v are byte arrays of e4m3 codes, v holding sqrt(v); m_scale and
+ * m and v are aligned to 32 bytes.  state_bits 32: they are fp32 arrays.  state_bits 8: byte arrays of e4m3 codes, v holding sqrt(v); m_scale and
  * v_scale have one entry per 256 state elements, and a code stands for code * scale.  The rounding is dithered by a fixed
  * function of the element's place and t, so steps repeat bit for bit.  A state that is not finite is kept as NaN.
  * step: device counter (starts at 0), advanced by the call; ticket: a device word that starts at 0 and returns to 0.  Calls that
  * share states must not overlap.  workspace: hgq_adamw_workspace(n_tensors) bytes, needed when clipnorm > 0.
  */
 size_t hgq_adamw_workspace(int64_t n_tensors);
-int hgq_adamw_step(const hgq_adamw_tensor *tensors, int64_t n_tensors, const int32_t *blocks, const int64_t *first_block,
+int hgq_adamw_step(const hgq_adamw_tensor *tensors, int64_t n_tensors, const int32_t *chunks, const int64_t *first_chunk,
                    const void *const *grads, const uint8_t *grad_types, int state_bits, void *m, void *v, float *m_scale,
                    float *v_scale, double lr, double beta1, double beta2, double eps, double grad_scale, double clipnorm,
                    long long *step, unsigned *ticket, void *workspace, size_t workspace_bytes, void *stream);
