@@ -368,13 +368,24 @@ static GnGeom gn_geom(int64_t group, int64_t S, int C, int G, int vec, int ctas_
     return g;
 }
 
+// The widest pack that the addresses and the channel count allow.
 static int gn_vec(const void *a, const void *b, const void *c, int C, int type) {
     const int size = type == HGQ_TYPE_F32 ? 4 : 2;
-    const int full = 16 / size;
-    for (int v : {full, 4, 2}) {
+    for (int v : {16 / size, 4, 2})
         if (C % v == 0 && aligned(a, (size_t)v * size) && aligned(b, (size_t)v * size) && aligned(c, (size_t)v * size)) return v;
-    }
     return 1;
+}
+
+// The one-read plan with the widest pack that the addresses allow (usable == false: none); rows may be joined to make packs fit.
+static SlabPlan gn_plan(const void *a, const void *b, const void *c, int64_t B, int64_t S, int C, int G, int type, bool bwd) {
+    const int size = type == HGQ_TYPE_F32 ? 4 : 2;
+    SlabPlan p{};
+    for (int v : {16 / size, 4, 2, 1}) {
+        if (!aligned(a, (size_t)v * size) || !aligned(b, (size_t)v * size) || !aligned(c, (size_t)v * size)) continue;
+        p = gn_slab_plan(B, S, C, G, type, v, bwd);
+        if (p.usable) return p;
+    }
+    return p;
 }
 
 // Partial sums of a call, for whichever access width its addresses allow (the one-read forward pass has none).
@@ -383,10 +394,12 @@ static size_t gn_part_floats(int64_t B, int64_t S, int C, int G, int type, bool 
     const int64_t group = gn_group(B, S, C, bwd ? 2 * size : size);
     size_t most = 0;
     for (int v : {16 / size, 4, 2, 1}) {
-        if (C % v != 0) continue;
         const SlabPlan p = gn_slab_plan(B, S, C, G, type, v, bwd);
+        size_t n = p.usable && bwd ? (size_t)p.workers * p.K * 2 * C : 0;
+        most = n > most ? n : most;
+        if (C % v != 0) continue;
         const GnGeom g = gn_geom(group, S, C, G, v, bwd ? kGnBwdCtas : kGnFwdCtas);
-        const size_t n = !p.usable ? (size_t)g.chunks * 2 * C * (size_t)(bwd ? B : group) : (bwd ? (size_t)p.workers * p.K * 2 * C : 0);
+        n = p.usable ? 0 : (size_t)g.chunks * 2 * C * (size_t)(bwd ? B : group);
         most = n > most ? n : most;
     }
     return most;
@@ -506,11 +519,11 @@ extern "C" int hgq_group_norm_fwd(const void *x, const float *gamma, const float
     const size_t size = type == HGQ_TYPE_F32 ? 4 : 2;
     if (!aligned(x, size) || !aligned(y, size) || !aligned(gamma, 4) || !aligned(beta, 4) || !aligned(mean, 4) || !aligned(rstd, 4))
         return HGQ_ERR_ALIGN;
-    const int vec = gn_vec(x, y, nullptr, C, type);
-    const SlabPlan plan = gn_slab_plan(B, S, C, G, type, vec, false);
+    const SlabPlan plan = gn_plan(x, y, nullptr, B, S, C, G, type, false);
     if (!plan.usable && (!workspace || workspace_bytes < hgq_group_norm_workspace(B, S, C, G, type, 0))) return HGQ_ERR_WORKSPACE;
     if (!aligned(workspace, 4)) return HGQ_ERR_ALIGN;
     if (plan.usable) return gn_slab_fwd(plan, x, gamma, beta, y, mean, rstd, B, S, C, G, eps, activation, type, (cudaStream_t)stream);
+    const int vec = gn_vec(x, y, nullptr, C, type);
     GN_DISPATCH(gn_fwd_any, x, gamma, beta, y, mean, rstd, B, S, C, G, eps, activation, (float *)workspace, (cudaStream_t)stream);
 }
 
@@ -538,15 +551,15 @@ extern "C" int hgq_group_norm_bwd(const void *gy, const void *x, const float *ga
         return HGQ_ERR_ALIGN;
     if (!workspace || workspace_bytes < hgq_group_norm_workspace(B, S, C, G, type, 1)) return HGQ_ERR_WORKSPACE;
     if (!aligned(workspace, 4)) return HGQ_ERR_ALIGN;
-    const int vec = gn_vec(gy, x, dx, C, type);
     float *part = (float *)workspace;
-    const SlabPlan plan = gn_slab_plan(B, S, C, G, type, vec, true);
+    const SlabPlan plan = gn_plan(gy, x, dx, B, S, C, G, type, true);
     if (plan.usable) {
         if (int e = gn_slab_bwd(plan, gy, x, gamma, beta, mean, rstd, dx, dgamma != nullptr ? part : nullptr, B, S, C, G, activation, type, st))
             return e;
         const int64_t rows = plan.workers * plan.K;
         return dgamma != nullptr ? gn_colsum(part, rows, C, part + rows * 2 * C, dgamma, dbeta, st) : HGQ_OK;
     }
+    const int vec = gn_vec(gy, x, dx, C, type);
     float *m = part + gn_part_floats(B, S, C, G, type, true);
     float *scratch = m + 2 * gn_group(B, S, C, 2 * (int)size) * G;
     GN_DISPATCH(gn_bwd_any, gy, x, gamma, beta, mean, rstd, dx, dgamma, dbeta, B, S, C, G, activation, part, m, scratch, st);

@@ -136,6 +136,7 @@ struct SlabPlan {
     bool usable;
     int groups_of_pack;  // numbers that a pack adds to: one a group where packs and groups nest, else one a channel
     int vec;        // channels a thread takes at once
+    int q;          // rows taken as one where vec does not divide the channels
     int R;          // packs of one tensor that a thread holds
     int K;          // CTAs of a cluster that share a slab's rows
     int slabs;      // along the channels; Cs channels (whole groups) each, the last one may have fewer

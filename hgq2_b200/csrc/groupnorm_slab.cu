@@ -22,8 +22,12 @@ constexpr int kSlabWarps = kSlabThreads / 32;
 constexpr int kMaxCluster = 2;  // clusters of 4 and 8 wait for one another longer than a second read from L2 takes
 constexpr int kMaxPairs = 512;  // (sample, group) pairs of a CTA
 
+// Channel counts that packs do not divide: q rows in a row are taken as one of q C channels, which packs do divide; S and C are
+// those of the joined rows, `channels` the real count.
 struct SlabArgs {
     int64_t B, S, items, workers;
+    float inv_n;  // 1 / (values of a group)
+    int channels, q;
     int C, G, Cg, Cs, Gs, slabs, TX, TY, K, subs, rows;
     int TYs;  // thread rows of one sample: TY / subs
     int per_row;  // neighbouring threads of a row that belong to one group (one a pack), or 1
@@ -31,9 +35,9 @@ struct SlabArgs {
     // certain bits of their index: those of lane_bits meet in shuffles, those of warp_bits through shared memory.
     bool bits;
     unsigned lane_bits, warp_bits;
-    // Otherwise: entries in shared memory, [TY][width], per_group of a row to one group.
-    int width, per_group;
-    FastDiv by_per_group;
+    // Otherwise: entries in shared memory, [TY][width]; a row has q runs (one every `channels`) of `run` entries for a group.
+    int width, run, per_group;  // per_group = q run
+    FastDiv by_per_group, by_run;
 };
 
 // Where a thread works: its channels, its sample among the CTA's and its first row.
@@ -51,7 +55,7 @@ __device__ __forceinline__ SlabPlace slab_place(const SlabArgs &a, int vec) {
     p.slab = cluster % a.slabs;
     p.worker = cluster / a.slabs;
     p.groups = min(a.Gs, a.G - p.slab * a.Gs);
-    p.channels = p.groups * a.Cg;
+    p.channels = a.q > 1 ? a.C : p.groups * a.Cg;
     p.tx = threadIdx.x % a.TX;
     p.ty = threadIdx.x / a.TX;
     p.in = p.ty < a.TY && p.tx * vec < p.channels;
@@ -142,9 +146,11 @@ __device__ __forceinline__ void group_totals(float (&v)[N][NG], SumSpace<NG, N> 
             for (int k = 0; k < N; ++k) s[k] = 0.f;
             if (pair < pairs) {
                 const int sub = a.subs > 1 ? pair / p.groups : 0, g = pair - sub * p.groups;
-                const float *e = sh.entries + (sub * rows) * a.width + g * a.per_group;
+                const float *e = sh.entries + (sub * rows) * a.width + g * a.run;
                 for (int j = l; j < n; j += lanes) {
-                    const int r = (int)fastdiv((uint32_t)j, a.by_per_group), c = j - r * a.per_group;
+                    const int r = (int)fastdiv((uint32_t)j, a.by_per_group);
+                    int c = j - r * a.per_group;
+                    if (a.q > 1) c += (int)fastdiv((uint32_t)c, a.by_run) * (a.channels - a.run);
 #pragma unroll
                     for (int k = 0; k < N; ++k) s[k] += e[k * NG * kSlabThreads + r * a.width + c];
                 }
@@ -199,21 +205,23 @@ __global__ void __launch_bounds__(kSlabThreads, slab_fwd_ctas(R * VEC, AHEAD))
     __shared__ SumSpace<NG, 1> sh;
     const SlabPlace p = slab_place(a, VEC);
     const int c0 = p.slab * a.Cs + p.tx * VEC;
-    const float inv_n = 1.f / ((float)a.S * (float)a.Cg);
+    const float inv_n = a.inv_n;
     float ga[VEC], be[VEC];
     int pair_of[NG], group_of[NG];
     unsigned writes = 0;
 #pragma unroll
     for (int i = 0; i < VEC; ++i) {
-        ga[i] = p.in && gamma != nullptr ? gamma[c0 + i] : 1.f;
-        be[i] = p.in && beta != nullptr ? beta[c0 + i] : 0.f;
+        const int c = a.q > 1 ? (c0 + i) % a.channels : c0 + i;
+        ga[i] = p.in && gamma != nullptr ? gamma[c] : 1.f;
+        be[i] = p.in && beta != nullptr ? beta[c] : 0.f;
     }
 #pragma unroll
     for (int i = 0; i < NG; ++i) {
-        group_of[i] = p.in ? (p.tx * VEC + i * W) / a.Cg : 0;
+        const int c = p.tx * VEC + i * W;
+        group_of[i] = p.in ? (a.q > 1 ? c % a.channels : c) / a.Cg : 0;
         pair_of[i] = (p.in ? p.sub : 0) * p.groups + group_of[i];
         // the first thread of each (sample, group) writes its statistics: the first row's first pack of it
-        if (p.in && p.rank == 0 && p.row == 0 && (p.tx * VEC + i * W) % a.Cg == 0) writes |= 1u << i;
+        if (p.in && p.rank == 0 && p.row == 0 && c < a.channels && c % a.Cg == 0) writes |= 1u << i;
     }
     const int64_t step = (int64_t)a.TYs * a.C, end = min(a.S, (int64_t)(p.rank + 1) * a.rows);
     const int64_t row = (int64_t)p.rank * a.rows + p.row;
@@ -300,18 +308,20 @@ __global__ void __launch_bounds__(kSlabThreads, 2)
     __shared__ float acc[2 * VEC][kSlabThreads];  // du and du xhat of this thread's channels, over all of the CTA's samples
     const SlabPlace p = slab_place(a, VEC);
     const int c0 = p.slab * a.Cs + p.tx * VEC;
-    const float inv_n = 1.f / ((float)a.S * (float)a.Cg);
+    const float inv_n = a.inv_n;
     float ga[VEC], be[VEC];
     int pair_of[NG], group_of[NG];
 #pragma unroll
     for (int i = 0; i < VEC; ++i) {
-        ga[i] = p.in && gamma != nullptr ? gamma[c0 + i] : 1.f;
-        be[i] = p.in && beta != nullptr ? beta[c0 + i] : 0.f;
+        const int c = a.q > 1 ? (c0 + i) % a.channels : c0 + i;
+        ga[i] = p.in && gamma != nullptr ? gamma[c] : 1.f;
+        be[i] = p.in && beta != nullptr ? beta[c] : 0.f;
         acc[i][threadIdx.x] = acc[VEC + i][threadIdx.x] = 0.f;
     }
 #pragma unroll
     for (int i = 0; i < NG; ++i) {
-        group_of[i] = p.in ? (p.tx * VEC + i * W) / a.Cg : 0;
+        const int c = p.tx * VEC + i * W;
+        group_of[i] = p.in ? (a.q > 1 ? c % a.channels : c) / a.Cg : 0;
         pair_of[i] = (p.in ? p.sub : 0) * p.groups + group_of[i];
     }
     const int64_t step = (int64_t)a.TYs * a.C, end = min(a.S, (int64_t)(p.rank + 1) * a.rows);
@@ -385,16 +395,18 @@ __global__ void __launch_bounds__(kSlabThreads, 2)
     }
     if (part != nullptr) {
         // this CTA's sums per channel, over its thread rows
-        float *out = part + (p.worker * a.K + p.rank) * 2 * a.C;
+        float *out = part + (p.worker * a.K + p.rank) * 2 * a.channels;
         __syncthreads();
-        for (int c = threadIdx.x; c < p.channels; c += kSlabThreads) {
+        const int real = a.q > 1 ? a.channels : p.channels;
+        for (int c = threadIdx.x; c < real; c += kSlabThreads) {
             float s1 = 0.f, s2 = 0.f;
-            for (int r = 0; r < a.TY; ++r) {
-                s1 += acc[c % VEC][r * a.TX + c / VEC];
-                s2 += acc[VEC + c % VEC][r * a.TX + c / VEC];
-            }
+            for (int k = c; k < p.channels; k += real)
+                for (int r = 0; r < a.TY; ++r) {
+                    s1 += acc[k % VEC][r * a.TX + k / VEC];
+                    s2 += acc[VEC + k % VEC][r * a.TX + k / VEC];
+                }
             out[p.slab * a.Cs + c] = s1;
-            out[a.C + p.slab * a.Cs + c] = s2;
+            out[a.channels + p.slab * a.Cs + c] = s2;
         }
     }
     if (a.K > 1) cg::this_cluster().sync();
@@ -416,13 +428,18 @@ static void slab_held(int type, int vec, bool backward, int &usual, int &most) {
 
 SlabPlan gn_slab_plan(int64_t B, int64_t S, int C, int G, int type, int vec, bool backward) {
     SlabPlan p{};
+    p.q = 1;
+    while ((int64_t)p.q * C % vec != 0) p.q <<= 1;  // vec is a power of two
+    if (S % p.q != 0 || (p.q > 1 && (int64_t)p.q * C / vec > kSlabThreads)) return p;
     const int Cg = C / G, size = type == HGQ_TYPE_F32 ? 4 : 2;
     int usual, most;
     slab_held(type, vec, backward, usual, most);
     p.vec = vec;
-    p.groups_of_pack = Cg % vec == 0 ? 1 : (vec % Cg == 0 ? vec / Cg : vec);
+    p.groups_of_pack = p.q > 1 ? vec : (Cg % vec == 0 ? 1 : (vec % Cg == 0 ? vec / Cg : vec));
     // whole groups whose channels are whole packs
-    int unit = Cg;
+    S /= p.q;
+    C *= p.q;
+    int unit = p.q > 1 ? C : Cg;
     while (unit % vec != 0) unit += Cg;  // at most vec groups
     if (C % unit != 0 || unit / vec > kSlabThreads) return p;
     // Slabs as wide as 128 threads allow (wide rows are read whole), narrower where the rows of a slab would not fit, but no
@@ -430,7 +447,7 @@ SlabPlan gn_slab_plan(int64_t B, int64_t S, int C, int G, int type, int vec, boo
     int units = C / unit;
     int per = units;
     while (per > 1 && (per * unit / vec > 128 || per * unit / Cg > kMaxPairs)) per = (per + 1) / 2;
-    if (per * unit / Cg > kMaxPairs) return p;
+    if (per * unit / Cg / p.q > kMaxPairs) return p;
     for (;; per = (per + 1) / 2) {
         p.Cs = per * unit;
         p.TX = p.Cs / vec;
@@ -439,7 +456,7 @@ SlabPlan gn_slab_plan(int64_t B, int64_t S, int C, int G, int type, int vec, boo
         if (S <= fits) break;
         if (per == 1 || ((per + 1) / 2) * unit * size < 64) return p;
     }
-    p.Gs = p.Cs / Cg;
+    p.Gs = p.Cs / Cg / p.q;
     p.slabs = (G + p.Gs - 1) / p.Gs;
     // As few thread rows for a sample as hold it (what a total costs is a matter of threads, not of values): the CTA's others take
     // other samples, if there are enough of them to give every SM two CTAs.
@@ -475,18 +492,21 @@ SlabPlan gn_slab_plan(int64_t B, int64_t S, int C, int G, int type, int vec, boo
 
 static SlabArgs slab_args(const SlabPlan &p, int64_t B, int64_t S, int C, int G) {
     SlabArgs a{};
-    a.B = B, a.S = S, a.items = p.items, a.workers = p.workers;
-    a.C = C, a.G = G, a.Cg = C / G, a.Cs = p.Cs, a.Gs = p.Gs, a.slabs = p.slabs, a.TX = p.TX, a.TY = p.TY, a.K = p.K, a.subs = p.subs,
+    a.channels = C, a.q = p.q, a.inv_n = 1.f / ((float)S * (float)(C / G));
+    a.B = B, a.S = S / p.q, a.items = p.items, a.workers = p.workers;
+    a.C = C * p.q, a.G = G, a.Cg = C / G, a.Cs = p.Cs, a.Gs = p.Gs, a.slabs = p.slabs, a.TX = p.TX, a.TY = p.TY, a.K = p.K, a.subs = p.subs,
     a.rows = p.rows, a.TYs = p.TYs;
     a.per_row = a.Cg % p.vec == 0 ? a.Cg / p.vec : 1;
     // one number a pack where it lies in one group, else one a group it touches or one a channel
     const int ng = p.groups_of_pack;
     a.width = p.TX * ng;
-    a.per_group = ng == 1 ? a.per_row : (ng * a.Cg == p.vec ? 1 : a.Cg);
+    a.run = ng == 1 ? a.per_row : (p.q == 1 && ng * a.Cg == p.vec ? 1 : a.Cg);
+    a.per_group = a.run * p.q;
     a.by_per_group = make_fastdiv((uint32_t)a.per_group);
+    a.by_run = make_fastdiv((uint32_t)a.run);
     auto pow2 = [](int64_t v) { return v > 0 && (v & (v - 1)) == 0; };
     // thread index, from the low bit: packs of a group, groups, rows of a sample, samples
-    a.bits = pow2(p.TX) && pow2(a.per_row) && p.TX * p.TY == kSlabThreads && C % p.Cs == 0 &&
+    a.bits = p.q == 1 && pow2(p.TX) && pow2(a.per_row) && p.TX * p.TY == kSlabThreads && a.C % p.Cs == 0 &&
              (ng == 1 ? a.Cg % p.vec == 0 : ng * a.Cg == p.vec);
     const unsigned bits = (unsigned)(a.per_row - 1) | ((unsigned)(p.TYs - 1) * (unsigned)p.TX);
     a.lane_bits = bits & 31u;

@@ -15,6 +15,9 @@ SHAPES = [  # (batch, spatial, channels, groups)
     (4, (3, 3), 37, 1), (2, (9,), 6, 6), (1, (300,), 1, 1), (2, (2, 2), 2048, 4), (1, (40, 40), 1030, 2), (5, (4, 4), 64, 8),
     (1, (129, 127), 24, 24), (300, (2,), 16, 2), (3, (), 128, 4), (1, (700,), 520, 260), (2, (33, 31), 10, 5), (700, (4, 4), 8, 2),
     (2, (200, 100), 64, 1), (1, (3, 1025, 7), 40, 20),
+    # channel counts that 16-byte accesses do not divide: rows joined, or not where their number does not allow it
+    (3, (8, 8), 37, 37), (2, (16,), 45, 9), (5, (4, 4), 20, 5), (300, (8,), 3, 1), (2, (40, 30), 21, 7), (2, (24,), 255, 5),
+    (400, (12,), 45, 3), (3, (30, 30), 44, 11),
 ]
 
 
