@@ -808,7 +808,7 @@ def _scan_args(x, z, h0, lengths):
         if lengths.shape != (B,) or lengths.is_floating_point() or lengths.dtype == torch.bool or lengths.device != x.device:
             raise ValueError(f'lengths must be {B} whole numbers on {x.device}')
         if lengths.dtype != torch.int32:
-            lengths = lengths.clamp(0, T).to(torch.int32)
+            lengths = lengths.to(torch.int64).clamp(0, T).to(torch.int32)
         lengths = lengths.contiguous()
     return x, z, h0, lengths, kind, B, T, D
 

@@ -3,6 +3,7 @@
 from __future__ import annotations
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from .. import kernels, routes
 from ..backend import bookkeeping
@@ -448,6 +449,7 @@ class GroupNormFn(torch.autograd.Function):
         return y
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, gy):
         x, gamma, beta, mean, rstd = ctx.saved_tensors
         groups, activation = ctx.meta
@@ -470,6 +472,7 @@ class GatedScanFn(torch.autograd.Function):
         return h, h_last
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, gh, g_last):
         p, h0, lengths, states = ctx.saved_tensors
         dp = torch.empty_like(p)

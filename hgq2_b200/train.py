@@ -158,7 +158,10 @@ class FusedAdamW:
 
     ``state_bits=8`` keeps the moments as e4m3 codes with an fp32 scale per 256 elements of a tensor: ``m`` (times ``m_scale``)
     and ``r`` (times ``r_scale``), the root of the second moment -- 2 bytes per weight instead of 8.  ``state_bits=32`` keeps
-    fp32 ``m`` and ``v``.  The state arrays are flat; tensor ``i`` starts at ``offsets[i]``, a multiple of 256."""
+    fp32 ``m`` and ``v``.  The state arrays are flat; tensor ``i`` starts at ``offsets[i]``, a multiple of 256.
+
+    The tensors' addresses are taken at construction: build the optimizer after whatever lays the parameters out
+    (``FlatState``), and after assigning new values to bf16 / fp16 tensors call ``sync_masters``."""
 
     def __init__(self, tensors, learning_rate=1e-3, beta_1=0.9, beta_2=0.999, epsilon=1e-7, weight_decay=0.004,
                  global_clipnorm: float | None = None, state_bits: int = 32):
@@ -233,6 +236,12 @@ class FusedAdamW:
         if grads is None:
             grads = [v.value.grad if isinstance(v, Variable) else v.grad for v in self._items]
         kernels.adamw_step(self, grads, grad_scale)
+
+    def sync_masters(self) -> None:
+        """Take the fp32 copies from the bf16 / fp16 tensors again (after new weights were loaded into those)."""
+        for w, master in zip(self.tensors, self.masters):
+            if master is not None:
+                master.copy_(w)
 
     def moments(self, i: int) -> tuple[torch.Tensor, torch.Tensor]:
         """The fp32 values of tensor ``i``'s first and second moment (for inspection; 8-bit states are decoded)."""

@@ -188,6 +188,9 @@ def test_half_precision_tensors_go_through_a_master_copy(bits, dtype):
     for w, master, f in zip(ws, a.masters, fp):
         assert torch.equal(master, f)
         assert torch.equal(w, f.to(dtype))
+    ws[1].fill_(0.5)
+    a.sync_masters()
+    assert torch.equal(a.masters[1], torch.full_like(a.masters[1], 0.5))
 
 
 @gpu

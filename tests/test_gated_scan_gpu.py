@@ -153,6 +153,40 @@ def test_slices_of_a_wider_projection_are_read_in_place(T):
 
 
 @gpu
+@pytest.mark.parametrize('kind', [torch.int8, torch.uint8, torch.int16, torch.int64])
+def test_lengths_of_any_whole_type(kind):
+    from hgq2_b200 import kernels as K
+
+    x, z, _, h0, _ = inputs((4, 300, 16), torch.float32, 8)
+    lengths = torch.tensor([0, 5, 100, 127], device='cuda')
+    want = K.gated_scan_fwd(x, z, h0, lengths.to(torch.int32))
+    got = K.gated_scan_fwd(x, z, h0, lengths.to(kind))
+    assert torch.equal(want[0], got[0]) and torch.equal(want[1], got[1])
+    far = K.gated_scan_fwd(x, z, h0, torch.tensor([-7, 5, 100, 1 << 40], device='cuda'))  # clamped to [0, T]
+    assert torch.equal(far[0][:3], want[0][:3]) and torch.equal(far[0][3], K.gated_scan_fwd(x, z, h0)[0][3])
+
+
+@gpu
+def test_long_sequences_with_wide_and_narrow_rows():
+    """The same values through 16-byte pieces fetched ahead, pairs and single channels: the access widths agree to the bit."""
+    from hgq2_b200 import kernels as K
+
+    for dtype in HALF_STEP:
+        x, z, gh, h0, g_last = inputs((3, 1500, 48), dtype, 9)
+        h, last, st = K.gated_scan_fwd(x, z, h0, want_states=True)
+        grads = K.gated_scan_bwd(gh, x, z, h0, None, st, g_last, want_dh0=True)
+        for pad, skip in ((2, 0), (2, 2), (1, 1)):  # row strides and offsets that allow pairs, or single channels only
+            buf = [torch.zeros(3, 1500, 48 + pad + skip, device='cuda', dtype=dtype) for _ in range(3)]
+            views = [b[..., skip:skip + 48] for b in buf]
+            for v, t in zip(views, (x, z, gh)):
+                v.copy_(t)
+            h2, last2, st2 = K.gated_scan_fwd(views[0], views[1], h0, want_states=True)
+            got = K.gated_scan_bwd(views[2], views[0], views[1], h0, None, st2, g_last, want_dh0=True)
+            assert torch.equal(h, h2) and torch.equal(last, last2) and torch.equal(st, st2)
+            assert all(torch.equal(a, b) for a, b in zip(grads, got))
+
+
+@gpu
 @pytest.mark.parametrize('T', [1, 50, 5000])
 def test_only_the_last_state_has_a_gradient(T):
     from hgq2_b200 import kernels as K

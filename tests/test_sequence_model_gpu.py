@@ -293,3 +293,15 @@ def test_autograd_of_the_layers_captures():
     want = grads()
     for a, b in zip(got, want):
         close(a, b, 1e-6, 'gradient')
+
+
+@gpu
+def test_second_derivatives_are_refused():
+    """The backward passes are kernels without a derivative of their own: asking for one is an error, not a zero."""
+    from hgq2_b200.layers import GroupNormalization
+
+    x = torch.randn(4, 9, 8, device='cuda', requires_grad=True)
+    for layer in (GroupNormalization(2, activation='silu'), recurrence(8, 9, 8, True)):
+        (g,) = torch.autograd.grad(layer(x, training=True).square().sum(), x, create_graph=True)
+        with pytest.raises(RuntimeError):
+            g.square().sum().backward()
