@@ -9,6 +9,12 @@
 // their variance.  All statistics are fp32 per thread, group totals fp32 or fp64; x, gy, y, dx are fp32, bf16 or fp16 and are
 // rounded once, on the way out.  The backward pass recomputes u from x (nothing of y is needed), so a pass moves x and gy in and
 // dx out.
+//
+// This file: the entries, and the kernels for samples that do not fit on chip (the others are in groupnorm_slab.cu).  Those read
+// twice: partial statistics per channel of runs of rows, totals in fp64, then the application, in groups of samples small enough
+// that the second read finds them in L2.  Bound by latency and by the activation's arithmetic more than by memory: [6, 255, 257, 96]
+// bf16 with SiLU 0.066 ms forward and 0.124 ms backward (75 MB a tensor).  One wave of CTAs: two more than the SMs hold
+// at once made the backward pass 0.160 ms.
 #include "groupnorm.cuh"
 
 namespace hgq {
@@ -67,8 +73,8 @@ __device__ __forceinline__ void sum_over_ty(float (&v)[N], float *sh, const GnGe
 }
 
 // Per (sample, chunk, channel): mean and centred sum of squares of its rows.  Sums are taken of x minus the chunk's first row, so
-// a large mean costs no digits as long as rows of one channel lie within a few spreads of one another; the totals' step is exact
-// about the rest.
+// a large mean costs no digits; if that row is itself the outlier of n rows, the squares lose at most about n 2^-24 of the variance
+// (its distance is part of the variance).  The totals' step is in fp64.
 template <typename T, int VEC>
 __global__ void __launch_bounds__(kThreads, kGnFwdCtas) k_gn_stats(const T *__restrict__ x, const GnGeom g, int64_t b_base, float *__restrict__ part) {
     __shared__ float sh[kThreads * 2 * VEC];
@@ -421,7 +427,8 @@ static int gn_fwd_any(const void *x, const float *gamma, const float *beta, void
     for (int64_t b0 = 0; b0 < B; b0 += group) {
         const int64_t nb = B - b0 < group ? B - b0 : group, pairs = nb * G;
         const int64_t ctas = nb * g.chunks * g.tiles;
-        const bool wide = (int64_t)g.chunks * g.Cg > 256;  // parts of a total: a block for each, or a warp
+        // parts of a total: a block for each where they are many or the totals few, else a warp
+        const bool wide = (int64_t)g.chunks * g.Cg > 256 || ((int64_t)g.chunks * g.Cg > 32 && pairs < 16 * num_sms());
         const int64_t sums = wide ? pairs : (pairs + kThreads / 32 - 1) / (kThreads / 32);
         if (ctas > INT32_MAX || sums > INT32_MAX || (int64_t)g.chunks * g.Cg > INT32_MAX) return HGQ_ERR_SIZE;
         k_gn_stats<T, VEC><<<(unsigned)ctas, kThreads, 0, st>>>((const T *)x, g, b0, part);
@@ -458,7 +465,8 @@ static int gn_bwd_any(const void *gy, const void *x, const float *gamma, const f
     for (int64_t b0 = 0; b0 < B; b0 += group) {
         const int64_t nb = B - b0 < group ? B - b0 : group, pairs = nb * G;
         const int64_t ctas = nb * g.chunks * g.tiles;
-        const bool wide = (int64_t)g.chunks * g.Cg > 256;  // parts of a total: a block for each, or a warp
+        // parts of a total: a block for each where they are many or the totals few, else a warp
+        const bool wide = (int64_t)g.chunks * g.Cg > 256 || ((int64_t)g.chunks * g.Cg > 32 && pairs < 16 * num_sms());
         const int64_t sums = wide ? pairs : (pairs + kThreads / 32 - 1) / (kThreads / 32);
         if (ctas > INT32_MAX || sums > INT32_MAX || (int64_t)g.chunks * g.Cg > INT32_MAX) return HGQ_ERR_SIZE;
         float *p = part + b0 * g.chunks * 2 * C;

@@ -8,6 +8,7 @@ from __future__ import annotations
 
 from array import array
 from contextlib import nullcontext
+from operator import attrgetter
 
 import torch
 
@@ -40,6 +41,7 @@ def workspace(nbytes: int, device: torch.device, slot: int = 0) -> torch.Tensor 
 
 
 _here = nullcontext()
+_dtype_of = attrgetter('dtype')
 
 
 def on_device(device: torch.device):
@@ -684,27 +686,28 @@ def adamw_step(opt, grads, grad_scale: float = 1.0) -> None:
     present = [g for g in grads if g is not None]
     if not present:
         raise ValueError('no gradients: every entry is None')
-    # checks over whole lists: a model has hundreds of tensors and this loop is on the path of every step
+    # checks over whole lists: a model has hundreds of tensors and this is on the path of every step
     T = torch.Tensor
     if set(map(T.get_device, present)) != {dev.index}:
         raise ValueError(f'gradients must be on {dev}')
-    shapes = opt._shapes
-    if len(present) < n:
-        shapes = [s for s, g in zip(shapes, grads) if g is not None]
+    shapes = opt._shapes if len(present) == n else [s for s, g in zip(opt._shapes, grads) if g is not None]
     if [g.shape for g in present] != shapes:
         raise ValueError('a gradient does not have the shape of its tensor')
-    dtypes = [g.dtype for g in present]
-    unknown = set(dtypes) - ELEMENT_TYPES.keys()
-    if unknown:
-        raise ValueError(f'gradients of {unknown} are not supported: fp32, bf16 and fp16 are')
+    dtypes = set(map(_dtype_of, present))
+    if not dtypes <= ELEMENT_TYPES.keys():
+        raise ValueError(f'gradients of {dtypes - ELEMENT_TYPES.keys()} are not supported: fp32, bf16 and fp16 are')
     if not all(map(T.is_contiguous, present)):
         present = [g.contiguous() for g in present]  # kept alive until the launch below
     ptrs = list(map(T.data_ptr, present))
-    kinds = [ELEMENT_TYPES[d] for d in dtypes]
+    if len(dtypes) == 1:
+        types = bytes([ELEMENT_TYPES[dtypes.pop()]]) * len(present)
+    else:
+        types = bytes([ELEMENT_TYPES[g.dtype] for g in present])
     if len(present) < n:
-        each = iter(zip(ptrs, kinds))
-        ptrs, kinds = zip(*[(0, 0) if g is None else next(each) for g in grads])
-    addresses, types = array('Q', ptrs), bytes(kinds)
+        each = iter(zip(ptrs, types))
+        ptrs, types = zip(*[(0, 0) if g is None else next(each) for g in grads])
+        types = bytes(types)
+    addresses = array('Q', ptrs)
     clip = opt.global_clipnorm or 0.0
     eight = opt.state_bits == 8
     with on_device(dev):
