@@ -444,6 +444,7 @@ SlabPlan gn_slab_plan(int64_t B, int64_t S, int C, int G, int type, int vec, boo
     slab_held(type, vec, backward, usual, most);
     p.vec = vec;
     p.groups_of_pack = p.q > 1 ? vec : (Cg % vec == 0 ? 1 : (vec % Cg == 0 ? vec / Cg : vec));
+    if (p.q == 1 && Cg > kSlabThreads * vec) return p;
     // whole groups whose channels are whole packs
     S /= p.q;
     C *= p.q;

@@ -112,14 +112,18 @@ __device__ __forceinline__ void load_packs(const T *__restrict__ p, int64_t stri
         for (int k = 0; k < VEC; ++k) v[i][k] = scan_float(q[i].v[k]);
 }
 
-// The same through shared memory, fetched a tile ahead: a warp's packs of one sequence are STEPS rows of 32 packs, copied as 16-byte
-// pieces (a quarter to an eighth of the instructions that copies of a lane's own packs take, which cost more issue slots than
-// the recurrence).  A piece lies in one batch row; steps that are not live are filled with zeros.
-template <typename T, int VEC, int STEPS, int N>
+// The same through shared memory, fetched a tile ahead: a warp's packs of one sequence are STEPS rows of 32 packs, copied as pieces of
+// 16 bytes (a quarter to an eighth of the instructions that copies of a lane's own packs take, which cost more issue slots than
+// the recurrence).  A piece lies in one batch row; steps that are not live are filled with zeros.  Rows that allow no more: pieces of 8
+// bytes still pay for 16-bit types ([64, 2048, 252] bf16 0.071 ms forward against 0.086 with direct loads), not for fp32
+// ([64, 2048, 254] 0.127 against 0.096), and pieces of 4 for neither (odd fp32 rows 0.144 against 0.086).  PIECE == 0: not used.
+template <typename T, int VEC, int STEPS, int N, int PIECE>
 struct Stages {
     using P = ScanPack<T, VEC>;
-    static constexpr int kPieces = 32 * (int)sizeof(P) / 16;  // of a row
-    static constexpr int kRows = 32 / kPieces;                // rows that one instruction of the warp copies
+    static constexpr int kPiece = PIECE > 0 ? PIECE : 16;
+    static constexpr int kPieces = 32 * (int)sizeof(P) / kPiece;  // of a row
+    static constexpr int kRows = 32 / kPieces;                    // rows that one instruction of the warp copies
+    static_assert(kRows >= 1, "a row's pieces fit a warp");
     P *base;        // this warp's buffers: [2][N][STEPS][32]
     uint32_t dst;   // where this lane's piece of a buffer's first rows goes
     int row;        // of this lane's piece
@@ -130,8 +134,8 @@ struct Stages {
         const int w = threadIdx.x >> 5, lane = threadIdx.x & 31, piece = lane % kPieces;
         base = reinterpret_cast<P *>(smem) + w * (2 * N * STEPS * 32);
         row = lane / kPieces;
-        dst = (uint32_t)__cvta_generic_to_shared(base) + (uint32_t)(row * kPieces + piece) * 16u;
-        const int64_t c = (((int64_t)blockIdx.x * s.WC + w / WT) * 32) * VEC + piece * (16 / (int)sizeof(T));
+        dst = (uint32_t)__cvta_generic_to_shared(base) + (uint32_t)((row * kPieces + piece) * kPiece);
+        const int64_t c = (((int64_t)blockIdx.x * s.WC + w / WT) * 32) * VEC + piece * (kPiece / (int)sizeof(T));
         in = c < s.channels;
         b = in ? c / s.D : 0;
         d = in ? c - b * s.D : 0;
@@ -147,11 +151,17 @@ struct Stages {
         const int64_t left = p != nullptr ? len - t0 : 0;
         uint32_t to = dst + (uint32_t)(((tile & 1) * N + n) * STEPS * 32 * (int)sizeof(P));
 #pragma unroll
-        for (int i = 0; i < STEPS; i += kRows, to += 512u) {
+        for (int i = 0; i < STEPS; i += kRows, to += 32u * kPiece) {
             const bool live = row + i < left;
             const T *q = live ? src + (t0 + row + i) * time : p;
-            if (p != nullptr) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(q), "r"(live ? 16 : 0) : "memory");
-            else asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(to), "r"(0) : "memory");
+            if (p == nullptr) {
+#pragma unroll
+                for (int k = 0; k < kPiece; k += 4) asm volatile("st.shared.b32 [%0], %1;" ::"r"(to + k), "r"(0) : "memory");
+            } else if (kPiece == 16) {
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(q), "r"(live ? 16 : 0) : "memory");
+            } else {
+                asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(to), "l"(q), "n"(kPiece), "r"(live ? kPiece : 0) : "memory");
+            }
         }
     }
     static __device__ __forceinline__ void commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
@@ -205,7 +215,7 @@ struct alignas(8 * VEC) Map {  // h -> A h + H for VEC channels
 };
 
 // Segment fold of the forward recurrence: agg[segment][channel] = (A, H).
-template <typename T, int VEC, int STEPS, int WARPS, bool AHEAD>
+template <typename T, int VEC, int STEPS, int WARPS, int PIECE>
 __global__ void __launch_bounds__(256) k_scan_fold(const T *__restrict__ x, const T *__restrict__ z, const int32_t *__restrict__ lengths,
                                                    const ScanDims s, float2 *__restrict__ agg) {
     __shared__ Map<VEC> sh[2][kScanMaxWarps][32];
@@ -217,7 +227,8 @@ __global__ void __launch_bounds__(256) k_scan_fold(const T *__restrict__ x, cons
 #pragma unroll
     for (int k = 0; k < VEC; ++k) A[k] = 1.f, H[k] = 0.f;
     extern __shared__ __align__(16) unsigned char staging[];
-    const Stages<T, VEC, STEPS, 2> stages(staging, s, WT, lengths);
+    constexpr bool AHEAD = PIECE > 0;
+    const Stages<T, VEC, STEPS, 2, PIECE> stages(staging, s, WT, lengths);
     auto fetch = [&](int64_t tile) {
         const int64_t t0 = (tile * WT + l.wt) * STEPS;
         stages.fetch(tile, 0, z, s.zsb, s.zst, t0);
@@ -269,7 +280,7 @@ __global__ void __launch_bounds__(256) k_scan_fold(const T *__restrict__ x, cons
         for (int k = 0; k < VEC; ++k) agg[(int64_t)seg * s.channels + l.c + k] = make_float2(A[k], H[k]);
 }
 
-template <typename T, int VEC, int STEPS, int WARPS, bool AHEAD>
+template <typename T, int VEC, int STEPS, int WARPS, int PIECE>
 __global__ void __launch_bounds__(256, VEC == 2 ? kFwdCtas : 4) k_scan_fwd(const T *__restrict__ x, const T *__restrict__ z, const float *__restrict__ h0,
                                                   const int32_t *__restrict__ lengths, const ScanDims s, const float2 *__restrict__ agg,
                                                   T *__restrict__ out, float *__restrict__ h_last, float *__restrict__ states) {
@@ -290,7 +301,8 @@ __global__ void __launch_bounds__(256, VEC == 2 ? kFwdCtas : 4) k_scan_fwd(const
                 carry[k] = q.x * carry[k] + q.y;
             }
     extern __shared__ __align__(16) unsigned char staging[];
-    const Stages<T, VEC, STEPS, 2> stages(staging, s, WT, lengths);
+    constexpr bool AHEAD = PIECE > 0;
+    const Stages<T, VEC, STEPS, 2, PIECE> stages(staging, s, WT, lengths);
     auto fetch = [&](int64_t tile) {
         const int64_t t0 = (tile * WT + l.wt) * STEPS;
         stages.fetch(tile, 0, z, s.zsb, s.zst, t0);
@@ -370,7 +382,7 @@ __global__ void __launch_bounds__(256, VEC == 2 ? kFwdCtas : 4) k_scan_fwd(const
 }
 
 // Segment fold of the backward recurrence: agg[segment][channel] = (A, L), the map of the gradient that arrives from the right.
-template <typename T, int VEC, int STEPS, int WARPS, bool AHEAD>
+template <typename T, int VEC, int STEPS, int WARPS, int PIECE>
 __global__ void __launch_bounds__(256) k_scan_bwd_fold(const T *__restrict__ gh, const T *__restrict__ z, const int32_t *__restrict__ lengths,
                                                        const ScanDims s, float2 *__restrict__ agg) {
     __shared__ Map<VEC> sh[2][kScanMaxWarps][32];
@@ -382,7 +394,8 @@ __global__ void __launch_bounds__(256) k_scan_bwd_fold(const T *__restrict__ gh,
 #pragma unroll
     for (int k = 0; k < VEC; ++k) A[k] = 1.f, L[k] = 0.f;
     extern __shared__ __align__(16) unsigned char staging[];
-    const Stages<T, VEC, STEPS, 2> stages(staging, s, WT, lengths);
+    constexpr bool AHEAD = PIECE > 0;
+    const Stages<T, VEC, STEPS, 2, PIECE> stages(staging, s, WT, lengths);
     auto fetch = [&](int64_t tile) {
         const int64_t t0 = (tile * WT + l.wt) * STEPS;
         stages.fetch(tile, 0, z, s.zsb, s.zst, t0);
@@ -434,7 +447,7 @@ __global__ void __launch_bounds__(256) k_scan_bwd_fold(const T *__restrict__ gh,
         for (int k = 0; k < VEC; ++k) agg[(int64_t)seg * s.channels + l.c + k] = make_float2(A[k], L[k]);
 }
 
-template <typename T, int VEC, int STEPS, int WARPS, bool AHEAD>
+template <typename T, int VEC, int STEPS, int WARPS, int PIECE>
 __global__ void __launch_bounds__(256, VEC == 2 ? kBwdCtas : 3) k_scan_bwd(const T *__restrict__ gh, const T *__restrict__ x, const T *__restrict__ z,
                                                   const float *__restrict__ h0, const int32_t *__restrict__ lengths,
                                                   const float *__restrict__ states, const float *__restrict__ g_last, const ScanDims s,
@@ -458,7 +471,8 @@ __global__ void __launch_bounds__(256, VEC == 2 ? kBwdCtas : 3) k_scan_bwd(const
                 mu[k] = q.x * mu[k] + q.y;
             }
     extern __shared__ __align__(16) unsigned char staging[];
-    const Stages<T, VEC, STEPS, 3> stages(staging, s, WT, lengths);
+    constexpr bool AHEAD = PIECE > 0;
+    const Stages<T, VEC, STEPS, 3, PIECE> stages(staging, s, WT, lengths);
     auto fetch = [&](int64_t tile) {
         const int64_t t0 = (tile * WT + l.wt) * STEPS;
         stages.fetch(tile, 0, z, s.zsb, s.zst, t0);
@@ -638,10 +652,13 @@ int allow_smem(K kernel, size_t bytes) {
     return (int)e;
 }
 
-// What a lane takes of the channels: one, a pair, or a pair out of pieces fetched ahead (the pieces for CTAs that walk several tiles).
-enum ScanAccess { kOne, kPair, kPieces };
+// What a lane takes of the channels, one or a pair, and the bytes of the pieces that are fetched ahead where a CTA walks several tiles
+// (0: direct loads).
+struct ScanAccess {
+    int vec, piece;
+};
 
-template <typename T, int VEC, bool AHEAD>
+template <typename T, int VEC, int PIECE>
 int scan_fwd(const ScanDims &s, const void *x, const void *z, const float *h0, const int32_t *lengths, void *h, float *h_last, float *states,
              float2 *agg, cudaStream_t st) {
     const dim3 grid((unsigned)((s.channels + 32 * VEC * s.WC - 1) / (32 * VEC * s.WC)), (unsigned)s.segments);
@@ -649,26 +666,26 @@ int scan_fwd(const ScanDims &s, const void *x, const void *z, const float *h0, c
     const T *px = (const T *)x, *pz = (const T *)z;
     T *ph = (T *)h;
     constexpr int W = kScanMaxWarps;
-    constexpr size_t bytes = AHEAD ? kStageBytes<T, VEC, 2> : 0;
+    constexpr size_t bytes = PIECE > 0 ? kStageBytes<T, VEC, 2> : 0;
     if (s.segments > 1) {  // more than one tile: WT is kScanMaxWarps
-        auto fold = k_scan_fold<T, VEC, kScanSteps, W, AHEAD>;
+        auto fold = k_scan_fold<T, VEC, kScanSteps, W, PIECE>;
         if (int e = allow_smem(fold, bytes)) return e;
         fold<<<grid, threads, bytes, st>>>(px, pz, lengths, s, agg);
         if (int e = check_launch()) return e;
     }
     if (s.WT == W) {
-        auto fwd = k_scan_fwd<T, VEC, kScanSteps, W, AHEAD>;
+        auto fwd = k_scan_fwd<T, VEC, kScanSteps, W, PIECE>;
         if (int e = allow_smem(fwd, bytes)) return e;
         fwd<<<grid, threads, bytes, st>>>(px, pz, h0, lengths, s, agg, ph, h_last, states);
     } else if (s.T == 1) {
-        k_scan_fwd<T, VEC, 1, 1, false><<<grid, threads, 0, st>>>(px, pz, h0, lengths, s, agg, ph, h_last, states);
+        k_scan_fwd<T, VEC, 1, 1, 0><<<grid, threads, 0, st>>>(px, pz, h0, lengths, s, agg, ph, h_last, states);
     } else {
-        k_scan_fwd<T, VEC, kScanSteps, 0, false><<<grid, threads, 0, st>>>(px, pz, h0, lengths, s, agg, ph, h_last, states);
+        k_scan_fwd<T, VEC, kScanSteps, 0, 0><<<grid, threads, 0, st>>>(px, pz, h0, lengths, s, agg, ph, h_last, states);
     }
     return check_launch();
 }
 
-template <typename T, int VEC, bool AHEAD>
+template <typename T, int VEC, int PIECE>
 int scan_bwd(const ScanDims &s, const void *gh, const void *x, const void *z, const float *h0, const int32_t *lengths, const float *states,
              const float *g_last, void *dx, void *dz, float *dh0, float2 *agg, cudaStream_t st) {
     const dim3 grid((unsigned)((s.channels + 32 * VEC * s.WC - 1) / (32 * VEC * s.WC)), (unsigned)s.segments);
@@ -677,39 +694,49 @@ int scan_bwd(const ScanDims &s, const void *gh, const void *x, const void *z, co
     T *pdx = (T *)dx, *pdz = (T *)dz;
     constexpr int W = kScanMaxWarps;
     if (s.segments > 1) {
-        constexpr size_t bytes = AHEAD ? kStageBytes<T, VEC, 2> : 0;
-        auto fold = k_scan_bwd_fold<T, VEC, kScanSteps, W, AHEAD>;
+        constexpr size_t bytes = PIECE > 0 ? kStageBytes<T, VEC, 2> : 0;
+        auto fold = k_scan_bwd_fold<T, VEC, kScanSteps, W, PIECE>;
         if (int e = allow_smem(fold, bytes)) return e;
         fold<<<grid, threads, bytes, st>>>(pg, pz, lengths, s, agg);
         if (int e = check_launch()) return e;
     }
     if (s.WT == W) {
-        constexpr size_t bytes = AHEAD ? kStageBytes<T, VEC, 3> : 0;
-        auto bwd = k_scan_bwd<T, VEC, kScanSteps, W, AHEAD>;
+        constexpr size_t bytes = PIECE > 0 ? kStageBytes<T, VEC, 3> : 0;
+        auto bwd = k_scan_bwd<T, VEC, kScanSteps, W, PIECE>;
         if (int e = allow_smem(bwd, bytes)) return e;
         bwd<<<grid, threads, bytes, st>>>(pg, px, pz, h0, lengths, states, g_last, s, agg, pdx, pdz, dh0);
     } else if (s.T == 1) {
-        k_scan_bwd<T, VEC, 1, 1, false><<<grid, threads, 0, st>>>(pg, px, pz, h0, lengths, states, g_last, s, agg, pdx, pdz, dh0);
+        k_scan_bwd<T, VEC, 1, 1, 0><<<grid, threads, 0, st>>>(pg, px, pz, h0, lengths, states, g_last, s, agg, pdx, pdz, dh0);
     } else {
-        k_scan_bwd<T, VEC, kScanSteps, 0, false><<<grid, threads, 0, st>>>(pg, px, pz, h0, lengths, states, g_last, s, agg, pdx, pdz, dh0);
+        k_scan_bwd<T, VEC, kScanSteps, 0, 0><<<grid, threads, 0, st>>>(pg, px, pz, h0, lengths, states, g_last, s, agg, pdx, pdz, dh0);
     }
     return check_launch();
+}
+
+ScanAccess scan_access(const ScanDims &s, size_t size, std::initializer_list<const void *> ptrs, std::initializer_list<int64_t> strides) {
+    ScanAccess how{scan_packs(s.D, size, 2, ptrs, strides) ? 2 : 1, 0};
+    if (s.tiles_per_segment > 1)
+        for (int bytes : {16, 8})
+            if (how.piece == 0 && (bytes == 16 || size == 2) && scan_packs(s.D, size, bytes / (int)size, ptrs, strides)) how.piece = bytes;
+    return how;
 }
 
 template <typename T>
 int scan_fwd_by(ScanAccess how, const ScanDims &s, const void *x, const void *z, const float *h0, const int32_t *lengths, void *h,
                 float *h_last, float *states, float2 *agg, cudaStream_t st) {
-    if (how == kPieces) return scan_fwd<T, 2, true>(s, x, z, h0, lengths, h, h_last, states, agg, st);
-    if (how == kPair) return scan_fwd<T, 2, false>(s, x, z, h0, lengths, h, h_last, states, agg, st);
-    return scan_fwd<T, 1, false>(s, x, z, h0, lengths, h, h_last, states, agg, st);
+    if (how.piece == 16) return scan_fwd<T, 2, 16>(s, x, z, h0, lengths, h, h_last, states, agg, st);
+    if (how.piece == 8) return scan_fwd<T, 2, (sizeof(T) == 2 ? 8 : 0)>(s, x, z, h0, lengths, h, h_last, states, agg, st);
+    if (how.vec == 2) return scan_fwd<T, 2, 0>(s, x, z, h0, lengths, h, h_last, states, agg, st);
+    return scan_fwd<T, 1, 0>(s, x, z, h0, lengths, h, h_last, states, agg, st);
 }
 
 template <typename T>
 int scan_bwd_by(ScanAccess how, const ScanDims &s, const void *gh, const void *x, const void *z, const float *h0, const int32_t *lengths,
                 const float *states, const float *g_last, void *dx, void *dz, float *dh0, float2 *agg, cudaStream_t st) {
-    if (how == kPieces) return scan_bwd<T, 2, true>(s, gh, x, z, h0, lengths, states, g_last, dx, dz, dh0, agg, st);
-    if (how == kPair) return scan_bwd<T, 2, false>(s, gh, x, z, h0, lengths, states, g_last, dx, dz, dh0, agg, st);
-    return scan_bwd<T, 1, false>(s, gh, x, z, h0, lengths, states, g_last, dx, dz, dh0, agg, st);
+    if (how.piece == 16) return scan_bwd<T, 2, 16>(s, gh, x, z, h0, lengths, states, g_last, dx, dz, dh0, agg, st);
+    if (how.piece == 8) return scan_bwd<T, 2, (sizeof(T) == 2 ? 8 : 0)>(s, gh, x, z, h0, lengths, states, g_last, dx, dz, dh0, agg, st);
+    if (how.vec == 2) return scan_bwd<T, 2, 0>(s, gh, x, z, h0, lengths, states, g_last, dx, dz, dh0, agg, st);
+    return scan_bwd<T, 1, 0>(s, gh, x, z, h0, lengths, states, g_last, dx, dz, dh0, agg, st);
 }
 
 }  // namespace
@@ -732,9 +759,7 @@ extern "C" int hgq_gated_scan_fwd(const void *x, int64_t x_batch, int64_t x_time
     if (s.tiles <= 1) states = nullptr;
     cudaStream_t st = (cudaStream_t)stream;
     float2 *agg = (float2 *)workspace;
-    ScanAccess how = kOne;
-    if (scan_packs(D, size, 2, {x, z, h}, {x_batch, x_time, z_batch, z_time})) how = kPair;
-    if (s.tiles_per_segment > 1 && scan_packs(D, size, (int)(16 / size), {x, z, h}, {x_batch, x_time, z_batch, z_time})) how = kPieces;
+    const ScanAccess how = scan_access(s, size, {x, z, h}, {x_batch, x_time, z_batch, z_time});
     if (type == HGQ_TYPE_F32) return scan_fwd_by<float>(how, s, x, z, h0, lengths, h, h_last, states, agg, st);
     if (type == HGQ_TYPE_BF16) return scan_fwd_by<__nv_bfloat16>(how, s, x, z, h0, lengths, h, h_last, states, agg, st);
     return scan_fwd_by<__half>(how, s, x, z, h0, lengths, h, h_last, states, agg, st);
@@ -764,9 +789,7 @@ extern "C" int hgq_gated_scan_bwd(const void *gh, int64_t g_batch, int64_t g_tim
     float2 *agg = (float2 *)workspace;
     const std::initializer_list<const void *> ptrs = {gh, x, z, dx, dz};
     const std::initializer_list<int64_t> strides = {g_batch, g_time, x_batch, x_time, z_batch, z_time, dx_batch, dx_time, dz_batch, dz_time};
-    ScanAccess how = kOne;
-    if (scan_packs(D, size, 2, ptrs, strides)) how = kPair;
-    if (s.tiles_per_segment > 1 && scan_packs(D, size, (int)(16 / size), ptrs, strides)) how = kPieces;
+    const ScanAccess how = scan_access(s, size, ptrs, strides);
     if (type == HGQ_TYPE_F32) return scan_bwd_by<float>(how, s, gh, x, z, h0, lengths, states, g_last, dx, dz, dh0, agg, st);
     if (type == HGQ_TYPE_BF16) return scan_bwd_by<__nv_bfloat16>(how, s, gh, x, z, h0, lengths, states, g_last, dx, dz, dh0, agg, st);
     return scan_bwd_by<__half>(how, s, gh, x, z, h0, lengths, states, g_last, dx, dz, dh0, agg, st);

@@ -175,7 +175,7 @@ def test_long_sequences_with_wide_and_narrow_rows():
         x, z, gh, h0, g_last = inputs((3, 1500, 48), dtype, 9)
         h, last, st = K.gated_scan_fwd(x, z, h0, want_states=True)
         grads = K.gated_scan_bwd(gh, x, z, h0, None, st, g_last, want_dh0=True)
-        for pad, skip in ((2, 0), (2, 2), (1, 1)):  # row strides and offsets that allow pairs, or single channels only
+        for pad, skip in ((4, 0), (4, 4), (2, 0), (2, 2), (1, 1)):  # strides and offsets that allow four, two, or single channels
             buf = [torch.zeros(3, 1500, 48 + pad + skip, device='cuda', dtype=dtype) for _ in range(3)]
             views = [b[..., skip:skip + 48] for b in buf]
             for v, t in zip(views, (x, z, gh)):
