@@ -265,6 +265,23 @@ def test_more_tensors_than_one_launch_takes(bits):
 
 
 @gpu
+@pytest.mark.parametrize('bits', [32, 8])
+def test_offsets_past_32_bits(bits):
+    from hgq2_b200.train import FusedAdamW
+
+    n = 2 ** 31 + 777
+    w = torch.empty(n, device='cuda').normal_()
+    g = torch.empty(n, device='cuda', dtype=torch.bfloat16).normal_()
+    tail = w[-2000:].double()
+    opt = FusedAdamW([w], learning_rate=LR, weight_decay=0.0, state_bits=bits)
+    opt.step([g])
+    zero = torch.zeros_like(tail)
+    want, off = want_step(tail, g[-2000:].double(), zero, zero, 1, 0.0, 1.0, 0.0, None, 0.0)
+    assert bool(((w[-2000:].double() - want[0]).abs() <= off[0] + 1e-30).all())
+    assert not bool((opt.m[:n][-2000:].float() == 0).all())
+
+
+@gpu
 def test_not_finite_gradients():
     """Without clipping a NaN or infinite gradient stays in its element; with clipping its norm reaches every weight."""
     from hgq2_b200.train import FusedAdamW

@@ -199,6 +199,22 @@ def test_only_the_last_state_has_a_gradient(T):
 
 
 @gpu
+def test_offsets_past_32_bits():
+    from hgq2_b200 import kernels as K
+
+    B, T, D = 4200, 4096, 128
+    x, z = (torch.empty(B, T, D, device='cuda', dtype=torch.bfloat16).normal_() for _ in range(2))
+    assert x.numel() > 2 ** 31
+    h, last, st = K.gated_scan_fwd(x, z, want_states=True)
+    want = reference(x[-1:], z[-1:], None, None, x[-1:], None)
+    close(h[-1:], want['h'], want['size'], torch.bfloat16, 40, 'h')
+    del h
+    dx, dz, _ = K.gated_scan_bwd(x, x, z, None, None, st)
+    close(dx[-1:], want['dx'], want['size_dx'], torch.bfloat16, 80, 'dx')
+    close(dz[-1:], want['dz'], want['size_dz'], torch.bfloat16, 160, 'dz')
+
+
+@gpu
 def test_gates_at_their_ends():
     """A gate of exactly 0 forgets, of exactly 1 keeps; very long memory stays accurate."""
     from hgq2_b200 import kernels as K

@@ -170,6 +170,28 @@ def test_not_finite_values_stay_in_their_group():
 
 
 @gpu
+def test_offsets_past_32_bits():
+    """2.2e9 elements in samples that fit on the chip and in images that do not: the last sample's last group is right."""
+    from hgq2_b200 import kernels as K
+
+    for B, S, C, G in ((16500, 2048, 64, 8), (3, 11300, 65536, 64)):
+        x = torch.empty(B, S, C, device='cuda', dtype=torch.bfloat16).normal_()
+        assert x.numel() > 2 ** 31
+        y, mean, rstd = K.group_norm_fwd(x, None, None, G, 1e-3, 'silu')
+        dx, _, dbeta = K.group_norm_bwd(x, x, None, None, mean, rstd, G, 'silu')
+        gr = slice(C - C // G, C)  # the last group of the last sample
+        want = reference(x[-1:, :, gr], None, None, 1, 1e-3, 'silu', x[-1:, :, gr])
+        # the bound is for sums of 200 terms a thread; here they are 2048 * 64 / 512 = 256, and for the image, 8 channels a thread
+        # and one wave of 148 * 512 threads or more, up to 3 * 11300 * 65536 / (148 * 512) = 29300
+        more = 2 if S == 2048 else 150
+        close(y[-1:, :, gr], (want['y'][0], want['y'][1] * more), 'y')
+        close(dx[-1:, :, gr], (want['dx'][0], want['dx'][1] * more), 'dx')
+        assert bool(torch.isfinite(dbeta).all())
+        del x, y, dx, want
+        torch.cuda.empty_cache()
+
+
+@gpu
 def test_empty_inputs():
     from hgq2_b200 import kernels as K
 
