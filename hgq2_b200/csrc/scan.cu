@@ -40,7 +40,8 @@ namespace hgq {
 constexpr int kScanSteps = 8;
 constexpr int kScanMaxWarps = 8;  // along time
 constexpr int kScanMaxSegments = 128;
-constexpr int kFwdCtas = 3, kBwdCtas = 2;  // CTAs of 256 threads an SM, by their registers
+constexpr int kFwdCtas = 3, kBwdCtas = 2;    // CTAs of 256 threads an SM, by their registers, with two channels a lane
+constexpr int kFwdCtas1 = 4, kBwdCtas1 = 3;  // and with one
 
 __device__ __forceinline__ float scan_float(float v) { return v; }
 __device__ __forceinline__ float scan_float(__nv_bfloat16 v) { return __bfloat162float(v); }
@@ -70,17 +71,29 @@ struct Lane {
     int wt, row, lane;  // row: of this warp in the CTA's exchange buffer, counted from its channel tile's first warp at row - wt
 };
 
-template <int VEC>
+// IN_ROWS: lanes do not cross batch rows, for an odd number of features (a kernel's own variant: the arithmetic costs the short
+// sequences 0.005 ms of 0.074).  A pair left half empty by the row's end becomes the row's last two channels, one of them its
+// neighbour's too (both compute and write the same bits).
+template <int VEC, bool IN_ROWS = false>
 __device__ __forceinline__ Lane scan_lane(const ScanDims &s, int WT, const int32_t *lengths) {
     Lane l;
     const int w = threadIdx.x >> 5;
     l.lane = threadIdx.x & 31;
     l.wt = w % WT;
     l.row = w;
-    l.c = (((int64_t)blockIdx.x * s.WC + w / WT) * 32 + l.lane) * VEC;
-    l.in = l.c < s.channels;
-    l.b = l.in ? l.c / s.D : 0;
-    l.d = l.in ? l.c - l.b * s.D : 0;
+    if (IN_ROWS) {
+        const int64_t p = ((int64_t)blockIdx.x * s.WC + w / WT) * 32 + l.lane, row = (s.D + VEC - 1) / VEC;
+        l.in = p < s.B * row;
+        l.b = l.in ? p / row : 0;
+        l.d = l.in ? (p - l.b * row) * VEC : 0;
+        if (l.in && l.d > s.D - VEC) l.d = s.D - VEC;
+        l.c = l.b * s.D + l.d;
+    } else {
+        l.c = (((int64_t)blockIdx.x * s.WC + w / WT) * 32 + l.lane) * VEC;
+        l.in = l.c < s.channels;
+        l.b = l.in ? l.c / s.D : 0;
+        l.d = l.in ? l.c - l.b * s.D : 0;
+    }
     l.len = l.in ? s.T : 0;
     if (l.in && lengths != nullptr) {
         const int64_t n = lengths[l.b];
@@ -89,21 +102,31 @@ __device__ __forceinline__ Lane scan_lane(const ScanDims &s, int WT, const int32
     return l;
 }
 
+// SINGLE: an access for each element, for rows whose packs are not aligned.
+template <typename T, int VEC, bool SINGLE>
+__device__ __forceinline__ ScanPack<T, VEC> load_pack(const T *__restrict__ p) {
+    if (!SINGLE) return *reinterpret_cast<const ScanPack<T, VEC> *>(p);
+    ScanPack<T, VEC> q;
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) q.v[k] = p[k];
+    return q;
+}
+
 // STEPS packs of a strided sequence as fp32; p: the lane's channel at the first of them, `left`: how many of them are live (the
 // others read as zero).
-template <typename T, int VEC, int STEPS>
+template <typename T, int VEC, int STEPS, bool SINGLE = false>
 __device__ __forceinline__ void load_packs(const T *__restrict__ p, int64_t stride, bool full, int64_t left, float (&v)[STEPS][VEC]) {
     using P = ScanPack<T, VEC>;
     P q[STEPS];
     if (full) {
 #pragma unroll
-        for (int i = 0; i < STEPS; ++i, p += stride) q[i] = *reinterpret_cast<const P *>(p);
+        for (int i = 0; i < STEPS; ++i, p += stride) q[i] = load_pack<T, VEC, SINGLE>(p);
     } else {
 #pragma unroll
         for (int i = 0; i < STEPS; ++i, p += stride) {
 #pragma unroll
             for (int k = 0; k < VEC; ++k) scan_round(0.f, q[i].v[k]);
-            if (i < left) q[i] = *reinterpret_cast<const P *>(p);
+            if (i < left) q[i] = load_pack<T, VEC, SINGLE>(p);
         }
     }
 #pragma unroll
@@ -116,7 +139,8 @@ __device__ __forceinline__ void load_packs(const T *__restrict__ p, int64_t stri
 // 16 bytes (a quarter to an eighth of the instructions that copies of a lane's own packs take, which cost more issue slots than
 // the recurrence).  A piece lies in one batch row; steps that are not live are filled with zeros.  Rows that allow no more: pieces of 8
 // bytes still pay for 16-bit types ([64, 2048, 252] bf16 0.071 ms forward against 0.086 with direct loads), not for fp32
-// ([64, 2048, 254] 0.127 against 0.096), and pieces of 4 for neither (odd fp32 rows 0.144 against 0.086).  PIECE == 0: not used.
+// ([64, 2048, 254] 0.127 against 0.096), and pieces of 4 for neither (odd fp32 rows 0.144 against 0.086).  PIECE == 0: not used; < 0: not used, and
+// an access for each element of a pack.
 template <typename T, int VEC, int STEPS, int N, int PIECE>
 struct Stages {
     using P = ScanPack<T, VEC>;
@@ -181,7 +205,7 @@ struct Stages {
     }
 };
 
-template <typename T, int VEC, int STEPS>
+template <typename T, int VEC, int STEPS, bool SINGLE = false>
 __device__ __forceinline__ void store_packs(T *p, int64_t stride, bool full, int64_t left, const float (&v)[STEPS][VEC]) {
     using P = ScanPack<T, VEC>;
 #pragma unroll
@@ -189,7 +213,14 @@ __device__ __forceinline__ void store_packs(T *p, int64_t stride, bool full, int
         P q;
 #pragma unroll
         for (int k = 0; k < VEC; ++k) scan_round(v[i][k], q.v[k]);
-        if (full || i < left) *reinterpret_cast<P *>(p) = q;
+        if (full || i < left) {
+            if (SINGLE) {
+#pragma unroll
+                for (int k = 0; k < VEC; ++k) p[k] = q.v[k];
+            } else {
+                *reinterpret_cast<P *>(p) = q;
+            }
+        }
     }
 }
 
@@ -281,7 +312,7 @@ __global__ void __launch_bounds__(256) k_scan_fold(const T *__restrict__ x, cons
 }
 
 template <typename T, int VEC, int STEPS, int WARPS, int PIECE>
-__global__ void __launch_bounds__(256, VEC == 2 ? kFwdCtas : 4) k_scan_fwd(const T *__restrict__ x, const T *__restrict__ z, const float *__restrict__ h0,
+__global__ void __launch_bounds__(256, VEC == 2 ? kFwdCtas : kFwdCtas1) k_scan_fwd(const T *__restrict__ x, const T *__restrict__ z, const float *__restrict__ h0,
                                                   const int32_t *__restrict__ lengths, const ScanDims s, const float2 *__restrict__ agg,
                                                   T *__restrict__ out, float *__restrict__ h_last, float *__restrict__ states) {
     __shared__ Map<VEC> sh[2][kScanMaxWarps][32];
@@ -387,7 +418,7 @@ __global__ void __launch_bounds__(256) k_scan_bwd_fold(const T *__restrict__ gh,
                                                        const ScanDims s, float2 *__restrict__ agg) {
     __shared__ Map<VEC> sh[2][kScanMaxWarps][32];
     const int WT = WARPS > 0 ? WARPS : s.WT;
-    const Lane l = scan_lane<VEC>(s, WT, lengths);
+    const Lane l = scan_lane<VEC, (PIECE < 0)>(s, WT, lengths);
     const int seg = blockIdx.y;
     const int64_t first = seg * s.tiles_per_segment, last = min(s.tiles, first + s.tiles_per_segment);
     float A[VEC], L[VEC];
@@ -413,8 +444,8 @@ __global__ void __launch_bounds__(256) k_scan_bwd_fold(const T *__restrict__ gh,
             stages.values(tile, 0, a);
             stages.values(tile, 1, g);
         } else {
-            load_packs<T, VEC, STEPS>(z + l.b * s.zsb + l.d + t0 * s.zst, s.zst, full, left, a);
-            load_packs<T, VEC, STEPS>(gh + l.b * s.gsb + l.d + t0 * s.gst, s.gst, full && gh != nullptr, gh != nullptr ? left : 0, g);
+            load_packs<T, VEC, STEPS, (PIECE < 0)>(z + l.b * s.zsb + l.d + t0 * s.zst, s.zst, full, left, a);
+            load_packs<T, VEC, STEPS, (PIECE < 0)>(gh + l.b * s.gsb + l.d + t0 * s.gst, s.gst, full && gh != nullptr, gh != nullptr ? left : 0, g);
         }
         make_gates<T, VEC, STEPS>(full, left, a, c);
         Map<VEC> m;
@@ -448,7 +479,7 @@ __global__ void __launch_bounds__(256) k_scan_bwd_fold(const T *__restrict__ gh,
 }
 
 template <typename T, int VEC, int STEPS, int WARPS, int PIECE>
-__global__ void __launch_bounds__(256, VEC == 2 ? kBwdCtas : 3) k_scan_bwd(const T *__restrict__ gh, const T *__restrict__ x, const T *__restrict__ z,
+__global__ void __launch_bounds__(256, VEC == 2 ? kBwdCtas : kBwdCtas1) k_scan_bwd(const T *__restrict__ gh, const T *__restrict__ x, const T *__restrict__ z,
                                                   const float *__restrict__ h0, const int32_t *__restrict__ lengths,
                                                   const float *__restrict__ states, const float *__restrict__ g_last, const ScanDims s,
                                                   const float2 *__restrict__ agg, T *__restrict__ dx, T *__restrict__ dz,
@@ -456,7 +487,7 @@ __global__ void __launch_bounds__(256, VEC == 2 ? kBwdCtas : 3) k_scan_bwd(const
     __shared__ Map<VEC> sh[2][kScanMaxWarps][32];
     __shared__ float shl[2][kScanMaxWarps][VEC][32];
     const int WT = WARPS > 0 ? WARPS : s.WT;
-    const Lane l = scan_lane<VEC>(s, WT, lengths);
+    const Lane l = scan_lane<VEC, (PIECE < 0)>(s, WT, lengths);
     const int seg = blockIdx.y;  // the fold went through the segments in this order too, each from its end
     const int64_t first = seg * s.tiles_per_segment, last = min(s.tiles, first + s.tiles_per_segment);
     float mu[VEC];  // gradient of the state behind the tile
@@ -492,9 +523,9 @@ __global__ void __launch_bounds__(256, VEC == 2 ? kBwdCtas : 3) k_scan_bwd(const
             stages.values(tile, 1, v);
             stages.values(tile, 2, g);
         } else {
-            load_packs<T, VEC, STEPS>(z + l.b * s.zsb + l.d + t0 * s.zst, s.zst, full, left, a);
-            load_packs<T, VEC, STEPS>(x + l.b * s.xsb + l.d + t0 * s.xst, s.xst, full, left, v);
-            load_packs<T, VEC, STEPS>(gh + l.b * s.gsb + l.d + t0 * s.gst, s.gst, full && gh != nullptr, gh != nullptr ? left : 0, g);
+            load_packs<T, VEC, STEPS, (PIECE < 0)>(z + l.b * s.zsb + l.d + t0 * s.zst, s.zst, full, left, a);
+            load_packs<T, VEC, STEPS, (PIECE < 0)>(x + l.b * s.xsb + l.d + t0 * s.xst, s.xst, full, left, v);
+            load_packs<T, VEC, STEPS, (PIECE < 0)>(gh + l.b * s.gsb + l.d + t0 * s.gst, s.gst, full && gh != nullptr, gh != nullptr ? left : 0, g);
         }
 #pragma unroll
         for (int k = 0; k < VEC; ++k) {
@@ -566,8 +597,8 @@ __global__ void __launch_bounds__(256, VEC == 2 ? kBwdCtas : 3) k_scan_bwd(const
 #pragma unroll
             for (int k = 0; k < VEC; ++k) mu[k] = m[k];
         const int64_t rest = l.in ? s.T - t0 : 0;
-        store_packs<T, VEC, STEPS>(dx + l.b * s.dxb + l.d + t0 * s.dxt, s.dxt, full, rest, g);
-        store_packs<T, VEC, STEPS>(dz + l.b * s.dzb + l.d + t0 * s.dzt, s.dzt, full, rest, v);
+        store_packs<T, VEC, STEPS, (PIECE < 0)>(dx + l.b * s.dxb + l.d + t0 * s.dxt, s.dxt, full, rest, g);
+        store_packs<T, VEC, STEPS, (PIECE < 0)>(dz + l.b * s.dzb + l.d + t0 * s.dzt, s.dzt, full, rest, v);
     }
     if (seg == 0 && l.wt == 0 && l.in && dh0 != nullptr)
 #pragma unroll
@@ -599,6 +630,16 @@ static ScanDims scan_dims(int64_t B, int64_t T, int64_t D, int ctas_per_sm) {
     s.tiles_per_segment = s.tiles > 0 ? (s.tiles + segments - 1) / segments : 0;
     s.segments = s.tiles > 0 ? (int)((s.tiles + s.tiles_per_segment - 1) / s.tiles_per_segment) : 1;
     return s;
+}
+
+static unsigned scan_ctas(const ScanDims &s, int vec) {
+    const int64_t lanes = s.B * ((s.D + vec - 1) / vec);
+    return (unsigned)((lanes + 32 * s.WC - 1) / (32 * s.WC));
+}
+
+static int64_t scan_waves(const ScanDims &s, int vec, int per_sm) {
+    const int64_t ctas = (int64_t)scan_ctas(s, vec) * s.segments, slots = (int64_t)per_sm * num_sms();
+    return (ctas + slots - 1) / slots;
 }
 
 // `n` neighbouring channels as one access: a number of features, strides and addresses that keep every pack aligned.
@@ -652,8 +693,16 @@ int allow_smem(K kernel, size_t bytes) {
     return (int)e;
 }
 
-// What a lane takes of the channels, one or a pair, and the bytes of the pieces that are fetched ahead where a CTA walks several tiles
-// (0: direct loads).
+// What a lane can take of the channels in one access, one or a pair, and the bytes of the pieces that are fetched ahead where a CTA walks
+// several tiles (0: direct loads).
+//
+// Direct loads leave a choice between one channel and a pair a lane, made by the waves of CTAs that the device runs: a wave of pairs
+// takes 1.25 (forward) and 13/9 (backward) as long as one of single channels, and holds 1.5 and 1.33 as many channels.  Forward, one
+// channel even where pairs are aligned: [64, 2048, 254] fp32 0.086 ms against 0.097, bf16 0.079 against 0.087 (1 wave each),
+// [96, 1999, 322] fp16 0.145 against 0.191 (2 each); pairs: [100, 2048, 254] fp32 0.123 against 0.142 (1 and 2), [8192, 256, 46] bf16
+// 0.174 against 0.199.  Backward, pairs by single accesses where rows or addresses are odd: [64, 2048, 255] fp32 0.138 against 0.177,
+// bf16 0.144 against 0.194 (1 and 2), [96, 1999, 321] fp16 0.284 against 0.303 (2 and 3); one channel: [8192, 256, 47] bf16 0.386 against
+// 0.425, [32768, 64, 9] fp32 0.092 against 0.139.
 struct ScanAccess {
     int vec, piece;
 };
@@ -661,7 +710,7 @@ struct ScanAccess {
 template <typename T, int VEC, int PIECE>
 int scan_fwd(const ScanDims &s, const void *x, const void *z, const float *h0, const int32_t *lengths, void *h, float *h_last, float *states,
              float2 *agg, cudaStream_t st) {
-    const dim3 grid((unsigned)((s.channels + 32 * VEC * s.WC - 1) / (32 * VEC * s.WC)), (unsigned)s.segments);
+    const dim3 grid(scan_ctas(s, VEC), (unsigned)s.segments);
     const unsigned threads = 32 * s.WT * s.WC;
     const T *px = (const T *)x, *pz = (const T *)z;
     T *ph = (T *)h;
@@ -688,7 +737,7 @@ int scan_fwd(const ScanDims &s, const void *x, const void *z, const float *h0, c
 template <typename T, int VEC, int PIECE>
 int scan_bwd(const ScanDims &s, const void *gh, const void *x, const void *z, const float *h0, const int32_t *lengths, const float *states,
              const float *g_last, void *dx, void *dz, float *dh0, float2 *agg, cudaStream_t st) {
-    const dim3 grid((unsigned)((s.channels + 32 * VEC * s.WC - 1) / (32 * VEC * s.WC)), (unsigned)s.segments);
+    const dim3 grid(scan_ctas(s, VEC), (unsigned)s.segments);
     const unsigned threads = 32 * s.WT * s.WC;
     const T *pg = (const T *)gh, *px = (const T *)x, *pz = (const T *)z;
     T *pdx = (T *)dx, *pdz = (T *)dz;
@@ -706,9 +755,9 @@ int scan_bwd(const ScanDims &s, const void *gh, const void *x, const void *z, co
         if (int e = allow_smem(bwd, bytes)) return e;
         bwd<<<grid, threads, bytes, st>>>(pg, px, pz, h0, lengths, states, g_last, s, agg, pdx, pdz, dh0);
     } else if (s.T == 1) {
-        k_scan_bwd<T, VEC, 1, 1, 0><<<grid, threads, 0, st>>>(pg, px, pz, h0, lengths, states, g_last, s, agg, pdx, pdz, dh0);
+        k_scan_bwd<T, VEC, 1, 1, (PIECE < 0 ? PIECE : 0)><<<grid, threads, 0, st>>>(pg, px, pz, h0, lengths, states, g_last, s, agg, pdx, pdz, dh0);
     } else {
-        k_scan_bwd<T, VEC, kScanSteps, 0, 0><<<grid, threads, 0, st>>>(pg, px, pz, h0, lengths, states, g_last, s, agg, pdx, pdz, dh0);
+        k_scan_bwd<T, VEC, kScanSteps, 0, (PIECE < 0 ? PIECE : 0)><<<grid, threads, 0, st>>>(pg, px, pz, h0, lengths, states, g_last, s, agg, pdx, pdz, dh0);
     }
     return check_launch();
 }
@@ -726,7 +775,8 @@ int scan_fwd_by(ScanAccess how, const ScanDims &s, const void *x, const void *z,
                 float *h_last, float *states, float2 *agg, cudaStream_t st) {
     if (how.piece == 16) return scan_fwd<T, 2, 16>(s, x, z, h0, lengths, h, h_last, states, agg, st);
     if (how.piece == 8) return scan_fwd<T, 2, (sizeof(T) == 2 ? 8 : 0)>(s, x, z, h0, lengths, h, h_last, states, agg, st);
-    if (how.vec == 2) return scan_fwd<T, 2, 0>(s, x, z, h0, lengths, h, h_last, states, agg, st);
+    const bool one = s.tiles_per_segment > 1 && 4 * scan_waves(s, 1, kFwdCtas1) <= 5 * scan_waves(s, 2, kFwdCtas);
+    if (how.vec == 2 && !one) return scan_fwd<T, 2, 0>(s, x, z, h0, lengths, h, h_last, states, agg, st);
     return scan_fwd<T, 1, 0>(s, x, z, h0, lengths, h, h_last, states, agg, st);
 }
 
@@ -735,6 +785,8 @@ int scan_bwd_by(ScanAccess how, const ScanDims &s, const void *gh, const void *x
                 const float *states, const float *g_last, void *dx, void *dz, float *dh0, float2 *agg, cudaStream_t st) {
     if (how.piece == 16) return scan_bwd<T, 2, 16>(s, gh, x, z, h0, lengths, states, g_last, dx, dz, dh0, agg, st);
     if (how.piece == 8) return scan_bwd<T, 2, (sizeof(T) == 2 ? 8 : 0)>(s, gh, x, z, h0, lengths, states, g_last, dx, dz, dh0, agg, st);
+    if (how.vec == 1 && s.D > 1 && 13 * scan_waves(s, 2, kBwdCtas) < 9 * scan_waves(s, 1, kBwdCtas1))
+        return scan_bwd<T, 2, -1>(s, gh, x, z, h0, lengths, states, g_last, dx, dz, dh0, agg, st);
     if (how.vec == 2) return scan_bwd<T, 2, 0>(s, gh, x, z, h0, lengths, states, g_last, dx, dz, dh0, agg, st);
     return scan_bwd<T, 1, 0>(s, gh, x, z, h0, lengths, states, g_last, dx, dz, dh0, agg, st);
 }

@@ -105,6 +105,41 @@ def test_forward_and_backward(index, dtype, padded):
     assert all(torch.equal(a, b) for a, b in zip((dx, dz), K.gated_scan_bwd(gh, x, z, h0, lengths, states, g_last)))
 
 
+ROWS = [(5, T, D) for T in (1, 3, 70, 900) for D in (7, 9, 10, 11, 63, 65, 127)]
+# as many channels as fill the chip a little more than once with one of them a lane, for each number of warps along time
+ROWS += [(B, T, D) for B, T in ((1000, 1), (500, 10), (250, 30), (125, 64), (125, 200)) for D in (130, 131)] + [(100, 200, 254)]
+
+
+@gpu
+@pytest.mark.parametrize('dtype', list(HALF_STEP), ids=str)
+@pytest.mark.parametrize('inside', [True, False])
+@pytest.mark.parametrize('shape', ROWS, ids=lambda s: 'x'.join(map(str, s)))
+def test_rows_that_pairs_do_not_fit(shape, inside, dtype):
+    """A row's last feature alone, or (with an odd base, inside a wider tensor) every pair across an access boundary."""
+    from hgq2_b200 import kernels as K
+
+    B, T, D = shape
+    x, z, gh, h0, g_last = inputs((B, T, D), dtype, D)
+    lengths = torch.tensor([T, 0, T // 2, T, 1] * (B // 5), device='cuda')
+    out = None
+    if inside:
+        wide = torch.full((B, T, 2 * D + 3), 7.0, device='cuda', dtype=dtype)
+        wide[..., 1:D + 1], wide[..., D + 2:-1] = x, z
+        x, z = wide[..., 1:D + 1], wide[..., D + 2:-1]
+        out = torch.full_like(wide, 7.0)
+    want = reference(x, z, h0, lengths, gh, g_last)
+    h, h_last, states = K.gated_scan_fwd(x, z, h0, lengths, want_states=True)
+    close(h, want['h'], want['size'], dtype, 40, 'h')
+    close(h_last, want['h_last'], want['size_last'], torch.float32, 40, 'h_last')
+    into = {'out_dx': out[..., 1:D + 1], 'out_dz': out[..., D + 2:-1]} if inside else {}
+    dx, dz, dh0 = K.gated_scan_bwd(gh, x, z, h0, lengths, states, g_last, want_dh0=True, **into)
+    close(dx, want['dx'], want['size_dx'], dtype, 80, 'dx')
+    close(dz, want['dz'], want['size_dz'], dtype, 160, 'dz')
+    close(dh0, want['dh0'], want['size_dh0'], torch.float32, 80, 'dh0')
+    if inside:
+        assert bool((out[..., [0, D + 1, -1]] == 7).all())
+
+
 @gpu
 @pytest.mark.parametrize('dtype', list(HALF_STEP), ids=str)
 def test_tokens_one_by_one_equal_the_sequence(dtype):
