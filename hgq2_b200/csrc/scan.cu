@@ -72,7 +72,7 @@ struct Lane {
 };
 
 // IN_ROWS: lanes do not cross batch rows, for an odd number of features (a kernel's own variant: the arithmetic costs the short
-// sequences 0.005 ms of 0.074).  A pair left half empty by the row's end becomes the row's last two channels, one of them its
+// sequences 0.006 to 0.008 ms of 0.075).  A pair left half empty by the row's end becomes the row's last two channels, one of them its
 // neighbour's too (both compute and write the same bits).
 template <int VEC, bool IN_ROWS = false>
 __device__ __forceinline__ Lane scan_lane(const ScanDims &s, int WT, const int32_t *lengths) {
