@@ -1,6 +1,7 @@
 // AdamW over a list of tensors in one launch, states in 32 bits or in 8.
 //
-//   g' = (g grad_scale + l1) c,  c = min(clipnorm / |g grad_scale + l1|_2, 1) over ALL tensors (1 without clipping)
+//   g' = (g grad_scale + l1) c,  c = min(clipnorm / |g grad_scale + l1|_2, 1) over ALL tensors (1 without clipping; NaN if the norm is
+//        not finite)
 //   m  = b1 m + (1 - b1) g';  v = b2 v + (1 - b2) g'^2;  alpha = lr sqrt(1 - b2^t) / (1 - b1^t)
 //   w  = clamp(w (1 - lr decay) - alpha m / (sqrt(v) + eps), lo, hi)
 //
@@ -413,8 +414,9 @@ __global__ void __launch_bounds__(kAdamWarps * 32, BITS == 32 ? kAdamCtas32 : kA
         if (a.clipnorm > 0.0) {
             double s = 0.0;
             for (int w = 0; w < kAdamWarps; ++w) s += red[w];
-            const double c = a.clipnorm / sqrt(s);
-            s_coef = (float)(c > 1.0 ? 1.0 : c);  // a NaN norm stays NaN and reaches every weight
+            const double norm = sqrt(s), c = a.clipnorm / norm;
+            // + 0, or NaN where the norm is infinite or NaN: it reaches every weight (1 / infinity would drop the finite gradients)
+            s_coef = (float)((c > 1.0 ? 1.0 : c) + (norm - norm));
         } else {
             s_coef = 1.f;
         }

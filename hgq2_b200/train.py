@@ -153,8 +153,8 @@ class FusedAdamW:
     tensors are updated through an fp32 copy that the optimizer keeps (``masters``); the tensor gets its rounded value.
 
     The rule is Keras' AdamW: ``w`` is first scaled by ``1 - learning_rate * weight_decay``, then takes Adam's step;
-    ``global_clipnorm`` scales all gradients so that their common 2-norm is at most that (a norm that is not finite reaches
-    every weight, as in Keras).  ``weight_decay`` is one number, or one per tensor (0 for biases and bitwidths, say).
+    ``global_clipnorm`` scales all gradients so that their common 2-norm is at most that (a norm that is infinite or NaN makes
+    every weight with a gradient NaN, as in Keras).  ``weight_decay`` is one number, or one per tensor (0 for biases and bitwidths, say).
 
     ``state_bits=8`` keeps the moments as e4m3 codes with an fp32 scale per 256 elements of a tensor: ``m`` (times ``m_scale``)
     and ``r`` (times ``r_scale``), the root of the second moment -- 2 bytes per weight instead of 8.  ``state_bits=32`` keeps

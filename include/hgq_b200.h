@@ -442,7 +442,8 @@ typedef struct {
 /*
  * One step over all tensors of a list.  Stands in for keras.optimizers.AdamW with global_clipnorm (Keras, not HGQ2, owns it)
  * followed by the variables' constraints, like hgq_adam_step does for Adam on one flat bucket.
- *   g' = (g grad_scale + l1) c,  c = min(clipnorm / |g grad_scale + l1| over all tensors, 1), or 1 if clipnorm <= 0
+ *   g' = (g grad_scale + l1) c,  c = min(clipnorm / |g grad_scale + l1| over all tensors, 1), or 1 if clipnorm <= 0; a norm that is
+ *   infinite or NaN makes c NaN
  *   m = b1 m + (1 - b1) g';  v = b2 v + (1 - b2) g'^2;  alpha = lr sqrt(1 - b2^t) / (1 - b1^t)
  *   w = clamp(w (1 - lr decay) - alpha m / (sqrt(v) + eps), lo, hi)
  * chunks: DEVICE array of (tensor, chunk of that tensor) pairs of int32, the tensors in order, ceil(n / 2048) each; first_chunk:

@@ -471,3 +471,40 @@ def test_trainer_captured_equals_eager(bits):
     assert int(cap.opt.step_count) == int(eager.opt.step_count) == 5
     assert torch.equal(eager.state.params, cap.state.params)
     assert bool(torch.isfinite(cap.state.params).all())
+
+
+@gpu
+@pytest.mark.parametrize('bits', [32, 8])
+@pytest.mark.parametrize('value,scale', [(float('inf'), 1.0), (-float('inf'), 1.0), (3e38, 4.0)])
+def test_infinite_norm_reaches_every_weight(bits, value, scale):
+    """One infinite gradient among finite ones, no NaN: Keras adds norm - norm to the clipping factor, which makes it NaN for an
+    infinite norm too.  A gradient that overflows only when it is scaled counts as infinite."""
+    from hgq2_b200.train import FusedAdamW
+
+    ws = [torch.ones(n, device='cuda') for n in (600, 300, 64)]
+    gs = [torch.ones_like(w) for w in ws]
+    gs[1][7] = value
+    kept = ws[2].clone()
+    opt = FusedAdamW(ws, state_bits=bits, global_clipnorm=1.0)
+    opt.step([gs[0], gs[1], None], grad_scale=scale)
+    for i in range(2):
+        assert bool(torch.isnan(ws[i]).all()), i
+        m, v = opt.moments(i)
+        assert bool(torch.isnan(m).all() and torch.isnan(v).all()), i
+    assert torch.equal(ws[2], kept)  # no gradient: left as it is
+
+
+@gpu
+@pytest.mark.parametrize('bits', [32, 8])
+def test_large_finite_norm_clips(bits):
+    """Gradients whose squares fp32 does not hold: their norm is finite in fp64 and scales them as any other does."""
+    from hgq2_b200.train import FusedAdamW
+
+    n = 1000
+    w = torch.ones(n, device='cuda')
+    g = torch.full((n,), 1e36, device='cuda')
+    before = w.double()
+    FusedAdamW([w], learning_rate=LR, weight_decay=0.0, global_clipnorm=1.0, state_bits=bits).step([g])
+    zero = torch.zeros(n, device='cuda', dtype=torch.float64)
+    want, off = want_step(before, g.double(), zero, zero, 1, 0.0, 1.0, 0.0, 1.0, float(torch.linalg.vector_norm(g.double())))
+    assert bool(((w.double() - want[0]).abs() <= off[0] + 1e-30).all())
