@@ -6,6 +6,7 @@ These functions are the seam between the Python mirror of the reference interfac
 
 from __future__ import annotations
 
+import threading
 from array import array
 from contextlib import nullcontext
 from operator import attrgetter
@@ -17,12 +18,19 @@ from ._lib import FLAG_ABSMAX_ACCUMULATE, FLAG_TRAINING, FLAG_ZERO_NONPOS, OVERF
 
 ELEMENT_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}  # HGQ_TYPE_*
 
-_workspaces: dict[tuple[int, int, int], torch.Tensor] = {}
+
+class _Workspaces(threading.local):
+    def __init__(self):
+        self.buffers: dict[tuple[int, int, int], torch.Tensor] = {}
+
+
+_workspaces = _Workspaces()
 
 
 def workspace(nbytes: int, device: torch.device, slot: int = 0) -> torch.Tensor | None:
-    """A scratch buffer that only ever grows (kept so steady-state steps allocate nothing), one per device, purpose
-    (``slot``) and stream: kernels queued on different streams may run at the same time and must not share scratch."""
+    """A scratch buffer that only ever grows (kept so steady-state steps allocate nothing), one per host thread, device, purpose
+    (``slot``) and stream: kernels queued on different streams may run at the same time and must not share scratch, nor may calls
+    of several launches from different threads, whose launches can interleave on one stream."""
     if nbytes <= 0:
         return None
     if torch.cuda.is_current_stream_capturing():
@@ -33,10 +41,11 @@ def workspace(nbytes: int, device: torch.device, slot: int = 0) -> torch.Tensor 
         return torch.empty(nbytes, dtype=torch.uint8, device=device)
     dev = device.index if device.index is not None else torch.cuda.current_device()
     key = (dev, slot, torch._C._cuda_getCurrentRawStream(dev))
-    ws = _workspaces.get(key)
+    buffers = _workspaces.buffers
+    ws = buffers.get(key)
     if ws is None or ws.numel() < nbytes:
         ws = torch.empty(max(nbytes, 1 << 20), dtype=torch.uint8, device=device)
-        _workspaces[key] = ws
+        buffers[key] = ws
     return ws
 
 
