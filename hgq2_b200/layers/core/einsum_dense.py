@@ -149,11 +149,13 @@ class QEinsumDense(QLayerBaseSingleInput):
         """The parameter-only part of a call: (quantised kernel, quantised bias)."""
         return self.kq(self._kernel.value), (self.bq(self._bias.value) if self.bias is not None else None)
 
-    def call(self, inputs, training=None):
+    def call(self, inputs, training=None, output_shape=None):
+        """``output_shape`` (without the batch axis): of a call whose free axes are not those that the layer is built for; the
+        caller knows that no bitwidth depends on them."""
         qkernel, qbias = take_prepared(self) or self.prepare_params()
-        return self._contract(inputs, qkernel, qbias, training, apply_iq=True)
+        return self._contract(inputs, qkernel, qbias, training, apply_iq=True, output_shape=output_shape)
 
-    def _contract(self, inputs, qkernel, qbias, training, apply_iq: bool):
+    def _contract(self, inputs, qkernel, qbias, training, apply_iq: bool, output_shape=None):
         """act(einsum(eq, iq(x), qkernel) + qbias): the fused tensor-core kernel when the equation is a plain matrix
         product, the library einsum otherwise.  ``apply_iq=False``: ``inputs`` are already quantised."""
         if self._matmul_form is not None:
@@ -163,7 +165,7 @@ class QEinsumDense(QLayerBaseSingleInput):
                 qb = qbias.reshape((1,) * (len(kfree_shape) - qbias.dim()) + tuple(qbias.shape)).expand(kfree_shape).reshape(N)
             y = fused_dense_call(self, inputs, n_con, qkernel.reshape(K, N), qb, training, apply_iq=apply_iq)
             if y is not None:
-                return y.reshape((inputs.shape[0],) + tuple(self.full_output_shape[1:]))
+                return y.reshape((inputs.shape[0],) + tuple(self.full_output_shape[1:] if output_shape is None else output_shape))
         routes.fallback('torch.einsum', f'QEinsumDense {self.name} "{self.equation}"')
         if self.enable_iq and apply_iq:
             inputs = self.iq(inputs, training=training)
@@ -187,7 +189,8 @@ class QEinsumDense(QLayerBaseSingleInput):
         a = bw_inp.permute(in_perm).reshape(-1, K)
         b = bw_ker.permute(ker_perm).reshape(K, -1)
         bw_bias = self.bq.bits_(tuple(self._bias.shape)).reshape(-1) if self.bq is not None else None
-        size = float(prod(int(d) for d in self.full_output_shape[1:]))
+        dims = dict(zip(ker, self._kernel.shape)) | dict(zip(inp, shape))  # of this call
+        size = float(prod(int(dims[c]) for c in self.equation.split('->')[1][1:]))
         return EbopsDenseFn.apply(a, b, bw_bias, size, self.parallelization_factor / self.n_parallel)
 
     def get_config(self):

@@ -91,11 +91,7 @@ class QGatedRecurrence(QLayerBase):
             if k is not None and len(k.shape) == 3 and k.shape[1] != 1:
                 raise ValueError(f'{q.name} has a bitwidth per step: {self.name} runs on the {built[1]} steps it is built for; make '
                                  'the time axis homogeneous (homogeneous_axis=(0, 1)) to run on others')
-        proj.full_output_shape = (built[0], steps, *built[2:])
-        try:
-            return proj(inputs, training=training)
-        finally:
-            proj.full_output_shape = built
+        return proj(inputs, training=training, output_shape=(steps, *built[2:]))
 
     def call(self, inputs, initial_state=None, lengths=None, training=None):
         h, state = GatedScanFn.apply(self._project(inputs, training), initial_state, lengths)

@@ -98,3 +98,51 @@ def test_threads_on_one_stream_do_not_meet():
             torch.cuda.synchronize()
             for outs in got:
                 assert all(torch.equal(a, b) for a, b in zip(outs, expected)), make.__name__
+
+
+@gpu
+def test_one_layer_serves_two_lengths_at_once():
+    """Two threads inside the projection of one recurrence layer, the first to come leaving before the second: each gets the
+    shape of its own call, and the layer keeps the one it is built for."""
+    from hgq2_b200.config import QuantizerConfigScope
+    from hgq2_b200.layers import QGatedRecurrence
+    from hgq2_b200.quantizer import QuantizerConfig
+
+    with QuantizerConfigScope(place='datalane', default_q_type='kif', overflow_mode='WRAP', i0=4, f0=8):
+        conf = QuantizerConfig(place='datalane', homogeneous_axis=(0, 1))
+    layer = QGatedRecurrence(8, iq_conf=conf, return_state=True)
+    x = torch.randn(2, 30, 6, device='cuda')
+    layer(x)
+    proj = layer.projection
+    want = [layer(x[:, :n], training=False)[0] for n in (7, 12, 30)]
+    prepare, first_in, second_in, first_out = proj.prepare_params, threading.Event(), threading.Event(), threading.Event()
+
+    def paused():
+        if not first_in.is_set():
+            first_in.set()
+            assert second_in.wait(60)
+        elif not second_in.is_set():
+            second_in.set()
+            assert first_out.wait(60)
+        return prepare()
+
+    proj.prepare_params = paused
+
+    def first():
+        try:
+            return layer(x[:, :7], training=False)[0]
+        finally:
+            first_out.set()
+
+    def second():
+        assert first_in.wait(60)
+        try:
+            return layer(x[:, :12], training=False)[0]
+        finally:
+            second_in.set()
+
+    got = in_threads(first, second)
+    del proj.prepare_params
+    torch.cuda.synchronize()
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    assert torch.equal(layer(x, training=False)[0], want[2])
