@@ -784,7 +784,9 @@ class Engine:
         return h_q, h_d
 
     def covers(self, variable) -> None:
-        """A node's word that its backward pass writes the gradient of ``variable`` into the flat bucket."""
+        """A node's word that its backward pass writes the gradient of ``variable`` into the flat bucket (writes, not adds: one
+        node a variable)."""
+        _require(all(v is not variable for v in self._float_variables), f'{variable.path}: one layer used in two places')
         self._float_variables.append(variable)
 
     def new_ebops_term(self) -> int:

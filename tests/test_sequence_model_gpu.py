@@ -305,3 +305,39 @@ def test_second_derivatives_are_refused():
         (g,) = torch.autograd.grad(layer(x, training=True).square().sum(), x, create_graph=True)
         with pytest.raises(RuntimeError):
             g.square().sum().backward()
+
+
+def shared_norm_model(T=24):
+    """One normalisation that stands in two places of the model."""
+    from hgq2_b200 import workloads as W
+    from hgq2_b200.backend import Sequential
+    from hgq2_b200.layers import GroupNormalization, QDense, QEinsumDense, QGatedRecurrence
+
+    w, a, l = W._scopes(4, 8, 1e-5)
+    with w, a, l:
+        norm = GroupNormalization(4, activation='silu')
+        layers = W._seeded([QEinsumDense('abc,cd->abd', (T, 32), bias_axes='d'), norm, QEinsumDense('abc,cd->abd', (T, 32), bias_axes='d'),
+                            norm, QGatedRecurrence(16, return_sequences=False), QDense(5)])
+    model = Sequential(layers, name='shared_norm_model')
+    model.input_shape, model.weight_bits = (T, 12), (5, 8)
+    return W.build(model)
+
+
+@gpu
+def test_a_normalisation_in_two_places_gets_both_gradients():
+    """The step plan writes a variable's gradient once; a model that uses it twice takes the autograd path, which adds them up."""
+    from hgq2_b200.engine import Unsupported
+
+    runs = []
+    for engine in (None, False):
+        tr = trainer(shared_norm_model(), engine)
+        assert tr.engine is None and (engine is False or 'two places' in tr.engine_refusal)
+        x, y = batch(tr.model)
+        _, loss = tr.forward_backward(x, y)
+        runs.append((loss, [v.value.grad.clone() for v in tr.state.variables], [v.path for v in tr.state.variables]))
+    assert sum(p.endswith('gamma') for p in runs[0][2]) == 1
+    close(runs[0][0], runs[1][0], 1e-6, 'loss')
+    for g, want, path in zip(runs[0][1], runs[1][1], runs[0][2]):
+        close(g, want, 1e-5 if g.numel() > 64 else 2e-3, f'gradient {path}')
+    with pytest.raises(Unsupported, match='two places'):
+        trainer(shared_norm_model(), True)
