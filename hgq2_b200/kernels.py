@@ -12,6 +12,7 @@ from contextlib import nullcontext
 from operator import attrgetter
 
 import torch
+from torch.autograd.graph import increment_version
 
 from . import _lib
 from ._lib import FLAG_ABSMAX_ACCUMULATE, FLAG_TRAINING, FLAG_ZERO_NONPOS, OVERFLOW_MODES, ROUND_MODES, check, lib, ptr, require_cuda, stream_handle
@@ -727,6 +728,8 @@ def adamw_step(opt, grads, grad_scale: float = 1.0) -> None:
             opt.lr, opt.b1, opt.b2, opt.eps, grad_scale, clip, ptr(opt.step_count), ptr(opt._ticket), ptr(ws),
             ws.numel() if ws is not None else 0, stream_handle())
     check(st, 'hgq_adamw_step')
+    # written behind autograd's back: a backward pass through a graph that saved a weight before this step has to raise
+    increment_version(opt._leaves if len(present) == n else [w for w, g in zip(opt._leaves, grads) if g is not None])
 
 
 ACTIVATIONS = {None: 0, 'relu': 1, 'silu': 2, 'gelu': 3}  # HGQ_ACT_*

@@ -179,8 +179,8 @@ class FusedAdamW:
             raise ValueError(f'{len(decays)} weight decays for {len(items)} tensors')
         self.lr, self.b1, self.b2, self.eps = learning_rate, beta_1, beta_2, epsilon
         self.global_clipnorm, self.state_bits = global_clipnorm, state_bits
-        self._items = items
         self.tensors = [v.value.data if isinstance(v, Variable) else v.detach() for v in items]
+        self._leaves = [v.value if isinstance(v, Variable) else v for v in items]
         dev = self.tensors[0].device
         _lib.require_cuda(*self.tensors)
         spans = []
@@ -234,7 +234,7 @@ class FusedAdamW:
         """One update.  ``grads``: one tensor (fp32, bf16 or fp16, of the parameter's shape) or None per parameter, None leaving
         that parameter and its moments as they are; by default the ``.grad`` of each."""
         if grads is None:
-            grads = [v.value.grad if isinstance(v, Variable) else v.grad for v in self._items]
+            grads = [w.grad for w in self._leaves]
         kernels.adamw_step(self, grads, grad_scale)
 
     def sync_masters(self) -> None:

@@ -508,3 +508,24 @@ def test_large_finite_norm_clips(bits):
     zero = torch.zeros(n, device='cuda', dtype=torch.float64)
     want, off = want_step(before, g.double(), zero, zero, 1, 0.0, 1.0, 0.0, 1.0, float(torch.linalg.vector_norm(g.double())))
     assert bool(((w.double() - want[0]).abs() <= off[0] + 1e-30).all())
+
+
+@gpu
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+def test_autograd_sees_the_update(dtype):
+    """A backward pass through a graph that was recorded before the step raises, as with torch's optimizers: the weights that it
+    saved are gone.  A tensor without a gradient is not touched, and its graph stays usable."""
+    from hgq2_b200.backend import Variable
+    from hgq2_b200.train import FusedAdamW
+
+    ps = [torch.nn.Parameter(torch.randn(50, device='cuda').to(dtype)) for _ in range(2)]
+    items = [*ps, Variable(torch.randn(50, device='cuda'), 'v', True, 'float32', None, None)] if dtype == torch.float32 else ps
+    leaves = [v.value if isinstance(v, Variable) else v for v in items]
+    opt = FusedAdamW(items)
+    values = [(p * p).sum() for p in leaves]
+    opt.step([None if i == 1 else torch.ones_like(p) for i, p in enumerate(leaves)])
+    values[1].backward()
+    for i, v in enumerate(values):
+        if i != 1:
+            with pytest.raises(RuntimeError, match='modified by an inplace operation'):
+                v.backward()
