@@ -436,8 +436,7 @@ __global__ void __launch_bounds__(kAdamWarps * 32, BITS == 32 ? kAdamCtas32 : kA
             T.clamps = !(T.t.lo == -INFINITY && T.t.hi == INFINITY);
             T.scales = a.clipnorm > 0.0 || a.grad_scale != 1.f || T.t.l1 != 0.f;
             uintptr_t bits = (uintptr_t)T.t.master;
-            if (T.t.master != nullptr) bits |= (uintptr_t)T.t.w << 1;  // 8-byte groups of the 16-bit copy
-            else bits |= (uintptr_t)T.t.w;
+            bits |= T.t.master != nullptr && T.t.w_type != HGQ_TYPE_F32 ? (uintptr_t)T.t.w << 1 : (uintptr_t)T.t.w;  // 16-bit copy: groups of 8 bytes
             bits |= T.gtype == HGQ_TYPE_F32 ? (uintptr_t)T.g : (uintptr_t)T.g << 1;
             T.aligned = (bits & 15) == 0;
             T.wide_g = ((uintptr_t)T.g & 31) == 0;

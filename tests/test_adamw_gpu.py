@@ -529,3 +529,28 @@ def test_autograd_sees_the_update(dtype):
         if i != 1:
             with pytest.raises(RuntimeError, match='modified by an inplace operation'):
                 v.backward()
+
+
+@gpu
+@pytest.mark.parametrize('offset', [0, 1, 2, 3])
+def test_an_fp32_tensor_beside_an_fp32_master(offset):
+    """The C interface allows a master beside a tensor of any type: an fp32 one at an address that 16-byte accesses do not fit
+    gets the master's values all the same."""
+    from hgq2_b200 import _lib
+    from hgq2_b200.train import FusedAdamW
+
+    gen = torch.Generator(device='cuda').manual_seed(12)
+    n = 256 * 9 + 5
+    base = torch.zeros(n + 4, device='cuda')
+    w, g = base[offset:offset + n], torch.randn(n, device='cuda', generator=gen)
+    w.copy_(torch.randn(n, device='cuda', generator=gen))
+    master, plain = w.clone(), w.clone()
+    opt = FusedAdamW([w], learning_rate=LR)
+    table = _lib.AdamWTensor.from_buffer_copy(bytes(opt._table.cpu().numpy()))
+    table.master = master.data_ptr()
+    opt._table.copy_(torch.frombuffer(bytearray(table), dtype=torch.uint8))
+    other = FusedAdamW([plain], learning_rate=LR)
+    for o in (opt, other):
+        o.step([g])
+    assert torch.equal(w, plain) and torch.equal(master, plain)
+    assert not bool(base[:offset].any()) and not bool(base[offset + n:].any())
