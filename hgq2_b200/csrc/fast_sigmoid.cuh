@@ -4,9 +4,10 @@
 
 namespace hgq {
 
-// a = sigmoid(z) = 1 / (1 + e) with e = exp(-z), and c = 1 - a = e / (1 + e), each to full relative precision (c is not the
-// difference where a is near 1).  FULL (fp32 data): z is held in [-88, 100], where the two are 0 and 1; the exponential is
-// 2^(-z log2 e) with the rounding error of the product carried along, the reciprocal's error is one ulp.  Otherwise (bf16 and fp16
+// a = sigmoid(z) = 1 / (1 + e) with e = exp(-z), and c = 1 - a = e / (1 + e), each with a small relative error wherever it is a
+// normal number (c is not the difference where a is near 1).  FULL (fp32 data): at most 12 x 2^-24; z is held in [-88, 100], where the
+// two are 0 and 1; the exponential is 2^(-z log2 e) with what the product loses carried along: its rounding, and the part of log2 e
+// below fp32 (2e-8, which would be 18 x 2^-24 of e at |z| = 80); the reciprocal's error is one ulp.  Otherwise (bf16 and fp16
 // data): z has at most 11 bits and the outputs no more, the product's rounding (|z| 2^-24 of e) is far below both; a closed gate is
 // 2^-126.  A NaN stays.
 template <bool FULL>
@@ -16,7 +17,8 @@ __device__ __forceinline__ void sigmoid_pair(float z, float &a, float &c) {
         asm("max.NaN.f32 %0, %0, 0fC2B00000;" : "+f"(z));
         asm("min.NaN.f32 %0, %0, 0f42C80000;" : "+f"(z));
         const float t = z * -1.44269504088896341f;
-        const float lo = fmaf(z, -1.44269504088896341f, -t);
+        float lo = fmaf(z, -1.44269504088896341f, -t);
+        lo = fmaf(z, -1.925962991126e-8f, lo);
         asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(t));
         e = fmaf(e, lo * 0.693147180559945309f, e);
         asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + e));

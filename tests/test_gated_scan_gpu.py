@@ -377,3 +377,21 @@ def test_refusals_need_no_gpu():
     assert need > 0 and fwd(nbytes=need - 1) == -5 and bwd(ws=None) == -5
     assert fwd(B=0) == 0 and bwd(D=0) == 0
     assert L.hgq_gated_scan_workspace(4096, 64, 64) == 0 and L.hgq_gated_scan_states(4096, 64, 64) == 0
+
+
+@gpu
+def test_gates_to_relative_precision():
+    """fp32 gates and their complements over the range where both are normal numbers: one step from x = 0, h0 = 1 gives a, one
+    from x = 1, h0 = 0 gives c.  Counted in U = 2^-24: 2^x within 2 ulps (5 U), its correction (1), 1 + e (1), the reciprocal within an ulp
+    (3), the product (1), and where c = 1 - a another rounding: at most 12 U."""
+    from hgq2_b200 import kernels as K
+
+    n = 1 << 20
+    z = torch.linspace(-85, 85, n, device='cuda').view(1, 1, n)
+    zero, one = torch.zeros_like(z), torch.ones_like(z)
+    a = K.gated_scan_fwd(zero, z, one[:, 0])[0].double()
+    c = K.gated_scan_fwd(one, z, zero[:, 0])[0].double()
+    e = torch.exp(-z.double())
+    for got, want, what in ((a, 1 / (1 + e), 'a'), (c, e / (1 + e), 'c')):
+        off = ((got - want) / want).abs()
+        assert float(off.max()) <= 12 * U, f'{what}: {float(off.max()) / U:.1f} U at z = {float(z.view(-1)[off.argmax()]):.2f}'
