@@ -18,6 +18,7 @@ from . import _lib
 from ._lib import FLAG_ABSMAX_ACCUMULATE, FLAG_TRAINING, FLAG_ZERO_NONPOS, OVERFLOW_MODES, ROUND_MODES, check, lib, ptr, require_cuda, stream_handle
 
 ELEMENT_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}  # HGQ_TYPE_*
+INT32_MAX = 2 ** 31 - 1
 
 
 class _Workspaces(threading.local):
@@ -822,6 +823,8 @@ def _scan_args(x, z, h0, lengths):
     if lengths is not None:
         if lengths.shape != (B,) or lengths.is_floating_point() or lengths.dtype == torch.bool or lengths.device != x.device:
             raise ValueError(f'lengths must be {B} whole numbers on {x.device}')
+        if T > INT32_MAX and torch.iinfo(lengths.dtype).max > INT32_MAX:
+            raise ValueError(f'lengths of an axis of {T} steps must be int32 (or narrower), got {lengths.dtype}')
         if lengths.dtype != torch.int32:
             lengths = lengths.to(torch.int64).clamp(0, T).to(torch.int32)
         lengths = lengths.contiguous()

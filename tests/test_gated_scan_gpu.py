@@ -395,3 +395,17 @@ def test_gates_to_relative_precision():
     for got, want, what in ((a, 1 / (1 + e), 'a'), (c, e / (1 + e), 'c')):
         off = ((got - want) / want).abs()
         assert float(off.max()) <= 12 * U, f'{what}: {float(off.max()) / U:.1f} U at z = {float(z.view(-1)[off.argmax()]):.2f}'
+
+
+@gpu
+def test_lengths_that_32_bits_do_not_hold():
+    """Lengths travel as int32: an axis longer than that takes no wider ones (they would wrap), but narrower ones and none."""
+    from hgq2_b200 import kernels as K
+
+    T = 2 ** 31 + 8
+    x = torch.ones(1, 1, 1, device='cuda', dtype=torch.float16).expand(1, T, 1)
+    with pytest.raises(ValueError, match='int32'):
+        K.gated_scan_fwd(x, x, lengths=torch.tensor([2 ** 31 + 4], device='cuda'))
+    h0 = torch.full((1, 1), 3.0, device='cuda')
+    h, last, _ = K.gated_scan_fwd(x, x, h0, lengths=torch.zeros(1, dtype=torch.int32, device='cuda'))
+    assert torch.equal(last, h0) and not bool(h[:, -1000:].any()) and not bool(h[:, :1000].any())
