@@ -837,6 +837,24 @@ def _scan_state(h, B: int, D: int, device, what: str):
     return h.contiguous()
 
 
+def _rows_meet(t) -> bool:
+    """Whether two rows of a [batch, time, features] tensor whose features are contiguous share memory."""
+    B, T, D = t.shape
+    sb, st = t.stride()[:2]
+    if t.numel() == 0 or ((T == 1 or st >= D) and (B == 1 or sb >= (T - 1) * st + D)):
+        return False
+    if (T > 1 and st < D) or (B > 1 and sb < D):
+        return True
+    (step, n), (jump, m) = sorted(((sb, B), (st, T)))
+    for j in range(1, m):  # against the row a jump of j away: the nearest ones below and above it
+        i, rest = divmod(j * jump, step)
+        if i >= n:
+            break
+        if rest < D or (i + 1 < n and step - rest < D):
+            return True
+    return False
+
+
 def gated_scan_fwd(x, z, h0=None, lengths=None, want_states: bool = False):
     """h_t = a_t h_{t-1} + (1 - a_t) x_t, a_t = sigmoid(z_t), along axis 1 of x, z [batch, time, features] (fp32, bf16 or fp16; the
     state is fp32).  ``h0`` [batch, features] fp32; ``lengths`` [batch]: steps of each row of a padded batch (h is 0 behind them).
@@ -859,7 +877,7 @@ def gated_scan_fwd(x, z, h0=None, lengths=None, want_states: bool = False):
 def gated_scan_bwd(gh, x, z, h0=None, lengths=None, states=None, g_last=None, want_dh0: bool = False, out_dx=None,
                    out_dz=None):
     """Gradients of ``gated_scan_fwd`` from the gradients ``gh`` of h and ``g_last`` of h_last (None: zeros): (dx, dz, dh0 or None);
-    dx and dz go to ``out_dx`` / ``out_dz`` when given (like x, the features contiguous, any other strides)."""
+    dx and dz go to ``out_dx`` / ``out_dz`` when given (like x, the features contiguous, any other strides that keep rows apart)."""
     x, z, h0, lengths, kind, B, T, D = _scan_args(x, z, h0, lengths)
     require_cuda(gh, states, g_last)
     if gh is not None:
@@ -879,6 +897,8 @@ def gated_scan_bwd(gh, x, z, h0=None, lengths=None, states=None, g_last=None, wa
         for o in (out_dx, out_dz):
             if o is not None and (o.shape != x.shape or o.dtype != x.dtype or o.device != dev or (o.stride(2) != 1 and D > 1)):
                 raise ValueError(f'gradients go to {x.dtype} tensors of shape {tuple(x.shape)} on {dev} with contiguous features')
+            if o is not None and _rows_meet(o):
+                raise ValueError('rows of a tensor that gradients go to share memory')
         dx = torch.empty((B, T, D), dtype=x.dtype, device=dev) if out_dx is None else out_dx
         dz = torch.empty((B, T, D), dtype=x.dtype, device=dev) if out_dz is None else out_dz
         dh0 = torch.empty((B, D), dtype=torch.float32, device=dev) if want_dh0 else None

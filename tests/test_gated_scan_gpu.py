@@ -409,3 +409,39 @@ def test_lengths_that_32_bits_do_not_hold():
     h0 = torch.full((1, 1), 3.0, device='cuda')
     h, last, _ = K.gated_scan_fwd(x, x, h0, lengths=torch.zeros(1, dtype=torch.int32, device='cuda'))
     assert torch.equal(last, h0) and not bool(h[:, -1000:].any()) and not bool(h[:, :1000].any())
+
+
+@gpu
+def test_gradients_into_a_tensor_that_overlaps_itself():
+    """Steps or rows of an output that share memory would be written in no order: refused."""
+    from hgq2_b200 import kernels as K
+
+    x = torch.randn(2, 5, 8, device='cuda')
+    row = torch.zeros(2, 5, 8, device='cuda')
+    for out in (row[:, :1].expand(2, 5, 8), row[:1].expand(2, 5, 8), row.view(-1).as_strided((2, 5, 8), (40, 4, 1)),
+                row.view(-1).as_strided((2, 5, 8), (7, 16, 1)), row.view(-1).as_strided((2, 5, 8), (8, 8, 1)),
+                row.view(-1).as_strided((2, 5, 8), (20, 9, 1))):
+        for name in ('out_dx', 'out_dz'):
+            with pytest.raises(ValueError, match='share memory'):
+                K.gated_scan_bwd(x, x, x, **{name: out})
+    one = K.gated_scan_bwd(x[:1, :1], x[:1, :1], x[:1, :1], out_dx=row[:1, :1].as_strided((1, 1, 8), (0, 0, 1)))  # nothing to share
+    assert torch.equal(one[0], K.gated_scan_bwd(x[:1, :1], x[:1, :1], x[:1, :1])[0])
+    turned = torch.zeros(5, 2, 8, device='cuda').transpose(0, 1)  # time-major
+    assert torch.equal(K.gated_scan_bwd(x, x, x, out_dx=turned)[0], K.gated_scan_bwd(x, x, x)[0])
+    woven = torch.zeros(16, device='cuda').as_strided((2, 3, 2), (6, 4, 1))  # rows at 0, 4, 8 and 6, 10, 14
+    y = x[:, :3, :2]
+    assert torch.equal(K.gated_scan_bwd(y, y, y, out_dz=woven)[1], K.gated_scan_bwd(y, y, y)[1])
+
+
+def test_rows_that_meet_are_found():
+    """Against the set of places that the rows touch, over all small shapes and strides."""
+    import itertools
+
+    from hgq2_b200.kernels import _rows_meet
+
+    buf = torch.empty(200)
+    for B, T, D in itertools.product((1, 2, 3, 4), (1, 2, 3), (1, 2, 3)):
+        for sb, st in itertools.product(range(11), range(11)):
+            places = [b * sb + t * st + d for b in range(B) for t in range(T) for d in range(D)]
+            assert _rows_meet(buf.as_strided((B, T, D), (sb, st, 1))) == (len(set(places)) < len(places)), (B, T, D, sb, st)
+    assert not _rows_meet(torch.empty(0, 3, 4)) and not _rows_meet(torch.empty(2, 0, 4)) and not _rows_meet(torch.empty(2, 3, 0))
