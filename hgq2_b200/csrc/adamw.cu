@@ -479,7 +479,9 @@ extern "C" int hgq_adamw_step(const hgq_adamw_tensor *tensors, int64_t n_tensors
     if (state_bits != 32 && state_bits != 8) return HGQ_ERR_MODE;
     if (!tensors || !chunks || !first_chunk || !grads || !grad_types || !m || !v || !step || !ticket) return HGQ_ERR_NULL;
     if (state_bits == 8 && (!m_scale || !v_scale)) return HGQ_ERR_NULL;
-    if (!aligned(m, 32) || !aligned(v, 32) || !aligned(chunks, 8) || !aligned(tensors, 8) || !aligned(step, 8)) return HGQ_ERR_ALIGN;
+    if (!aligned(m, 32) || !aligned(v, 32) || !aligned(chunks, 8) || !aligned(tensors, 8) || !aligned(step, 8) || !aligned(m_scale, 4) ||
+        !aligned(v_scale, 4) || !aligned(ticket, 4))
+        return HGQ_ERR_ALIGN;
     if (n_tensors == 0) return HGQ_OK;
     for (int64_t i = 0; i < n_tensors; ++i) {
         if (first_chunk[i + 1] < first_chunk[i]) return HGQ_ERR_SIZE;

@@ -554,3 +554,21 @@ def test_an_fp32_tensor_beside_an_fp32_master(offset):
         o.step([g])
     assert torch.equal(w, plain) and torch.equal(master, plain)
     assert not bool(base[:offset].any()) and not bool(base[offset + n:].any())
+
+
+def test_c_entry_refuses_misaligned_scales_and_counters():
+    import ctypes
+
+    from hgq2_b200 import _lib, build
+
+    build.build()
+    L = _lib.lib()
+    first, grads = (ctypes.c_int64 * 2)(0, 1), (ctypes.c_uint64 * 1)(0)
+    p = 4096  # never dereferenced: every call below is refused on the host
+
+    def call(m_scale=p, v_scale=p, ticket=p, bits=8):
+        return L.hgq_adamw_step(p, 1, p, first, grads, bytes([0]), bits, p, p, m_scale, v_scale, 1e-3, 0.9, 0.999, 1e-7, 1.0, 0.0, p,
+                                ticket, None, 0, None)
+
+    assert call(m_scale=p + 2) == -4 and call(v_scale=p + 1) == -4
+    assert call(ticket=p + 2) == -4 and call(ticket=p + 2, bits=32) == -4
