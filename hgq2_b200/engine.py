@@ -745,9 +745,9 @@ class Engine:
             return _Dense(self, layer, in_shape), layer.compute_output_shape(in_shape)
         if isinstance(layer, QConv2D):
             return _Conv(self, layer, in_shape), layer.compute_output_shape(in_shape)
-        if isinstance(layer, GroupNormalization):
+        if type(layer) is GroupNormalization:
             return _GroupNorm(self, layer), in_shape
-        if isinstance(layer, QGatedRecurrence):
+        if type(layer) is QGatedRecurrence:
             _require(len(in_shape) == 3, 'recurrence input rank')
             return _GatedRecurrence(self, layer, in_shape), layer.compute_output_shape(in_shape)
         if isinstance(layer, MaxPooling2D):

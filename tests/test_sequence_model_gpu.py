@@ -341,3 +341,33 @@ def test_a_normalisation_in_two_places_gets_both_gradients():
         close(g, want, 1e-5 if g.numel() > 64 else 2e-3, f'gradient {path}')
     with pytest.raises(Unsupported, match='two places'):
         trainer(shared_norm_model(), True)
+
+
+@gpu
+def test_a_layer_of_ones_own_is_not_taken_for_its_parent():
+    """A subclass may compute something else: the step plan covers the two layers themselves only."""
+    from hgq2_b200 import workloads as W
+    from hgq2_b200.backend import Sequential
+    from hgq2_b200.layers import GroupNormalization, QDense, QEinsumDense, QGatedRecurrence
+
+    class Shifted(GroupNormalization):
+        def call(self, inputs):
+            return super().call(inputs) + 1.0
+
+    class Doubled(QGatedRecurrence):
+        def call(self, inputs, initial_state=None, lengths=None, training=None):
+            return 2.0 * super().call(inputs, initial_state, lengths, training)
+
+    for make in (lambda: Shifted(4), lambda: Doubled(32)):
+        runs = []
+        for engine in (None, False):
+            w, a, l = W._scopes(4, 8, 1e-5)
+            with w, a, l:
+                layers = W._seeded([QEinsumDense('abc,cd->abd', (24, 32), bias_axes='d'), make(), lambda x: x.mean(dim=1), QDense(5)])
+            model = Sequential(layers)
+            model.input_shape, model.weight_bits = (24, 12), (5, 8)
+            tr = trainer(W.build(model), engine)
+            assert tr.engine is None
+            x, y = batch(tr.model)
+            runs.append(tr.forward_backward(x, y)[0])
+        close(runs[0], runs[1], 1e-6, 'loss')
