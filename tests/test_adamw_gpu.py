@@ -572,3 +572,43 @@ def test_c_entry_refuses_misaligned_scales_and_counters():
 
     assert call(m_scale=p + 2) == -4 and call(v_scale=p + 1) == -4
     assert call(ticket=p + 2) == -4 and call(ticket=p + 2, bits=32) == -4
+
+
+@gpu
+@pytest.mark.parametrize('bits,clip', [(32, None), (32, 0.5), (8, None), (8, 0.5)])
+def test_states_past_32_bits(bits, clip):
+    """More than 2^31 elements: weights, moments, codes and scales at both ends, and the norm over all of them."""
+    from hgq2_b200.train import FusedAdamW
+
+    n, ends = 2 ** 31 + 777, 1024 + 9  # whole blocks of 256 from the tail's start, the last of them with 9 elements
+    w = torch.empty(n, device='cuda').normal_()
+    g = torch.empty(n, device='cuda', dtype=torch.bfloat16).normal_()
+    norm = 0.0
+    for piece in g.split(1 << 28):
+        norm += float(torch.linalg.vector_norm(piece, dtype=torch.float64)) ** 2
+    norm = math.sqrt(norm)
+    parts = [slice(0, 2048), slice(n - ends, n)]
+    assert (n - ends) % 256 == 0
+    before = [w[p].double() for p in parts]
+    opt = FusedAdamW([w], learning_rate=LR, weight_decay=0.0, state_bits=bits, global_clipnorm=clip)
+    opt.step([g])
+    for p, old in zip(parts, before):
+        zero = torch.zeros_like(old)
+        want, off = want_step(old, g[p].double(), zero, zero, 1, 0.0, 1.0, 0.0, clip, norm)
+        assert bool(((w[p].double() - want[0]).abs() <= off[0] + 1e-30).all())
+        if bits == 32:
+            assert bool(((opt.m[p].double() - want[1]).abs() <= off[1] + 1e-30).all())
+            assert bool(((opt.v[p].double() - want[2]).abs() <= off[2] + 1e-30).all())
+            continue
+        blocks = slice(p.start // 256, -(-p.stop // 256))
+        for codes, scales, x, root in ((opt.m, opt.m_scale, want[1], False), (opt.r, opt.r_scale, want[2].sqrt(), True)):
+            s = scales[blocks]
+            got = codes[p].double() * s.double().repeat_interleave(256)[:x.numel()]
+            grid = torch.maximum(x.abs() / 8, s.double().repeat_interleave(256)[:x.numel()] * 2.0 ** -9)
+            assert bool(((got - x).abs() <= grid * (1 + 1e-5) + 1e-6 * x.abs()).all())
+            if clip is None:  # to the bit; clipped moments are a rounded factor of the norm away from that
+                pad = torch.nn.functional.pad(g[p].float(), (0, -x.numel() % 256)).view(-1, 256)
+                exact = torch.sqrt((pad * pad) * (1.0 - B2)) if root else pad * (1.0 - B1)
+                place = torch.arange(blocks.start * 256, blocks.stop * 256, device='cuda').view(-1, 256)
+                code, top = reference_codes(exact, place, 1, root)
+                assert torch.equal(codes[p].float(), code.float().view(-1)[:x.numel()]) and torch.equal(s, top)

@@ -311,3 +311,27 @@ def test_refusals_need_no_gpu():
     assert L.hgq_group_norm_workspace(2, 3, 8, 2, 0, 1) > 0 and bwd(nbytes=4) == -5
     assert fwd(B=0) == 0 and fwd(S=0) == 0
     assert L.hgq_group_norm_workspace(2, 3, 8, 3, 0, 0) == 0
+
+
+@gpu
+@pytest.mark.parametrize('shape', [(16500, 2048, 64, 8), (3, 11300, 65536, 64)], ids=str)
+def test_parameter_gradients_past_32_bits(shape):
+    """dgamma and dbeta of the last group's channels over more than 2^31 elements."""
+    from hgq2_b200 import kernels as K
+
+    B, S, C, G = shape
+    x = torch.empty(B, S, C, device='cuda', dtype=torch.bfloat16).normal_()
+    assert x.numel() > 2 ** 31
+    _, mean, rstd = K.group_norm_fwd(x, None, None, G, 1e-3, 'silu')
+    none, dgamma, dbeta = K.group_norm_bwd(x, x, None, None, mean, rstd, G, 'silu', want_dx=False)
+    for gr in (slice(0, C // G), slice(C - C // G, C)):
+        totals = [torch.zeros(C // G, device='cuda', dtype=torch.float64) for _ in range(4)]
+        for part in x[:, :, gr].split(500):
+            want = reference(part, None, None, 1, 1e-3, 'silu', part)
+            for t, v in zip(totals, (*want['dgamma'], *want['dbeta'])):
+                t += v
+            del want
+        # the bound is for sums of a few hundred terms a thread; an image's thread adds up to 11300 / (148 * 2 / 32) = 1220 rows
+        more = 1 if S == 2048 else 4
+        for got, value, off in ((dgamma[gr], *totals[:2]), (dbeta[gr], *totals[2:])):
+            assert bool(((got.double() - value).abs() <= off * more + U * value.abs()).all())
