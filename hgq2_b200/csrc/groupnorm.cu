@@ -19,10 +19,6 @@
 
 namespace hgq {
 
-
-
-
-
 // ---- any shape: partial statistics, totals, application ---------------------------------------------------------------------
 // A CTA takes a run of rows of one sample and a tile of channels; a thread owns VEC neighbouring channels for all of its rows.
 

@@ -555,9 +555,11 @@ template <typename T, int VEC, int R>
 static int slab_fwd(const SlabPlan &p, const SlabArgs &a, const void *x, const float *gamma, const float *beta, void *y, float *mean, float *rstd,
                     float eps, int act, cudaStream_t st) {
     const int64_t ctas = p.workers * p.slabs * p.K;
-    constexpr bool can = Held<T, VEC, R>::kAhead;
-    const size_t smem = p.ahead ? Held<T, VEC, R>::kStageBytes : 0;
-#define SLAB_FWD(NG) (p.ahead ? k_gn_slab_fwd<T, VEC, R, NG, can> : k_gn_slab_fwd<T, VEC, R, NG, false>)
+    // 16-byte packs are always fetched ahead, but for the samples that two CTAs share: those fill the most packs a thread can hold
+    constexpr bool can = Held<T, VEC, R>::kAhead, always = can && R < (sizeof(T) == 2 ? 8 : 16);
+    const bool ahead = always || p.ahead;
+    const size_t smem = ahead ? Held<T, VEC, R>::kStageBytes : 0;
+#define SLAB_FWD(NG) (ahead ? k_gn_slab_fwd<T, VEC, R, NG, can> : k_gn_slab_fwd<T, VEC, R, NG, always>)
     auto kernel = SLAB_FWD(1);
     if (VEC > 1 && p.groups_of_pack == 2) kernel = SLAB_FWD((VEC > 1 ? 2 : 1));
     if (VEC > 4 && p.groups_of_pack == 4) kernel = SLAB_FWD((VEC > 4 ? 4 : VEC));
