@@ -724,7 +724,7 @@ def adamw_step(opt, grads, grad_scale: float = 1.0) -> None:
     with on_device(dev):
         ws = workspace(lib().hgq_adamw_workspace(n), dev, slot=7) if clip else None
         st = lib().hgq_adamw_step(
-            ptr(opt._table), n, ptr(opt._chunks), opt._first_chunk.ctypes.data, addresses.buffer_info()[0], types, opt.state_bits,
+            ptr(opt._table), n, ptr(opt._chunks), opt._first_chunk, addresses.buffer_info()[0], types, opt.state_bits,
             ptr(opt.m), ptr(opt.r if eight else opt.v), ptr(opt.m_scale) if eight else None, ptr(opt.r_scale) if eight else None,
             opt.lr, opt.b1, opt.b2, opt.eps, grad_scale, clip, ptr(opt.step_count), ptr(opt._ticket), ptr(ws),
             ws.numel() if ws is not None else 0, stream_handle())

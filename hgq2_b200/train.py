@@ -14,6 +14,7 @@ flat fp32 bucket:
 
 from __future__ import annotations
 
+import ctypes
 import math
 import os
 
@@ -206,7 +207,7 @@ class FusedAdamW:
         counts = [-(-n // _lib.ADAMW_CHUNK) for n in self._numels]
         first = np.zeros(len(items) + 1, dtype=np.int64)
         np.cumsum(counts, out=first[1:])
-        self._first_chunk = first
+        self._first_chunk = (ctypes.c_int64 * len(first))(*first.tolist())
         table = (_lib.AdamWTensor * len(items))()
         for i, (t, v) in enumerate(zip(table, items)):
             w, master = self.tensors[i], self.masters[i]
