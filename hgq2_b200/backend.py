@@ -16,6 +16,7 @@ that also applies constraints and regularizers the way Keras' trainer does.
 
 from __future__ import annotations
 
+import itertools
 import math
 import threading
 from collections.abc import Callable, Sequence
@@ -277,10 +278,11 @@ class _CallContext(threading.local):
         self.depth = 0
         self.training = None
         self.root = None
-        self.pass_id = 0  # number of the current top-level call: per-pass memos (rounded bitwidths) are keyed on it
+        self.pass_id = 0  # number of the current top-level call, its own in all threads: per-pass memos (rounded bitwidths) are keyed on it
 
 
 _ctx = _CallContext()
+_pass_numbers = itertools.count(1)
 
 
 class Layer(nn.Module):
@@ -384,7 +386,7 @@ class Layer(nn.Module):
         training = _ctx.training
         if top:
             _ctx.root = self
-            _ctx.pass_id += 1
+            _ctx.pass_id = next(_pass_numbers)
             self._losses = []
         if _accepts_training(self):
             kwargs['training'] = training

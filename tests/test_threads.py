@@ -146,3 +146,22 @@ def test_one_layer_serves_two_lengths_at_once():
     torch.cuda.synchronize()
     assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
     assert torch.equal(layer(x, training=False)[0], want[2])
+
+
+def test_passes_of_different_threads_have_different_numbers():
+    """What a quantizer remembers of a pass is for that pass alone: one thread's must not be taken for another's, whose stream may
+    not have computed it yet."""
+    from hgq2_b200 import backend
+
+    class Probe(backend.Layer):
+        def call(self, inputs):
+            return backend.current_pass()
+
+    layer, ready = Probe(), threading.Barrier(2)
+
+    def passes():
+        ready.wait(60)
+        return [layer(torch.zeros(1)) for _ in range(5)]
+
+    a, b = in_threads(passes, passes)
+    assert len(set(a)) == len(set(b)) == 5 and not set(a) & set(b)
