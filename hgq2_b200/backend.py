@@ -233,20 +233,20 @@ def queue_params(layers) -> None:
         prep = getattr(layer, 'prepare_params', None)
         if prep is not None and layer.built:
             with bookkeeping():
-                layer._prepared = prep()
-                layer._prepared_event = torch.cuda.Event()
-                layer._prepared_event.record()
+                params, event = prep(), torch.cuda.Event()
+                event.record()
+            _ctx.prepared[id(layer)] = params, event
 
 
 def take_prepared(layer):
     """The (quantised kernel, quantised bias) a ``Sequential`` queued ahead for this call of ``layer``, or None.  The current
     stream is made to wait for them."""
-    p = getattr(layer, '_prepared', None)
-    if p is None:
+    queued = _ctx.prepared.pop(id(layer), None)
+    if queued is None:
         return None
-    layer._prepared = None
+    p, event = queued
     main = torch.cuda.current_stream()
-    main.wait_event(layer._prepared_event)
+    main.wait_event(event)
     for t in p:
         if t is not None:
             t.record_stream(main)
@@ -279,6 +279,7 @@ class _CallContext(threading.local):
         self.training = None
         self.root = None
         self.pass_id = 0  # number of the current top-level call, its own in all threads: per-pass memos (rounded bitwidths) are keyed on it
+        self.prepared = {}  # parameters queued ahead in this call, by the layer's id: none outlives it (a call may fail halfway)
 
 
 _ctx = _CallContext()
@@ -403,6 +404,7 @@ class Layer(nn.Module):
             _ctx.training = prev_training
             if top:
                 _ctx.root = None
+                _ctx.prepared.clear()
 
     def call(self, *args, **kwargs):
         raise NotImplementedError

@@ -165,3 +165,29 @@ def test_passes_of_different_threads_have_different_numbers():
 
     a, b = in_threads(passes, passes)
     assert len(set(a)) == len(set(b)) == 5 and not set(a) & set(b)
+
+
+def two_layers():
+    from hgq2_b200.backend import Sequential
+    from hgq2_b200.config import QuantizerConfigScope
+    from hgq2_b200.layers import QDense
+
+    with QuantizerConfigScope(place='all', default_q_type='kif', f0=6), QuantizerConfigScope(place='datalane', i0=3):
+        model = Sequential([QDense(8), QDense(4)])
+    x = torch.randn(16, 6, device='cuda')
+    model(x)
+    return model, x
+
+
+@gpu
+def test_parameters_queued_by_a_pass_that_fails_are_dropped():
+    """A training pass that raises in its first layer has queued the second layer's quantised kernel: a later pass must not use it."""
+    model, x = two_layers()
+    first, second = model.layers
+    wrong = torch.randn(16, 7, device='cuda')
+    with pytest.raises(Exception):  # noqa: B017 -- whatever the shape mismatch raises
+        model(wrong, training=True)
+    second._kernel.assign(second.kernel * 0.0)
+    y = model(x, training=False)
+    assert torch.equal(y, second(first(x, training=False), training=False))
+    assert torch.equal(y, model(x, training=False))
