@@ -278,8 +278,13 @@ class FusedAdamW:
         for k, a in own.items():
             if tuple(state[k].shape) != tuple(a.shape):
                 raise ValueError(f'{k} has shape {tuple(state[k].shape)}, expected {tuple(a.shape)}')
+            if a.dtype == torch.float8_e4m3fn and state[k].dtype not in (torch.uint8, a.dtype):  # bytes, never numbers to round again
+                raise ValueError(f'{k} holds e4m3 codes (bytes), got {state[k].dtype}')
         for k, a in own.items():
-            (a.view(torch.uint8) if a.dtype == torch.float8_e4m3fn else a).copy_(state[k])
+            if a.dtype == torch.float8_e4m3fn:
+                a.view(torch.uint8).copy_(state[k].view(torch.uint8))
+            else:
+                a.copy_(state[k])
 
 
 class PeerExchange:

@@ -612,3 +612,19 @@ def test_states_past_32_bits(bits, clip):
                 place = torch.arange(blocks.start * 256, blocks.stop * 256, device='cuda').view(-1, 256)
                 code, top = reference_codes(exact, place, 1, root)
                 assert torch.equal(codes[p].float(), code.float().view(-1)[:x.numel()]) and torch.equal(s, top)
+
+
+@gpu
+def test_codes_are_loaded_as_bytes():
+    """e4m3 codes given as e4m3 tensors are the same bytes; as numbers of another type they are refused, and nothing is taken over."""
+    from hgq2_b200.train import FusedAdamW
+
+    gen = torch.Generator(device='cuda').manual_seed(13)
+    a, b = (FusedAdamW([torch.zeros(700, device='cuda')], state_bits=8) for _ in range(2))
+    set_state(a, gen)
+    state = a.state_dict()
+    with pytest.raises(ValueError, match='codes'):
+        b.load_state_dict({**state, 'm': a.m.float()})
+    assert not bool(b.m.float().any()) and not bool(b.m_scale.any())
+    b.load_state_dict({**state, 'm': a.m.clone(), 'r': a.r.clone()})
+    assert all(torch.equal(v, b.state_dict()[k]) for k, v in state.items())
