@@ -20,9 +20,11 @@
 // to step, travel in the kernel's parameters, so a step copies nothing to the device and a captured graph keeps its own.
 //
 // What bounds it (B200, 6.57 TB/s copy).  32 bits: memory, 28 bytes an element: 30 M elements in 320 tensors 0.124 ms = 6.7 TB/s, with
-// the norm's pass over the gradients (0.030 ms) 0.157 ms.  8 bits: arithmetic and latency, about 80 instructions an element (an
-// IEEE root, two dithered codes and their mix are half of them; 37 go to the half-rate integer pipe) against 14 to 16 bytes: 49 M
-// elements with bf16 gradients 0.19 ms = 0.55 of the copy rate, 299 M with clipping 1.27 ms.  Tried and left out, same two cases:
+// the norm's pass over the gradients (0.030 ms) 0.157 ms.  8 bits: latency before anything else.  About 80 instructions an
+// element (an IEEE root, two dithered codes and their mix are half of them; 37 go to the half-rate integer pipe) against 14 to 16
+// bytes fill 58 % of the issue slots and 45 % of the integer pipe; a warp loads a block, reduces, divides, encodes and stores with
+// nothing of its next block on the way, and 80 registers (16 bytes of them spilled) leave 36 % of the warps: the first stall is the
+// loads'.  49 M elements with bf16 gradients 0.19 ms = 0.55 of the copy rate, 299 M with clipping 1.24 to 1.29 ms.  Tried and left out, same two cases:
 // the next block copied ahead into shared memory (0.20 ms, 1.62 ms: its copies cost more issue slots than the latency they hide),
 // prefetches to L2 (0.185, 1.28), four CTAs an SM at 64 registers (0.18, 1.31: spills), neighbouring chunks to one CTA
 // instead of every grid-th (0.19, 1.33).

@@ -12,8 +12,10 @@
 //
 // This file: the entries, and the kernels for samples that do not fit on chip (the others are in groupnorm_slab.cu).  Those read
 // twice: partial statistics per channel of runs of rows, totals in fp64, then the application, in groups of samples small enough
-// that the second read finds them in L2.  Bound by latency and by the activation's arithmetic more than by memory: [6, 255, 257, 96]
-// bf16 with SiLU 0.066 ms forward and 0.124 ms backward (75 MB a tensor).  One wave of CTAs: two more than the SMs hold
+// that the second read finds them in L2.  Bound by latency: a thread loads 4 to 8 packs and then computes with
+// nothing on the way, which fills 34 to 42 % of the DRAM rate and 42 to 46 % of the issue slots at 22 to 34 % of the warps (k_gn_stats of
+// 16-byte packs of 16-bit types also spills 20 bytes at its 80 registers).  [6, 255, 257, 96] bf16 with SiLU 0.066 ms forward and 0.124 ms
+// backward (75 MB a tensor).  One wave of CTAs: two more than the SMs hold
 // at once made the backward pass 0.160 ms.
 #include "groupnorm.cuh"
 

@@ -16,7 +16,8 @@
 // one's totals are taken.  Backward: du gamma in registers leaves two CTAs an SM, 0.175 and 0.089 ms for the fp32 shapes (0.62 and
 // 0.69).  Two CTAs share a sample that one cannot hold; four or eight wait for one another longer than the second read of the other
 // kernels takes ([256, 1024, 128] bf16: 0.104 ms with eight, 0.062 with two or none).  x staged in shared memory for its second use
-// in the backward pass made the registers spill (0.187 -> 0.189 ms) and was left out.
+// in the backward pass made the registers spill more (0.187 -> 0.189 ms) and was left out.  As it is, 53 of the 144 variants spill, most of
+// them those with a number a channel (packs that groups do not nest with; up to 224 bytes, fp32 backward) and those of narrow packs.
 #include <cooperative_groups.h>
 
 #include "groupnorm.cuh"

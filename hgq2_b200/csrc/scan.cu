@@ -22,7 +22,9 @@
 //
 // What bounds it (B200, 6.57 TB/s copy): fp32, memory: [8192, 64, 64] 0.075 ms forward and 0.115 ms backward (0.82 and 0.88 of the copy
 // rate for 3 and 5 tensors), [64, 2048, 256] 0.074 and 0.118 ms (0.83, 0.86).  bf16 / fp16: issue slots, 24 to 38 instructions an
-// element and pass at half the bytes: [2, 65521, 256] bf16 0.201 ms for both passes in their two launches each.  What the steps
+// element and pass at half the bytes: [2, 65521, 256] bf16 0.201 ms for both passes in their two launches each.  Padded rows of
+// an odd length, [96, 1999, 321] fp16, 0.138 ms forward: issue slots too, 50 instructions an element, half of them for steps behind the
+// rows' ends, which are computed like live ones, and accesses of 2 bytes.  What the steps
 // gave: expf, IEEE division and a 64-bit multiply per address took 93 instructions an element (0.149 ms for the forward pass of
 // [8192, 64, 64]); the gates in fast_sigmoid.cuh, running pointers, two channels a lane and no predicates in full runs 47 (0.070);
 // tiles fetched ahead 0.315 -> 0.261 ms for the long bf16 case with a lane's own 4 bytes a copy, 0.201 with 16-byte pieces.

@@ -877,7 +877,8 @@ def gated_scan_fwd(x, z, h0=None, lengths=None, want_states: bool = False):
 def gated_scan_bwd(gh, x, z, h0=None, lengths=None, states=None, g_last=None, want_dh0: bool = False, out_dx=None,
                    out_dz=None):
     """Gradients of ``gated_scan_fwd`` from the gradients ``gh`` of h and ``g_last`` of h_last (None: zeros): (dx, dz, dh0 or None);
-    dx and dz go to ``out_dx`` / ``out_dz`` when given (like x, the features contiguous, any other strides that keep rows apart)."""
+    dx and dz go to ``out_dx`` / ``out_dz`` when given (like x, the features contiguous, any other strides that keep rows apart;
+    not over any input)."""
     x, z, h0, lengths, kind, B, T, D = _scan_args(x, z, h0, lengths)
     require_cuda(gh, states, g_last)
     if gh is not None:

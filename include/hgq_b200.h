@@ -418,6 +418,8 @@ int hgq_adam_step(float *w, const float *g, float *m, float *v, const float *lo,
                   float grad_scale, long long *step, void *stream);
 
 /* ---- element types of the entries that take more than fp32 -------------------------------- */
+/* A call of the entries below may be several launches that meet in its workspace: calls that can run, or be queued on one stream, at the
+ * same time (from several host threads) need workspaces of their own. */
 #define HGQ_TYPE_F32 0
 #define HGQ_TYPE_BF16 1
 #define HGQ_TYPE_F16 2
@@ -453,7 +455,7 @@ typedef struct {
  * v_scale have one entry per 256 state elements, and a code stands for code * scale.  The rounding is dithered by a fixed
  * function of the element's place and t, so steps repeat bit for bit.  A state that is not finite is kept as NaN.
  * step: device counter (starts at 0), advanced by the call; ticket: a device word that starts at 0 and returns to 0.  Calls that
- * share states must not overlap.  workspace: hgq_adamw_workspace(n_tensors) bytes, needed when clipnorm > 0.
+ * share states must not overlap.  m_scale, v_scale and ticket are aligned to 4 bytes.  workspace: hgq_adamw_workspace(n_tensors) bytes, needed when clipnorm > 0.
  */
 size_t hgq_adamw_workspace(int64_t n_tensors);
 int hgq_adamw_step(const hgq_adamw_tensor *tensors, int64_t n_tensors, const int32_t *chunks, const int64_t *first_chunk,
